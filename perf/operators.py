@@ -253,7 +253,7 @@ def _prepare_verify(case, g):
     st["seq"] = seq
     if own:
         be = _be()
-        st["ws"] = be.verify_draft_workspace(len(rows), n, v)
+        st["ws"] = be.verify_draft_workspace(n, v)
     return st
 
 
