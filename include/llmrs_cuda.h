@@ -50,7 +50,8 @@ extern "C" {
 #define LLMRS_EDEVICE 7    /* device-side error word set (bad token id, bad position) */
 
 /* ---- dtypes: block scales (LLMRS_F16 / LLMRS_F32); raw checkpoint tensors
- *      of llmrs_model_load_weight (LLMRS_F32 / LLMRS_BF16) ---- */
+ *      of llmrs_model_load_weight (LLMRS_F32 / LLMRS_BF16); rows of the
+ *      llmrs_kv8_* and llmrs_verify_* calls (all three) ---- */
 #define LLMRS_F16 0
 #define LLMRS_F32 1
 #define LLMRS_BF16 2
@@ -187,6 +188,101 @@ int llmrs_rms_norm_quantize_q8_0(llmrs_ctx *ctx, const float *d_x, const float *
 /* Tensor::quantize_q4 (src/core/tensor.rs:102-167): n values -> planar nibbles
  * [(n+1)/2] and f32 scales [(n+31)/32]; bit-exact */
 int llmrs_quantize_q4(llmrs_ctx *ctx, const float *d_w, size_t n, uint8_t *d_qs, float *d_scales);
+
+/* ======================================================================
+ * Paged 8-bit KV cache: the cache of a batch of sequences.  No counterpart in
+ * the reference (one sequence, contiguous f32 cache, src/core/layer.rs:114-128).
+ *
+ * Keys and values are int8 codes with one f32 scale for each (page, KV head);
+ * a cached value is code * scale.  The caller owns every buffer.  All calls run
+ * on the context's stream on the context's device; none of them synchronises,
+ * and with a workspace of the caller's none allocates, so they can be captured
+ * into CUDA graphs (graphs that may run at the same time need a workspace
+ * each).  Arrays named d_* are read when the work runs, not when the call is
+ * made.  Numbers in them that lead outside the buffers are skipped and reported
+ * by the next llmrs_sync (LLMRS_EDEVICE): a sequence whose rows or length do
+ * not fit counts as having no rows, tokens of a page id outside the pool are
+ * left out.
+ * ====================================================================== */
+typedef struct {
+    int8_t *d_k_codes, *d_v_codes; /* [n_pages][n_kv_heads][page_size][head_dim], 16-byte aligned */
+    float *d_k_scales, *d_v_scales; /* [n_pages][n_kv_heads] */
+    int n_pages;
+    int page_size;                 /* tokens of a page: 16, 32, 64 or 128 */
+    int n_kv_heads, head_dim;      /* head_dim 64 or 128 */
+} llmrs_kv8;
+
+/* The new rows of n_seqs sequences, packed: sequence s owns rows
+ * [d_row_start[s], d_row_start[s+1]) (none, one or many; rows behind the last
+ * sequence's belong to nobody and are neither read nor written) and has
+ * d_lens[s] tokens in the cache in front of them, so its row i stands at
+ * position d_lens[s] + i.  d_page_table[s][p] is the pool page of positions
+ * [p*page_size, (p+1)*page_size); entries behind the last needed one are not
+ * read.  Sequences may share pages in front of their new rows; a page that a
+ * call writes must belong to one sequence. */
+typedef struct {
+    int n_seqs;
+    const int *d_row_start;  /* [n_seqs + 1] */
+    const int *d_lens;       /* [n_seqs] */
+    const int *d_page_table; /* [n_seqs][max_pages] */
+    int max_pages;
+} llmrs_kv8_batch;
+
+/* Append the batch's rows to the cache.  d_k / d_v: rows of n_kv_heads*head_dim
+ * elements of dtype (LLMRS_F32, LLMRS_BF16 or LLMRS_F16), ld elements apart (so
+ * they may lie inside packed q|k|v rows), each row on a 16-byte boundary; n_rows
+ * rows at least up to d_row_start[n_seqs].  Keys are rotated by their positions
+ * with the tables of llmrs_rope_table ([n_pos][head_dim/2]; NULL tables: not
+ * rotated; a row whose position is past n_pos is an error of its sequence).
+ * A page's scale becomes max(its scale, largest new magnitude / 127), the new
+ * codes are rint(x * (1/scale)), and codes that the page's older tokens had are
+ * rounded again when the scale grew; a scale below 2^-126 is zero.  What an
+ * unused page held before does not matter.  An infinite or NaN value is stored
+ * as zero and reported by llmrs_sync. */
+int llmrs_kv8_append(llmrs_ctx *ctx, const llmrs_kv8 *cache, const llmrs_kv8_batch *batch, const void *d_k,
+                     const void *d_v, int dtype, long long ld, int n_rows, const float *d_rope_cos,
+                     const float *d_rope_sin, int n_pos);
+/* Pages back as values: d_k, d_v [n][n_kv_heads][page_size][head_dim] of dtype */
+int llmrs_kv8_read(llmrs_ctx *ctx, const llmrs_kv8 *cache, const int *d_pages, int n, void *d_k, void *d_v, int dtype);
+/* Causal attention of the batch's rows over the cache, after llmrs_kv8_append of
+ * the same batch: row i of sequence s attends to its positions
+ * [0, d_lens[s] + i].  d_q, d_out: rows of n_heads*head_dim elements of dtype,
+ * ld_q / ld_out elements apart, on 16-byte boundaries; query head h reads KV
+ * head h / (n_heads/n_kv_heads), any whole ratio.  q is rotated on the way (NULL
+ * tables: it is not).  scale multiplies q.k (0: 1/sqrt(head_dim)).  f32 rows are
+ * computed to f32 accuracy, 16-bit rows to that of their type.  A row for which
+ * no page can be read gets zeros.  d_workspace: llmrs_kv8_attention_workspace
+ * bytes (which depend on the sizes only), 16-byte aligned, contents irrelevant; NULL: the
+ * context's scratch (not while capturing). */
+int llmrs_kv8_attention_workspace(const llmrs_kv8 *cache, const llmrs_kv8_batch *batch, int n_heads, int n_rows,
+                                  size_t *bytes);
+int llmrs_kv8_attention(llmrs_ctx *ctx, const llmrs_kv8 *cache, const llmrs_kv8_batch *batch, const void *d_q,
+                        long long ld_q, void *d_out, long long ld_out, int dtype, int n_rows, int n_heads,
+                        const float *d_rope_cos, const float *d_rope_sin, int n_pos, float scale, void *d_workspace,
+                        size_t workspace_bytes);
+
+/* Verify drafted tokens.  Sequence s has rows [d_row_start[s], d_row_start[s+1])
+ * of target logits: one for each of its drafts and one behind them (one row:
+ * plain sampling; no rows: nothing but d_accepted[s] = 0).  d_draft_tokens holds
+ * the drafts of all sequences packed (one fewer than the rows of each sequence
+ * that has rows), d_draft_probs [drafts][ld_probs] the f32 distributions they
+ * were drawn from (NULL: each draft was certain, e.g. found by lookup).  With
+ * p = softmax(logits / temperature), draft i is accepted while
+ *   u[row i] * q_i(d_i) < p_i(d_i),
+ * and the next token is drawn with u[last row] from max(p - q, 0) of the first
+ * rejected draft's row (from p where nothing is left over), or from the last
+ * row's p when all were accepted: the first token, in index order, whose running
+ * sum exceeds u times the total (64-bit sums).  d_temperature [n_seqs] (NULL: 1);
+ * 0 takes the first most likely token.  -inf (and NaN) logits have no weight; a row
+ * without any yields token -1 and accepts nothing.  A draft outside the vocabulary is
+ * rejected and reported by llmrs_sync.  Out: d_tokens[rows] the accepted drafts,
+ * then the next token, then -1; d_accepted[n_seqs]; d_token_probs[rows] (may be
+ * NULL) p of each token given out, 0 behind them. */
+int llmrs_verify_draft_workspace(int n_rows, int vocab, size_t *bytes);
+int llmrs_verify_draft(llmrs_ctx *ctx, const void *d_logits, long long ld_logits, int dtype, int vocab, int n_rows,
+                       int n_seqs, const int *d_row_start, const int *d_draft_tokens, const float *d_draft_probs,
+                       long long ld_probs, const float *d_uniforms, const float *d_temperature, int *d_tokens,
+                       int *d_accepted, float *d_token_probs, void *d_workspace, size_t workspace_bytes);
 
 /* ======================================================================
  * Model: device-resident weights + KV cache, fused decode step

@@ -43,6 +43,8 @@ EXPORTS = [
     "llmrs_model_profile_decode", "llmrs_time_gemv",
     "llmrs_attention_decode", "llmrs_attention_decode_noalloc", "llmrs_attention_prefill",
     "llmrs_sample", "llmrs_model_sample", "llmrs_model_trace_decode",
+    "llmrs_kv8_append", "llmrs_kv8_read", "llmrs_kv8_attention", "llmrs_kv8_attention_workspace",
+    "llmrs_verify_draft", "llmrs_verify_draft_workspace",
     "llmrs_model_tp_region", "llmrs_model_tp_connect", "llmrs_ipc_get_handle", "llmrs_ipc_open_handle",
     "llmrs_ipc_close_handle", "llmrs_model_set_peer_timeout", "llmrs_model_tp_epoch", "llmrs_model_tp_resync",
 ]
@@ -66,6 +68,23 @@ class Config(ctypes.Structure):
     ]
 
 
+class Kv8Struct(ctypes.Structure):
+    """llmrs_kv8"""
+    _fields_ = [
+        ("d_k_codes", ctypes.c_void_p), ("d_v_codes", ctypes.c_void_p), ("d_k_scales", ctypes.c_void_p),
+        ("d_v_scales", ctypes.c_void_p), ("n_pages", ctypes.c_int), ("page_size", ctypes.c_int),
+        ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+    ]
+
+
+class Kv8BatchStruct(ctypes.Structure):
+    """llmrs_kv8_batch"""
+    _fields_ = [
+        ("n_seqs", ctypes.c_int), ("d_row_start", ctypes.c_void_p), ("d_lens", ctypes.c_void_p),
+        ("d_page_table", ctypes.c_void_p), ("max_pages", ctypes.c_int),
+    ]
+
+
 _lib = None
 
 
@@ -79,6 +98,7 @@ def lib():
                           "(or __graft_entry__.build())")
     L = ctypes.CDLL(LIB_PATH)
     vp, sz, ci, cf = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_float
+    cl = ctypes.c_longlong
     pp = ctypes.POINTER(ctypes.c_void_p)
     ip = ctypes.POINTER(ctypes.c_int)
     fp = ctypes.POINTER(ctypes.c_float)
@@ -137,6 +157,12 @@ def lib():
         "llmrs_model_sample": (ci, [vp, vp, ci, cf, cf, cf, cf, ip]),
         "llmrs_attention_decode_noalloc": (ci, [vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp]),
         "llmrs_model_trace_decode": (ci, [vp, ci, ci, vp, vp, ip]),
+        "llmrs_kv8_append": (ci, [vp, vp, vp, vp, vp, ci, cl, ci, vp, vp, ci]),
+        "llmrs_kv8_read": (ci, [vp, vp, vp, ci, vp, vp, ci]),
+        "llmrs_kv8_attention_workspace": (ci, [vp, vp, ci, ci, ctypes.POINTER(sz)]),
+        "llmrs_kv8_attention": (ci, [vp, vp, vp, vp, cl, vp, cl, ci, ci, ci, vp, vp, ci, cf, vp, sz]),
+        "llmrs_verify_draft_workspace": (ci, [ci, ci, ctypes.POINTER(sz)]),
+        "llmrs_verify_draft": (ci, [vp, vp, cl, ci, ci, ci, ci, vp, vp, vp, cl, vp, vp, vp, vp, vp, vp, sz]),
         "llmrs_model_tp_region": (ci, [vp, pp, ctypes.POINTER(sz)]),
         "llmrs_model_tp_connect": (ci, [vp, pp]),
         "llmrs_ipc_get_handle": (ci, [vp, vp]),
@@ -209,6 +235,12 @@ class Context:
     def sync(self):
         check(lib().llmrs_sync(self.h))
 
+    def set_stream(self, cuda_stream):
+        """Run on a cudaStream_t of the caller's (an int, e.g. torch's
+        `stream.cuda_stream`; 0, the default stream, by its name
+        cudaStreamLegacy); None goes back to the context's own stream."""
+        check(lib().llmrs_ctx_set_stream(self.h, 1 if cuda_stream == 0 else cuda_stream))
+
 
 class DeviceTensor:
     """Device buffer with a numpy dtype and shape (the reference's Tensor on Device::Cuda)."""
@@ -266,6 +298,104 @@ class QuantWeight:
         else:
             scales = np.asarray(scales, np.float32)
         self.scales = DeviceTensor.from_numpy(ctx, scales)
+
+
+# element types of device arrays: DeviceTensor's numpy dtypes (bfloat16 as its
+# uint16 bits), and torch's by name
+_DTYPES = {np.dtype(np.float32): F32, np.dtype(np.float16): F16, np.dtype(np.uint16): BF16,
+           "torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
+_INT32 = (np.dtype(np.int32), "torch.int32")
+_INT8 = (np.dtype(np.int8), "torch.int8")
+_F32 = (np.dtype(np.float32), "torch.float32")
+
+
+def _address(x):
+    """Device address of a DeviceTensor, or of a torch tensor (anything with data_ptr())."""
+    return x.ptr.value if isinstance(x, DeviceTensor) else x.data_ptr()
+
+
+def _type(x):
+    return x.dtype if isinstance(x, DeviceTensor) else str(x.dtype)
+
+
+def _array(x, types, what):
+    """Address of a contiguous array of one of `types`."""
+    if _type(x) not in types:
+        raise TypeError("%s: dtype %s" % (what, x.dtype))
+    if not isinstance(x, DeviceTensor) and not x.is_contiguous():
+        raise ValueError("%s must be contiguous" % what)
+    return _address(x)
+
+
+def _rows(x, width, what):
+    """(address, dtype code, rows, row stride) of rows of `width` elements: [n, width]
+    or [n, heads, D], the elements of a row next to each other."""
+    t = _type(x)
+    if t not in _DTYPES:
+        raise TypeError("%s: dtype %s" % (what, x.dtype))
+    n, size = x.shape[0], 1
+    for s in x.shape[1:]:
+        size *= s
+    if size != width:
+        raise ValueError("%s: rows of %d elements, not %d" % (what, size, width))
+    if isinstance(x, DeviceTensor):
+        return x.ptr.value, _DTYPES[t], n, width
+    strides, inner = x.stride(), 1
+    for s, st in zip(reversed(x.shape[1:]), reversed(strides[1:])):
+        if s != 1 and st != inner:
+            raise ValueError("%s: the elements of a row must lie next to each other" % what)
+        inner *= s
+    return x.data_ptr(), _DTYPES[t], n, strides[0] if n > 1 else max(strides[0], width)
+
+
+class Kv8Cache:
+    """Paged 8-bit KV cache (llmrs_kv8): int8 codes [n_pages, n_kv_heads, page_size,
+    head_dim] and f32 scales [n_pages, n_kv_heads] for keys and values.  Allocates
+    its pools unless they are given (DeviceTensors or torch tensors)."""
+
+    def __init__(self, ctx, n_pages, page_size, n_kv_heads, head_dim, k_codes=None, v_codes=None, k_scales=None,
+                 v_scales=None):
+        codes, scales = (n_pages, n_kv_heads, page_size, head_dim), (n_pages, n_kv_heads)
+        self.ctx, self.shape = ctx, codes
+        self.k_codes = DeviceTensor(ctx, codes, np.int8) if k_codes is None else k_codes
+        self.v_codes = DeviceTensor(ctx, codes, np.int8) if v_codes is None else v_codes
+        self.k_scales = DeviceTensor(ctx, scales) if k_scales is None else k_scales
+        self.v_scales = DeviceTensor(ctx, scales) if v_scales is None else v_scales
+        for x, shape in ((self.k_codes, codes), (self.v_codes, codes), (self.k_scales, scales),
+                         (self.v_scales, scales)):
+            if tuple(x.shape) != shape:
+                raise ValueError("Kv8Cache: pool of shape %s, not %s" % (tuple(x.shape), shape))
+        self.struct = Kv8Struct(_array(self.k_codes, _INT8, "k_codes"), _array(self.v_codes, _INT8, "v_codes"),
+                                _array(self.k_scales, _F32, "k_scales"), _array(self.v_scales, _F32, "v_scales"),
+                                n_pages, page_size, n_kv_heads, head_dim)
+        self._ref = ctypes.addressof(self.struct)
+
+
+class SeqBatch:
+    """The new rows of a batch of sequences (llmrs_kv8_batch): int32 device arrays
+    row_start [n+1], lens [n] (cached tokens in front of the rows), page_table
+    [n, max_pages].  Their contents may change between calls."""
+
+    def __init__(self, row_start, lens, page_table):
+        n = lens.shape[0]
+        if tuple(row_start.shape) != (n + 1,) or len(page_table.shape) != 2 or page_table.shape[0] != n:
+            raise ValueError("SeqBatch: row_start %s, lens %s, page_table %s" % (
+                tuple(row_start.shape), tuple(lens.shape), tuple(page_table.shape)))
+        self.row_start, self.lens, self.page_table, self.n_seqs = row_start, lens, page_table, n
+        self.struct = Kv8BatchStruct(n, _array(row_start, _INT32, "row_start"), _array(lens, _INT32, "lens"),
+                                     _array(page_table, _INT32, "page_table"), page_table.shape[1])
+        self._ref = ctypes.addressof(self.struct)
+
+
+def _rope(cos, sin, head_dim):
+    """(cos address, sin address, rows) of the rotation tables, or none."""
+    if cos is None and sin is None:
+        return None, None, 0
+    if cos is None or sin is None:
+        raise ValueError("rope tables: both or neither")
+    if tuple(cos.shape) != tuple(sin.shape) or len(cos.shape) != 2 or cos.shape[1] != head_dim // 2:
+        raise ValueError("rope tables: shapes %s, %s" % (tuple(cos.shape), tuple(sin.shape)))
+    return _array(cos, _F32, "rope_cos"), _array(sin, _F32, "rope_sin"), cos.shape[0]
 
 
 class CudaBackend:
@@ -378,6 +508,95 @@ class CudaBackend:
                                  int(r.size), float(repeat_penalty), float(temperature), float(top_p), float(u),
                                  ctypes.byref(tok)))
         return tok.value
+
+    # ---- paged 8-bit KV cache and drafts: the rows and outputs may be DeviceTensors
+    # or torch tensors, on any GPU memory of the context's device
+    def kv8_append(self, cache, batch, k, v, rope_cos=None, rope_sin=None):
+        """Append the batch's new rows (k, v: [n, n_kv_heads*head_dim], strided rows allowed)."""
+        _, kv, _, d = cache.shape
+        kp, kt, kn, kld = _rows(k, kv * d, "k")
+        vp, vt, vn, vld = _rows(v, kv * d, "v")
+        if kt != vt or kn != vn or (kld != vld and kn > 1):
+            raise ValueError("kv8_append: k and v must agree in dtype, rows and row stride")
+        cp, sp, n_pos = _rope(rope_cos, rope_sin, d)
+        check(lib().llmrs_kv8_append(self.ctx.h, cache._ref, batch._ref, kp, vp, kt, kld, kn, cp, sp, n_pos))
+
+    def kv8_read(self, cache, pages, k_out, v_out):
+        """The values of `pages` (int32 [n]) into k_out, v_out [n, n_kv_heads, page_size, head_dim]."""
+        n = pages.shape[0]
+        shape = (n,) + cache.shape[1:]
+        if tuple(k_out.shape) != shape or tuple(v_out.shape) != shape or _type(k_out) != _type(v_out):
+            raise ValueError("kv8_read: outputs must be two arrays of shape %s" % (shape,))
+        check(lib().llmrs_kv8_read(self.ctx.h, cache._ref, _array(pages, _INT32, "pages"), n,
+                                   _array(k_out, _DTYPES, "k_out"), _array(v_out, _DTYPES, "v_out"),
+                                   _DTYPES[_type(k_out)]))
+
+    def kv8_attention_workspace(self, cache, batch, n_heads, n_rows):
+        """A workspace for kv8_attention of this many heads and rows (one call at a time)."""
+        n = ctypes.c_size_t(0)
+        check(lib().llmrs_kv8_attention_workspace(cache._ref, batch._ref, int(n_heads), int(n_rows), ctypes.byref(n)))
+        return DeviceTensor(self.ctx, (n.value,), np.uint8)
+
+    def kv8_attention(self, cache, batch, q, out=None, rope_cos=None, rope_sin=None, scale=None, workspace=None):
+        """Causal attention of the batch's rows q [n, n_heads*head_dim] over the cache,
+        after kv8_append of the same batch; writes and returns `out`."""
+        d = cache.shape[3]
+        width = 1
+        for s in q.shape[1:]:
+            width *= s
+        n_heads = width // d
+        if n_heads * d != width:
+            raise ValueError("kv8_attention: q rows of %d elements are no heads of %d" % (width, d))
+        if out is None:
+            out = DeviceTensor(self.ctx, tuple(q.shape), {F32: np.float32, F16: np.float16, BF16: np.uint16}[
+                _rows(q, width, "q")[1]])
+        qp, qt, qn, qld = _rows(q, width, "q")
+        op, ot, on, old = _rows(out, width, "out")
+        if qt != ot or qn != on:
+            raise ValueError("kv8_attention: q and out must agree in dtype and rows")
+        cp, sp, n_pos = _rope(rope_cos, rope_sin, d)
+        check(lib().llmrs_kv8_attention(self.ctx.h, cache._ref, batch._ref, qp, qld, op, old, qt, qn, n_heads, cp, sp,
+                                        n_pos, 0.0 if scale is None else float(scale),
+                                        None if workspace is None else _address(workspace),
+                                        0 if workspace is None else workspace.nbytes))
+        return out
+
+    def verify_draft_workspace(self, n_rows, vocab):
+        """A workspace for verify_draft of this many logits rows (one call at a time)."""
+        n = ctypes.c_size_t(0)
+        check(lib().llmrs_verify_draft_workspace(int(n_rows), int(vocab), ctypes.byref(n)))
+        return DeviceTensor(self.ctx, (max(16, n.value),), np.uint8)
+
+    def verify_draft(self, logits, row_start, draft_tokens, draft_probs, uniforms, tokens, accepted, token_probs=None,
+                     temperature=None, workspace=None):
+        """Verify drafted tokens (llmrs_verify_draft): logits [n, vocab]; row_start int32
+        [seqs+1]; draft_tokens int32 and draft_probs f32 [drafts, vocab] (or None: certain
+        drafts), packed; uniforms f32 [n].  Writes tokens int32 [n], accepted int32
+        [seqs] and token_probs f32 [n]."""
+        vocab, n_seqs = logits.shape[1], row_start.shape[0] - 1
+        lp, lt, n, ld = _rows(logits, vocab, "logits")
+        qp, qld = None, 0
+        if draft_probs is not None and draft_probs.shape[0]:
+            qp, qt, qn, qld = _rows(draft_probs, vocab, "draft_probs")
+            if qt != F32:
+                raise TypeError("draft_probs: dtype %s" % draft_probs.dtype)
+            if qn != draft_tokens.shape[0]:
+                raise ValueError("verify_draft: %d drafted tokens, %d distributions" % (draft_tokens.shape[0], qn))
+        if tuple(uniforms.shape) != (n,) or tuple(tokens.shape) != (n,) or tuple(accepted.shape) != (n_seqs,):
+            raise ValueError("verify_draft: uniforms and tokens must be [%d], accepted [%d]" % (n, n_seqs))
+        if token_probs is not None and tuple(token_probs.shape) != (n,):
+            raise ValueError("verify_draft: token_probs must be [%d]" % n)
+        if temperature is not None and tuple(temperature.shape) != (n_seqs,):
+            raise ValueError("verify_draft: temperature must be [%d]" % n_seqs)
+        some = draft_tokens is not None and draft_tokens.shape[0] > 0
+        check(lib().llmrs_verify_draft(
+            self.ctx.h, lp, ld, lt, vocab, n, n_seqs, _array(row_start, _INT32, "row_start"),
+            _array(draft_tokens, _INT32, "draft_tokens") if some else None, qp, qld,
+            _array(uniforms, _F32, "uniforms"),
+            None if temperature is None else _array(temperature, _F32, "temperature"),
+            _array(tokens, _INT32, "tokens"), _array(accepted, _INT32, "accepted"),
+            None if token_probs is None else _array(token_probs, _F32, "token_probs"),
+            None if workspace is None else _address(workspace), 0 if workspace is None else workspace.nbytes))
 
     # CpuBackend::quantize_row_q8_0 and Tensor::quantize_q4 (bit-exact)
     def quantize_row_q8_0(self, x):

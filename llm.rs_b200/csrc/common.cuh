@@ -51,6 +51,9 @@ enum : uint32_t {
     DEV_ERR_PEER_TIMEOUT = 2,
     DEV_ERR_BAD_TOKEN = 3,
     DEV_ERR_BAD_POS = 4,
+    DEV_ERR_BAD_BATCH = 5, // a sequence's rows or length lead outside the buffers
+    DEV_ERR_BAD_PAGE = 6,  // a page id outside the pool
+    DEV_ERR_NONFINITE = 7, // a key or value that cannot be held as a code
 };
 
 // launch a kernel; with pdl=true it may begin before the previous kernel in the

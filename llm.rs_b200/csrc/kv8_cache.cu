@@ -1,0 +1,224 @@
+// kv8_cache.cu - writing and reading the paged 8-bit KV cache (sm_100a).
+//
+// Append, for each page p and KV head that new rows fall into (x: the new
+// rows' values there, keys rotated by their positions first):
+//   s1   = max(s0, max|x| / 127)      s0 = 0 when the page held none of the
+//                                     sequence's tokens before; s1 < 2^-126 -> 0
+//   new  = rint(x * (1 / s1))         older codes c of the page, when s1 > s0:
+//                                     rint(c * (s0 / s1))
+// Every operation is one f32 rounding (no FMA), so the codes do not depend on
+// how the work is split.  No counterpart in the reference: its cache is f32
+// and contiguous (src/core/layer.rs:114-128, 219-246).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <float.h>
+
+#include <algorithm>
+
+#include "kv8.cuh"
+
+namespace llmrs {
+
+namespace {
+
+constexpr int AP_THREADS = 256;
+
+__device__ __forceinline__ float rot_lo(float lo, float hi, float c, float s)
+{
+    return __fsub_rn(__fmul_rn(lo, c), __fmul_rn(hi, s));
+}
+__device__ __forceinline__ float rot_hi(float lo, float hi, float c, float s)
+{
+    return __fadd_rn(__fmul_rn(lo, s), __fmul_rn(hi, c));
+}
+
+// a value that is no number, or infinite, is stored as zero and reported
+__device__ __forceinline__ float finite_or_zero(float x, bool &bad)
+{
+    if (fabsf(x) <= FLT_MAX)
+        return x;
+    bad = true;
+    return 0.0f;
+}
+
+__device__ __forceinline__ uint32_t code4(float4 x, float inv)
+{
+    const float v[4] = {x.x, x.y, x.z, x.w};
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float r = fminf(fmaxf(rintf(__fmul_rn(v[i], inv)), -127.0f), 127.0f);
+        w |= ((uint32_t)(int)r & 0xffu) << (8 * i);
+    }
+    return w;
+}
+
+// One CTA per (touched page, KV head, K or V).  Bound by reading the rows.
+template <class T, int D>
+__global__ void __launch_bounds__(AP_THREADS) kv8_append_kernel(Kv8 c, Kv8Batch b, const T *k, const T *v,
+                                                                long long ld, Kv8Rope rope, uint32_t *err)
+{
+    constexpr int TPR = D / 8;              // threads per row: dims 4j.. and D/2 + 4j..
+    constexpr int RPI = AP_THREADS / TPR;   // rows per round
+    __shared__ float s_max[AP_THREADS / 32];
+    const int page = c.page, g = blockIdx.y;
+    const bool is_v = blockIdx.z != 0;
+    long long within = 0;
+    const int s = kv8_find_unit<AP_THREADS>(
+        b.n_seqs, blockIdx.x,
+        [&](int i) -> long long {
+            int r0, n, len;
+            kv8_seq(b, i, err, r0, n, len);
+            return n ? (len + n - 1) / page - len / page + 1 : 0;
+        },
+        within);
+    if (s < 0)
+        return;
+    int r0, n, len;
+    kv8_seq(b, s, err, r0, n, len);
+    const int p = len / page + (int)within;
+    const int id = kv8_page(b, c, s, p, err);
+    if (id < 0)
+        return;
+    const int t0 = max(len, p * page), t1 = min(len + n, (p + 1) * page); // new positions in this page
+    const int held = t0 - p * page;                                      // older tokens in front of them
+    const T *src = (is_v ? v : k) + (size_t)(r0 + t0 - len) * ld + (size_t)g * D;
+    const size_t at = ((size_t)id * c.n_kv + g);
+    int8_t *codes = (is_v ? c.vq : c.kq) + at * page * D;
+    float *scale = (is_v ? c.vs : c.ks) + at;
+    const float s0 = held ? *scale : 0.0f;
+    const int j = threadIdx.x % TPR, rr = threadIdx.x / TPR;
+    const bool turn = !is_v && rope.cos;
+    bool bad = false;
+    auto row = [&](int i, float4 &lo, float4 &hi) { // new row i: 4 values of each half, rotated
+        const T *x = src + (size_t)i * ld;
+        lo = kv8_load4(x + 4 * j);
+        hi = kv8_load4(x + D / 2 + 4 * j);
+        if (turn) {
+            const size_t o = (size_t)(t0 + i) * (D / 2) + 4 * j;
+            const float4 cs = *reinterpret_cast<const float4 *>(rope.cos + o);
+            const float4 sn = *reinterpret_cast<const float4 *>(rope.sin + o);
+            const float4 a = lo, h = hi;
+            lo = make_float4(rot_lo(a.x, h.x, cs.x, sn.x), rot_lo(a.y, h.y, cs.y, sn.y),
+                             rot_lo(a.z, h.z, cs.z, sn.z), rot_lo(a.w, h.w, cs.w, sn.w));
+            hi = make_float4(rot_hi(a.x, h.x, cs.x, sn.x), rot_hi(a.y, h.y, cs.y, sn.y),
+                             rot_hi(a.z, h.z, cs.z, sn.z), rot_hi(a.w, h.w, cs.w, sn.w));
+        }
+        lo = make_float4(finite_or_zero(lo.x, bad), finite_or_zero(lo.y, bad), finite_or_zero(lo.z, bad),
+                         finite_or_zero(lo.w, bad));
+        hi = make_float4(finite_or_zero(hi.x, bad), finite_or_zero(hi.y, bad), finite_or_zero(hi.z, bad),
+                         finite_or_zero(hi.w, bad));
+    };
+    float m = 0.0f;
+    for (int i = rr; i < t1 - t0; i += RPI) {
+        float4 lo, hi;
+        row(i, lo, hi);
+        m = fmaxf(m, fmaxf(fmaxf(fabsf(lo.x), fabsf(lo.y)), fmaxf(fabsf(lo.z), fabsf(lo.w))));
+        m = fmaxf(m, fmaxf(fmaxf(fabsf(hi.x), fabsf(hi.y)), fmaxf(fabsf(hi.z), fabsf(hi.w))));
+    }
+    m = warp_max(m);
+    if ((threadIdx.x & 31) == 0)
+        s_max[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < AP_THREADS / 32; w++)
+        m = fmaxf(m, s_max[w]);
+    float s1 = fmaxf(s0, __fdiv_rn(m, 127.0f));
+    if (s1 < FLT_MIN)
+        s1 = 0.0f;
+    const float inv = s1 > 0.0f ? __fdiv_rn(1.0f, s1) : 0.0f;
+    for (int i = rr; i < t1 - t0; i += RPI) {
+        float4 lo, hi;
+        row(i, lo, hi);
+        int8_t *dst = codes + (size_t)(held + i) * D;
+        *reinterpret_cast<uint32_t *>(dst + 4 * j) = code4(lo, inv);
+        *reinterpret_cast<uint32_t *>(dst + D / 2 + 4 * j) = code4(hi, inv);
+    }
+    if (s1 > s0 && held) {
+        const float ratio = __fdiv_rn(s0, s1);
+        for (int w = threadIdx.x; w < held * D / 4; w += AP_THREADS) {
+            const char4 o = reinterpret_cast<const char4 *>(codes)[w];
+            reinterpret_cast<uint32_t *>(codes)[w] = code4(make_float4(o.x, o.y, o.z, o.w), ratio);
+        }
+    }
+    if (threadIdx.x == 0)
+        *scale = s1;
+    if (bad)
+        atomicCAS(err, 0u, (uint32_t)DEV_ERR_NONFINITE);
+}
+
+__device__ __forceinline__ void store1(float *p, float x) { *p = x; }
+__device__ __forceinline__ void store1(__half *p, float x) { *p = __float2half_rn(x); }
+__device__ __forceinline__ void store1(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
+
+// pages back as values: one CTA per (page, KV head, K or V), 16 codes a thread
+template <class T>
+__global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, const int *pages, T *k, T *v, uint32_t *err)
+{
+    const int id = pages[blockIdx.x], g = blockIdx.y;
+    if (id < 0 || id >= c.n_pages) {
+        if (threadIdx.x == 0)
+            atomicCAS(err, 0u, (uint32_t)DEV_ERR_BAD_PAGE);
+        return;
+    }
+    const size_t at = (size_t)id * c.n_kv + g, n = (size_t)c.page * c.D;
+    const int8_t *codes = (blockIdx.z ? c.vq : c.kq) + at * n;
+    const float s = (blockIdx.z ? c.vs : c.ks)[at];
+    T *out = (blockIdx.z ? v : k) + ((size_t)blockIdx.x * c.n_kv + g) * n;
+    for (size_t i = (size_t)threadIdx.x * 16; i < n; i += 256 * 16) {
+        const int4 w = *reinterpret_cast<const int4 *>(codes + i);
+        int8_t q[16];
+        memcpy(q, &w, 16);
+        __align__(16) T o[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            store1(&o[e], __fmul_rn((float)q[e], s));
+#pragma unroll
+        for (int e = 0; e < (int)sizeof(T); e++)
+            reinterpret_cast<int4 *>(out + i)[e] = reinterpret_cast<const int4 *>(o)[e];
+    }
+}
+
+template <class T>
+cudaError_t append_t(const Kv8 &c, const Kv8Batch &b, const void *k, const void *v, long long ld, const Kv8Rope &r,
+                     uint32_t *err, dim3 grid, cudaStream_t stream)
+{
+    const T *kt = reinterpret_cast<const T *>(k), *vt = reinterpret_cast<const T *>(v);
+    if (c.D == 128)
+        return launch(kv8_append_kernel<T, 128>, grid, dim3(AP_THREADS), 0, stream, false, c, b, kt, vt, ld, r, err);
+    return launch(kv8_append_kernel<T, 64>, grid, dim3(AP_THREADS), 0, stream, false, c, b, kt, vt, ld, r, err);
+}
+
+} // namespace
+
+int kv8_append(const Kv8 &c, const Kv8Batch &b, const void *k, const void *v, int dtype, long long ld,
+               const Kv8Rope &r, uint32_t *err, cudaStream_t stream)
+{
+    // n rows of one sequence touch at most n pages, and at most n/page + 2
+    const long long units = std::min((long long)b.n_rows, (long long)b.n_rows / c.page + 2LL * b.n_seqs);
+    const dim3 grid((unsigned)units, (unsigned)c.n_kv, 2);
+    if (dtype == LLMRS_F32)
+        LLMRS_CUDA_TRY(append_t<float>(c, b, k, v, ld, r, err, grid, stream));
+    else if (dtype == LLMRS_BF16)
+        LLMRS_CUDA_TRY(append_t<__nv_bfloat16>(c, b, k, v, ld, r, err, grid, stream));
+    else
+        LLMRS_CUDA_TRY(append_t<__half>(c, b, k, v, ld, r, err, grid, stream));
+    return LLMRS_OK;
+}
+
+int kv8_read(const Kv8 &c, const int *pages, int n, void *k, void *v, int dtype, uint32_t *err, cudaStream_t stream)
+{
+    const dim3 grid((unsigned)n, (unsigned)c.n_kv, 2), block(256);
+    if (dtype == LLMRS_F32)
+        LLMRS_CUDA_TRY(launch(kv8_read_kernel<float>, grid, block, 0, stream, false, c, pages, (float *)k, (float *)v,
+                              err));
+    else if (dtype == LLMRS_BF16)
+        LLMRS_CUDA_TRY(launch(kv8_read_kernel<__nv_bfloat16>, grid, block, 0, stream, false, c, pages,
+                              (__nv_bfloat16 *)k, (__nv_bfloat16 *)v, err));
+    else
+        LLMRS_CUDA_TRY(launch(kv8_read_kernel<__half>, grid, block, 0, stream, false, c, pages, (__half *)k,
+                              (__half *)v, err));
+    return LLMRS_OK;
+}
+
+} // namespace llmrs

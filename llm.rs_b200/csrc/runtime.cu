@@ -19,10 +19,12 @@
 #include "attention.cuh"
 #include "common.cuh"
 #include "gemv.cuh"
+#include "kv8.cuh"
 #include "prefill.cuh"
 #include "sample.cuh"
 #include "llmrs_synth.h"
 #include "ops.cuh"
+#include "verify.cuh"
 
 // ------------------------------------------------------------------ errors
 namespace llmrs {
@@ -232,6 +234,8 @@ int llmrs_ctx_create(int device, llmrs_ctx **out)
         rc = attention_prepare();
     if (rc == LLMRS_OK)
         rc = prefill_prepare();
+    if (rc == LLMRS_OK)
+        rc = kv8_prepare();
     if (rc != LLMRS_OK) {
         cudaFree(c->d_err);
         cudaStreamDestroy(c->own);
@@ -328,8 +332,12 @@ static int ctx_check_err(llmrs_ctx *ctx)
     LLMRS_CUDA_TRY(cudaMemcpy(&e, ctx->d_err, sizeof(e), cudaMemcpyDeviceToHost));
     if (e) {
         cudaMemset(ctx->d_err, 0, sizeof(uint32_t));
+        const char *what = e == DEV_ERR_BAD_BATCH   ? " (a sequence's rows or length lead outside the buffers)"
+                           : e == DEV_ERR_BAD_PAGE  ? " (a page id outside the pool)"
+                           : e == DEV_ERR_NONFINITE ? " (a key or value that is infinite or no number)"
+                                                    : "";
         return fail(e == DEV_ERR_MBAR_TIMEOUT || e == DEV_ERR_PEER_TIMEOUT ? LLMRS_ETIMEDOUT : LLMRS_EDEVICE,
-                    "device error word %u", e);
+                    "device error word %u%s", e, what);
     }
     return LLMRS_OK;
 }
@@ -549,6 +557,229 @@ int llmrs_quantize_q4(llmrs_ctx *ctx, const float *d_w, size_t n, uint8_t *d_qs,
 {
     LLMRS_CHECK_ARG(ctx && (n == 0 || (d_w && d_qs && d_scales)), "quantize_q4: bad arguments");
     return op_quantize_q4(ctx->stream, d_w, n, d_qs, d_scales);
+}
+
+// ---------------------------------------------------------------- paged 8-bit KV cache, drafts
+namespace {
+
+// make the context's device current for the launches of one call
+struct OnDevice {
+    int before = -1, device;
+    explicit OnDevice(int d) : device(d)
+    {
+        if (cudaGetDevice(&before) != cudaSuccess)
+            before = -1;
+        if (before != device)
+            cudaSetDevice(device);
+    }
+    ~OnDevice()
+    {
+        if (before >= 0 && before != device)
+            cudaSetDevice(before);
+    }
+};
+
+bool known_dtype(int t) { return t == LLMRS_F32 || t == LLMRS_BF16 || t == LLMRS_F16; }
+bool aligned16(const void *p) { return !((uintptr_t)p & 15); }
+
+int check_kv8(const llmrs_kv8 *c)
+{
+    LLMRS_CHECK_ARG(c, "kv8: cache is NULL");
+    LLMRS_CHECK_ARG(c->d_k_codes && c->d_v_codes && c->d_k_scales && c->d_v_scales, "kv8: NULL pool");
+    LLMRS_CHECK_ARG(aligned16(c->d_k_codes) && aligned16(c->d_v_codes), "kv8: code pools must be 16-byte aligned");
+    LLMRS_CHECK_ARG(c->page_size == 16 || c->page_size == 32 || c->page_size == 64 || c->page_size == 128,
+                    "kv8: page_size %d not 16, 32, 64 or 128", c->page_size);
+    LLMRS_CHECK_ARG(c->head_dim == 64 || c->head_dim == 128, "kv8: head_dim %d not 64 or 128", c->head_dim);
+    LLMRS_CHECK_ARG(c->n_kv_heads > 0 && c->n_kv_heads <= 1024, "kv8: n_kv_heads %d outside [1, 1024]",
+                    c->n_kv_heads);
+    LLMRS_CHECK_ARG(c->n_pages > 0 && (long long)c->n_pages * c->n_kv_heads * c->page_size <= INT32_MAX,
+                    "kv8: %d pages of %d tokens x %d heads (at most 2^31 - 1 rows)", c->n_pages, c->page_size,
+                    c->n_kv_heads);
+    return LLMRS_OK;
+}
+
+int check_batch(const llmrs_kv8 *c, const llmrs_kv8_batch *b)
+{
+    LLMRS_CHECK_ARG(b, "kv8: batch is NULL");
+    LLMRS_CHECK_ARG(b->n_seqs >= 0 && b->n_seqs <= 65535, "kv8: n_seqs %d outside [0, 65535]", b->n_seqs);
+    LLMRS_CHECK_ARG(b->n_seqs == 0 || (b->d_row_start && b->d_lens && b->d_page_table), "kv8: NULL batch array");
+    LLMRS_CHECK_ARG(b->max_pages > 0 && (long long)b->max_pages * c->page_size <= INT32_MAX,
+                    "kv8: max_pages %d (at most 2^31 - 1 positions)", b->max_pages);
+    return LLMRS_OK;
+}
+
+int check_rows(const char *op, const llmrs_kv8 *c, const void *p, int dtype, long long ld, int n_rows, int heads)
+{
+    LLMRS_CHECK_ARG(known_dtype(dtype), "%s: dtype %d unknown", op, dtype);
+    const int es = dtype == LLMRS_F32 ? 4 : 2;
+    LLMRS_CHECK_ARG(n_rows >= 0 && n_rows <= (1 << 24), "%s: n_rows %d outside [0, 2^24]", op, n_rows);
+    LLMRS_CHECK_ARG(n_rows == 0 || p, "%s: NULL rows", op);
+    LLMRS_CHECK_ARG(ld >= (long long)heads * c->head_dim, "%s: row stride %lld shorter than %d heads of %d", op, ld,
+                    heads, c->head_dim);
+    LLMRS_CHECK_ARG(aligned16(p) && ld * es % 16 == 0, "%s: rows must start on 16-byte boundaries", op);
+    return LLMRS_OK;
+}
+
+int check_rope(const char *op, const float *cs, const float *sn, int n_pos)
+{
+    LLMRS_CHECK_ARG(!cs == !sn, "%s: rope tables: both or neither", op);
+    LLMRS_CHECK_ARG(!cs || (n_pos > 0 && aligned16(cs) && aligned16(sn)),
+                    "%s: rope tables must be 16-byte aligned, with n_pos > 0 rows", op);
+    return LLMRS_OK;
+}
+
+Kv8 kv8_of(const llmrs_kv8 *c)
+{
+    return Kv8{c->d_k_codes, c->d_v_codes, c->d_k_scales, c->d_v_scales,
+               c->n_pages,   c->page_size, c->n_kv_heads, c->head_dim};
+}
+
+Kv8Batch batch_of(const llmrs_kv8 *c, const llmrs_kv8_batch *b, int n_rows, const float *cs, int n_pos)
+{
+    const int reach = b->max_pages * c->page_size;
+    return Kv8Batch{b->d_row_start, b->d_lens, b->d_page_table, b->n_seqs, b->max_pages, n_rows,
+                    cs ? std::min(reach, n_pos) : reach};
+}
+
+// the caller's workspace, or the context's scratch (which a capture must not grow)
+int take_workspace(llmrs_ctx *ctx, const char *op, void *d_ws, size_t have, size_t need, void **out)
+{
+    if (d_ws) {
+        LLMRS_CHECK_ARG(have >= need, "%s: workspace of %zu bytes, %zu needed", op, have, need);
+        LLMRS_CHECK_ARG(aligned16(d_ws), "%s: workspace must be 16-byte aligned", op);
+        *out = d_ws;
+        return LLMRS_OK;
+    }
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    LLMRS_CUDA_TRY(cudaStreamIsCapturing(ctx->stream, &st));
+    LLMRS_CHECK_ARG(st == cudaStreamCaptureStatusNone, "%s: a captured call needs its own workspace", op);
+    return ctx_scratch(ctx, need, out);
+}
+
+} // namespace
+
+int llmrs_kv8_append(llmrs_ctx *ctx, const llmrs_kv8 *cache, const llmrs_kv8_batch *batch, const void *d_k,
+                     const void *d_v, int dtype, long long ld, int n_rows, const float *d_rope_cos,
+                     const float *d_rope_sin, int n_pos)
+{
+    LLMRS_TRY(check_kv8(cache));
+    LLMRS_TRY(check_batch(cache, batch));
+    LLMRS_TRY(check_rows("kv8_append", cache, d_k, dtype, ld, n_rows, cache->n_kv_heads));
+    LLMRS_TRY(check_rows("kv8_append", cache, d_v, dtype, ld, n_rows, cache->n_kv_heads));
+    LLMRS_TRY(check_rope("kv8_append", d_rope_cos, d_rope_sin, n_pos));
+    LLMRS_CHECK_ARG(ctx, "kv8_append: ctx is NULL");
+    if (n_rows == 0 || batch->n_seqs == 0)
+        return LLMRS_OK;
+    OnDevice on(ctx->device);
+    return kv8_append(kv8_of(cache), batch_of(cache, batch, n_rows, d_rope_cos, n_pos), d_k, d_v, dtype, ld,
+                      Kv8Rope{d_rope_cos, d_rope_sin}, ctx->d_err, ctx->stream);
+}
+
+int llmrs_kv8_read(llmrs_ctx *ctx, const llmrs_kv8 *cache, const int *d_pages, int n, void *d_k, void *d_v, int dtype)
+{
+    LLMRS_TRY(check_kv8(cache));
+    LLMRS_CHECK_ARG(n >= 0 && (n == 0 || (d_pages && d_k && d_v)), "kv8_read: bad arguments");
+    LLMRS_CHECK_ARG(known_dtype(dtype), "kv8_read: dtype %d unknown", dtype);
+    LLMRS_CHECK_ARG(aligned16(d_k) && aligned16(d_v), "kv8_read: outputs must be 16-byte aligned");
+    LLMRS_CHECK_ARG(ctx, "kv8_read: ctx is NULL");
+    if (n == 0)
+        return LLMRS_OK;
+    OnDevice on(ctx->device);
+    return kv8_read(kv8_of(cache), d_pages, n, d_k, d_v, dtype, ctx->d_err, ctx->stream);
+}
+
+int llmrs_kv8_attention_workspace(const llmrs_kv8 *cache, const llmrs_kv8_batch *batch, int n_heads, int n_rows,
+                                  size_t *bytes)
+{
+    LLMRS_TRY(check_kv8(cache));
+    LLMRS_TRY(check_batch(cache, batch));
+    LLMRS_CHECK_ARG(bytes && n_rows >= 0 && n_heads > 0 && n_heads % cache->n_kv_heads == 0,
+                    "kv8_attention_workspace: bad arguments");
+    *bytes = llmrs::kv8_attention_workspace(n_heads, cache->head_dim, n_rows, batch->n_seqs);
+    return LLMRS_OK;
+}
+
+int llmrs_kv8_attention(llmrs_ctx *ctx, const llmrs_kv8 *cache, const llmrs_kv8_batch *batch, const void *d_q,
+                        long long ld_q, void *d_out, long long ld_out, int dtype, int n_rows, int n_heads,
+                        const float *d_rope_cos, const float *d_rope_sin, int n_pos, float scale, void *d_workspace,
+                        size_t workspace_bytes)
+{
+    LLMRS_TRY(check_kv8(cache));
+    LLMRS_TRY(check_batch(cache, batch));
+    LLMRS_CHECK_ARG(n_heads > 0 && n_heads <= 65535 && n_heads % cache->n_kv_heads == 0,
+                    "kv8_attention: bad head counts %d/%d", n_heads, cache->n_kv_heads);
+    LLMRS_TRY(check_rows("kv8_attention", cache, d_q, dtype, ld_q, n_rows, n_heads));
+    LLMRS_TRY(check_rows("kv8_attention", cache, d_out, dtype, ld_out, n_rows, n_heads));
+    LLMRS_TRY(check_rope("kv8_attention", d_rope_cos, d_rope_sin, n_pos));
+    LLMRS_CHECK_ARG(scale >= 0.0f && scale <= 3.0e38f, "kv8_attention: scale must be finite and not negative");
+    LLMRS_CHECK_ARG(ctx, "kv8_attention: ctx is NULL");
+    if (n_rows == 0 || batch->n_seqs == 0)
+        return LLMRS_OK;
+    OnDevice on(ctx->device);
+    void *ws = nullptr;
+    LLMRS_TRY(take_workspace(ctx, "kv8_attention", d_workspace, workspace_bytes,
+                             llmrs::kv8_attention_workspace(n_heads, cache->head_dim, n_rows, batch->n_seqs), &ws));
+    Kv8Attn a{};
+    a.c = kv8_of(cache);
+    a.b = batch_of(cache, batch, n_rows, d_rope_cos, n_pos);
+    a.r = Kv8Rope{d_rope_cos, d_rope_sin};
+    a.q = d_q;
+    a.out = d_out;
+    a.ld_q = ld_q;
+    a.ld_out = ld_out;
+    a.dtype = dtype;
+    a.n_heads = n_heads;
+    a.scale = scale > 0.0f ? scale : 1.0f / sqrtf((float)cache->head_dim);
+    a.err = ctx->d_err;
+    return llmrs::kv8_attention(a, ws, ctx->sms, ctx->stream);
+}
+
+int llmrs_verify_draft_workspace(int n_rows, int vocab, size_t *bytes)
+{
+    LLMRS_CHECK_ARG(bytes && n_rows >= 0 && vocab > 0, "verify_draft_workspace: bad arguments");
+    *bytes = verify_workspace(n_rows, vocab);
+    return LLMRS_OK;
+}
+
+int llmrs_verify_draft(llmrs_ctx *ctx, const void *d_logits, long long ld_logits, int dtype, int vocab, int n_rows,
+                       int n_seqs, const int *d_row_start, const int *d_draft_tokens, const float *d_draft_probs,
+                       long long ld_probs, const float *d_uniforms, const float *d_temperature, int *d_tokens,
+                       int *d_accepted, float *d_token_probs, void *d_workspace, size_t workspace_bytes)
+{
+    LLMRS_CHECK_ARG(known_dtype(dtype), "verify_draft: dtype %d unknown", dtype);
+    LLMRS_CHECK_ARG(vocab > 0 && n_rows >= 0 && n_rows <= 65535 && n_seqs >= 0 && n_seqs <= 65535,
+                    "verify_draft: vocab %d, n_rows %d, n_seqs %d (at most 65535 rows)", vocab, n_rows, n_seqs);
+    LLMRS_CHECK_ARG(n_seqs == 0 || (d_row_start && d_accepted), "verify_draft: NULL argument");
+    LLMRS_CHECK_ARG(n_seqs == 0 || n_rows == 0 || (d_logits && d_uniforms && d_tokens),
+                    "verify_draft: NULL argument");
+    LLMRS_CHECK_ARG(n_rows <= n_seqs || d_draft_tokens, "verify_draft: no drafted tokens for %d rows of %d sequences",
+                    n_rows, n_seqs);
+    LLMRS_CHECK_ARG(ld_logits >= vocab && (!d_draft_probs || ld_probs >= vocab),
+                    "verify_draft: row strides %lld, %lld shorter than the vocabulary", ld_logits, ld_probs);
+    LLMRS_CHECK_ARG(ctx, "verify_draft: ctx is NULL");
+    if (n_seqs == 0)
+        return LLMRS_OK;
+    OnDevice on(ctx->device);
+    void *ws = nullptr;
+    LLMRS_TRY(take_workspace(ctx, "verify_draft", d_workspace, workspace_bytes, verify_workspace(n_rows, vocab), &ws));
+    VerifyParams p{};
+    p.logits = d_logits;
+    p.ld = ld_logits;
+    p.dtype = dtype;
+    p.vocab = vocab;
+    p.n_rows = n_rows;
+    p.n_seqs = n_seqs;
+    p.row_start = d_row_start;
+    p.draft = d_draft_tokens;
+    p.q = d_draft_probs;
+    p.ldq = ld_probs;
+    p.u = d_uniforms;
+    p.temperature = d_temperature;
+    p.tokens = d_tokens;
+    p.accepted = d_accepted;
+    p.probs = d_token_probs;
+    p.err = ctx->d_err;
+    return verify_launch(p, ws, ctx->stream);
 }
 
 // ---------------------------------------------------------------- model

@@ -1,0 +1,400 @@
+// verify.cu - verification of drafted tokens against the target's
+// probabilities, from given uniform draws (sm_100a).
+//
+// A sequence with k drafts d_0 .. d_{k-1} has k + 1 rows of target logits; row
+// i gives p_i = softmax(logits_i / temperature), and q_i is the distribution
+// that d_i was drawn from.
+//   accept d_i while u_i * q_i(d_i) < p_i(d_i)      (probability min(1, p/q))
+//   at the first rejection, i = a: the next token comes from max(p_a - q_a, 0),
+//   after k acceptances from p_k, by the inverse CDF in index order: the first
+//   token whose running sum exceeds u_k * total.
+// The tokens that come out are distributed as if drawn from p row by row.
+// Temperature 0 makes p one at the row's first maximum.  The reference draws
+// one token at a time on the host (src/main.rs:192-305).
+//
+// Two kernels.  verify_rows: every row's maximum and sum of exponentials, one
+// CTA per (row, chunk of VCHUNK tokens); bound by reading the logits once.
+// verify_pick: a cluster of PICK_CTAS CTAs per sequence decides the
+// acceptances, then walks the one row that the next token comes from, with
+// exponentials and sums in 64 bits: a draw next to the border of two tokens
+// would otherwise be decided by the rounding of a 32-bit running sum over the
+// whole vocabulary.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <float.h>
+#include <limits.h>
+#include <math.h>
+
+#include "common.cuh"
+#include "verify.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace llmrs {
+
+namespace {
+
+constexpr int VT = 256;         // threads of verify_rows
+constexpr int VPER = 32;        // logits a thread holds
+constexpr int VCHUNK = VT * VPER;
+constexpr int PICK_CTAS = 8;
+constexpr int PT = 512;
+constexpr int PW = PT / 32;
+
+// a chunk's part of its row's statistics
+struct RowPart {
+    float m;      // maximum
+    int at;       // its first place
+    double s;     // sum of exp((l - m) / T)
+};
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// a logit that is no number has no weight; infinite ones share it
+__device__ __forceinline__ float clean(float l)
+{
+    return l != l ? -INFINITY : fminf(l, FLT_MAX);
+}
+
+__device__ __forceinline__ double warp_sum_d(double v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// largest value, the lower place on a tie
+__device__ __forceinline__ void warp_best(float &m, int &at)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
+        const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
+        if (m2 > m || (m2 == m && a2 < at)) {
+            m = m2;
+            at = a2;
+        }
+    }
+}
+
+// sequence of a packed row, -1 behind the last one
+__device__ __forceinline__ int seq_of_row(const int *row_start, int n_seqs, int row)
+{
+    int lo = 0, hi = n_seqs; // the last s with row_start[s] <= row
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (row_start[mid] <= row)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return row >= row_start[lo] && row < row_start[lo + 1] ? lo : -1;
+}
+
+template <class T>
+__global__ void __launch_bounds__(VT) verify_rows_kernel(VerifyParams p, RowPart *part, int n_chunks)
+{
+    __shared__ float s_m[VT / 32];
+    __shared__ int s_at[VT / 32];
+    __shared__ double s_s[VT / 32];
+    const int row = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const T *x = reinterpret_cast<const T *>(p.logits) + (size_t)row * p.ld;
+    const int c0 = chunk * VCHUNK, c1 = min(p.vocab, c0 + VCHUNK);
+    float l[VPER];
+    float m = -INFINITY;
+    int at = INT_MAX;
+#pragma unroll
+    for (int i = 0; i < VPER; i++) {
+        const int t = c0 + i * VT + threadIdx.x;
+        l[i] = t < c1 ? clean(to_float(x[t])) : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < VPER; i++)
+        if (l[i] > m) {
+            m = l[i];
+            at = c0 + i * VT + threadIdx.x;
+        }
+    warp_best(m, at);
+    if (lane == 0) {
+        s_m[warp] = m;
+        s_at[warp] = at;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < VT / 32; w++)
+        if (s_m[w] > m || (s_m[w] == m && s_at[w] < at)) {
+            m = s_m[w];
+            at = s_at[w];
+        }
+    const int seq = seq_of_row(p.row_start, p.n_seqs, row);
+    const float T_ = seq >= 0 && p.temperature ? p.temperature[seq] : 1.0f;
+    const float inv = T_ > 0.0f ? 1.0f / T_ : 0.0f;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPER; i++)
+        sum += l[i] > -INFINITY ? expf((l[i] - m) * inv) : 0.0f;
+    const double d = warp_sum_d((double)sum);
+    if (lane == 0)
+        s_s[warp] = d;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double s = 0.0;
+        for (int w = 0; w < VT / 32; w++)
+            s += s_s[w];
+        RowPart r;
+        r.m = m;
+        r.at = at;
+        r.s = s;
+        part[(size_t)row * n_chunks + chunk] = r;
+    }
+}
+
+// a row's statistics from its chunks (whole warp)
+__device__ __forceinline__ RowPart row_stats(const RowPart *part, int n_chunks, double inv)
+{
+    const int lane = threadIdx.x & 31;
+    RowPart r;
+    r.m = -INFINITY;
+    r.at = INT_MAX;
+    for (int c = lane; c < n_chunks; c += 32)
+        if (part[c].m > r.m) {
+            r.m = part[c].m;
+            r.at = part[c].at;
+        }
+    warp_best(r.m, r.at);
+    double s = 0.0;
+    for (int c = lane; c < n_chunks; c += 32)
+        if (part[c].m > -INFINITY)
+            s += part[c].s * exp(((double)part[c].m - (double)r.m) * inv);
+    r.s = warp_sum_d(s);
+    return r;
+}
+
+template <class T>
+__global__ void __cluster_dims__(PICK_CTAS, 1, 1) __launch_bounds__(PT)
+    verify_pick_kernel(VerifyParams p, const RowPart *part, int n_chunks)
+{
+    cg::cluster_group cluster = cg::this_cluster();
+    __shared__ int s_first;                       // first rejected draft
+    __shared__ double s_z[PICK_CTAS];             // each CTA's share of the row's sum
+    __shared__ double s_w[2][PICK_CTAS * PW];     // each warp's share: of max(p - q, 0), of p
+    __shared__ int s_final[2][PICK_CTAS * PW];    // last token with weight in each warp's range
+    __shared__ double s_red[PW];
+    const int seq = blockIdx.x / PICK_CTAS, rank = (int)cluster.block_rank();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int r0 = p.row_start[seq], r1 = p.row_start[seq + 1], n = r1 - r0;
+    if (n <= 0 || r0 < 0 || r1 > p.n_rows) { // the same for the whole cluster
+        if (rank == 0 && threadIdx.x == 0) {
+            p.accepted[seq] = 0;
+            if (n != 0)
+                atomicCAS(p.err, 0u, (uint32_t)DEV_ERR_BAD_BATCH);
+        }
+        return;
+    }
+    // drafts lie packed without the last rows: one less than the rows for each
+    // sequence in front that has any
+    int in_front = 0;
+    bool rising = p.row_start[0] >= 0;
+    for (int i0 = 0; i0 < seq; i0 += PT) {
+        const int i = i0 + (int)threadIdx.x, rows = i < seq ? p.row_start[i + 1] - p.row_start[i] : 0;
+        in_front += __syncthreads_count(rows > 0);
+        rising = !__syncthreads_or(rows < 0) && rising;
+    }
+    if (!rising) {
+        if (rank == 0 && threadIdx.x == 0) {
+            p.accepted[seq] = 0;
+            atomicCAS(p.err, 0u, (uint32_t)DEV_ERR_BAD_BATCH);
+        }
+        return;
+    }
+    const int k = n - 1, d0 = r0 - p.row_start[0] - in_front; // drafts and their first place
+    const float T_ = p.temperature ? p.temperature[seq] : 1.0f;
+    const bool greedy = !(T_ > 0.0f);
+    const double inv = greedy ? 1.0 : 1.0 / (double)T_;
+    if (threadIdx.x == 0)
+        s_first = k;
+    __syncthreads();
+    for (int i = warp; i < k; i += PW) {
+        const int row = r0 + i, d = p.draft[d0 + i];
+        const RowPart r = row_stats(part + (size_t)row * n_chunks, n_chunks, inv);
+        if (lane == 0) {
+            double pd = 0.0;
+            if (d < 0 || d >= p.vocab)
+                atomicCAS(p.err, 0u, (uint32_t)DEV_ERR_BAD_TOKEN);
+            else if (greedy)
+                pd = d == r.at ? 1.0 : 0.0;
+            else if (r.m > -INFINITY) {
+                const float l = clean(to_float(reinterpret_cast<const T *>(p.logits)[(size_t)row * p.ld + d]));
+                pd = exp(((double)l - (double)r.m) * inv) / r.s;
+            }
+            const bool known = d >= 0 && d < p.vocab;
+            const double qd = p.q && known ? (double)p.q[(size_t)(d0 + i) * p.ldq + d] : 1.0;
+            if (!((double)p.u[row] * qd < pd))
+                atomicMin(&s_first, i);
+            if (rank == 0 && p.probs)
+                p.probs[row] = (float)pd; // overwritten below behind the first rejection
+        }
+    }
+    __syncthreads();
+    const int a = s_first, row = r0 + a;
+    if (rank == 0)
+        for (int i = threadIdx.x; i < n; i += PT) {
+            if (i != a)
+                p.tokens[r0 + i] = i < a ? p.draft[d0 + i] : -1;
+            if (i > a && p.probs)
+                p.probs[r0 + i] = 0.0f;
+            if (i == 0)
+                p.accepted[seq] = a;
+        }
+    const RowPart r = row_stats(part + (size_t)row * n_chunks, n_chunks, inv);
+    if (greedy || !(r.m > -INFINITY)) { // the first maximum; no token when every one is masked
+        if (rank == 0 && threadIdx.x == 0) {
+            const bool some = r.m > -INFINITY;
+            p.tokens[row] = some ? r.at : -1;
+            if (p.probs)
+                p.probs[row] = some ? 1.0f : 0.0f;
+        }
+        return;
+    }
+    const T *x = reinterpret_cast<const T *>(p.logits) + (size_t)row * p.ld;
+    const bool rest = a < k;
+    const float *q = rest && p.q ? p.q + (size_t)(d0 + a) * p.ldq : nullptr;
+    const int gone = rest && !p.q ? p.draft[d0 + a] : -1; // a certain draft's own token
+    // warp `gw` of the cluster's warps owns the tokens [t0, t1)
+    const int gw = rank * PW + warp;
+    const int per = (p.vocab + PICK_CTAS * PW - 1) / (PICK_CTAS * PW);
+    const int t0 = min(p.vocab, gw * per), t1 = min(p.vocab, t0 + per);
+    auto weight = [&](int t) { // exp((l - m) / T) in 64 bits
+        const float l = clean(to_float(x[t]));
+        return l > -INFINITY ? exp(((double)l - (double)r.m) * inv) : 0.0;
+    };
+    double z = 0.0;
+    for (int t = t0 + lane; t < t1; t += 32)
+        z += weight(t);
+    z = warp_sum_d(z);
+    if (lane == 0)
+        s_red[warp] = z;
+    __syncthreads();
+    if (threadIdx.x < PICK_CTAS) {
+        double c = 0.0;
+        for (int w = 0; w < PW; w++)
+            c += s_red[w];
+        cluster.map_shared_rank(s_z, threadIdx.x)[rank] = c;
+    }
+    cluster.sync();
+    z = 0.0;
+    for (int c = 0; c < PICK_CTAS; c++)
+        z += s_z[c];
+    const double invz = 1.0 / z;
+    auto residual = [&](int t, double pt) {
+        const double w = t == gone ? 0.0 : q ? pt - (double)q[t] : pt;
+        return w > 0.0 ? w : 0.0;
+    };
+    double sw = 0.0, sp = 0.0;
+    int fw = -1, fp = -1;
+    for (int t = t0 + lane; t < t1; t += 32) {
+        const double pt = weight(t) * invz, w = residual(t, pt);
+        sw += w;
+        sp += pt;
+        fw = w > 0.0 ? t : fw;
+        fp = pt > 0.0 ? t : fp;
+    }
+    sw = warp_sum_d(sw);
+    sp = warp_sum_d(sp);
+    fw = __reduce_max_sync(0xffffffffu, fw);
+    fp = __reduce_max_sync(0xffffffffu, fp);
+    if (lane < PICK_CTAS) {
+        cluster.map_shared_rank(&s_w[0][0], lane)[gw] = sw;
+        cluster.map_shared_rank(&s_w[1][0], lane)[gw] = sp;
+        cluster.map_shared_rank(&s_final[0][0], lane)[gw] = fw;
+        cluster.map_shared_rank(&s_final[1][0], lane)[gw] = fp;
+    }
+    cluster.sync(); // the last access to another CTA's shared memory
+    double total = 0.0;
+    for (int w = 0; w < PICK_CTAS * PW; w++)
+        total += s_w[0][w];
+    const int use = total > 0.0 ? 0 : 1; // p equals q: nothing is left over, draw from p
+    if (use) {
+        total = 0.0;
+        for (int w = 0; w < PICK_CTAS * PW; w++)
+            total += s_w[1][w];
+    }
+    const double target = (double)p.u[r1 - 1] * total;
+    double before = 0.0;
+    int owner = -1, last = -1; // the warp whose range the target falls into
+    for (int w = 0; w < PICK_CTAS * PW; w++) {
+        if (s_final[use][w] >= 0)
+            last = w;
+        if (owner < 0) {
+            if (s_final[use][w] >= 0 && before + s_w[use][w] > target)
+                owner = w;
+            else
+                before += s_w[use][w];
+        }
+    }
+    const bool past = owner < 0; // the draw lies behind the rounded sum
+    if (past)
+        owner = last;
+    if (gw != owner)
+        return;
+    int token = -1;
+    if (!past)
+        for (int b = t0; b < t1 && token < 0; b += 32) {
+            const int t = b + lane;
+            const double pt = t < t1 ? weight(t) * invz : 0.0;
+            const double w = t < t1 ? (use ? pt : residual(t, pt)) : 0.0;
+            double c = w;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double y = __shfl_up_sync(0xffffffffu, c, o);
+                if (lane >= o)
+                    c += y;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, w > 0.0 && before + c > target);
+            if (hit)
+                token = b + __ffs(hit) - 1;
+            before += __shfl_sync(0xffffffffu, c, 31);
+        }
+    if (token < 0)
+        token = s_final[use][owner];
+    if (lane == 0) {
+        p.tokens[row] = token;
+        if (p.probs)
+            p.probs[row] = (float)(weight(token) * invz);
+    }
+}
+
+template <class T>
+int run(const VerifyParams &p, RowPart *part, cudaStream_t stream)
+{
+    const int n_chunks = (p.vocab + VCHUNK - 1) / VCHUNK;
+    if (p.n_rows > 0)
+        LLMRS_CUDA_TRY(launch(verify_rows_kernel<T>, dim3(n_chunks, p.n_rows), dim3(VT), 0, stream, false, p, part,
+                              n_chunks));
+    LLMRS_CUDA_TRY(launch(verify_pick_kernel<T>, dim3(p.n_seqs * PICK_CTAS), dim3(PT), 0, stream, false, p,
+                          (const RowPart *)part, n_chunks));
+    return LLMRS_OK;
+}
+
+} // namespace
+
+size_t verify_workspace(int n_rows, int vocab)
+{
+    return (size_t)n_rows * ((vocab + VCHUNK - 1) / VCHUNK) * sizeof(RowPart);
+}
+
+int verify_launch(const VerifyParams &p, void *ws, cudaStream_t stream)
+{
+    RowPart *part = reinterpret_cast<RowPart *>(ws);
+    if (p.dtype == LLMRS_F32)
+        return run<float>(p, part, stream);
+    if (p.dtype == LLMRS_BF16)
+        return run<__nv_bfloat16>(p, part, stream);
+    return run<__half>(p, part, stream);
+}
+
+} // namespace llmrs

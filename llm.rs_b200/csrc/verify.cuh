@@ -1,0 +1,29 @@
+// verify.cuh - verification of drafted tokens (host interface).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace llmrs {
+
+struct VerifyParams {
+    const void *logits;       // [n_rows][ld]
+    long long ld;
+    int dtype, vocab, n_rows, n_seqs;
+    const int *row_start;     // [n_seqs + 1]
+    const int *draft;         // [drafts], packed: one fewer than the rows of each sequence
+    const float *q;           // [drafts][ldq] the drafting model's probabilities; nullptr: each draft was certain
+    long long ldq;
+    const float *u;           // [n_rows] uniform draws
+    const float *temperature; // [n_seqs] or nullptr (1)
+    int *tokens;              // [n_rows]
+    int *accepted;            // [n_seqs]
+    float *probs;             // [n_rows] or nullptr
+    uint32_t *err;
+};
+
+size_t verify_workspace(int n_rows, int vocab);
+int verify_launch(const VerifyParams &p, void *ws, cudaStream_t stream);
+
+} // namespace llmrs

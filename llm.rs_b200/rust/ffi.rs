@@ -8,7 +8,7 @@
 //! on every OpenCL call in src/backend/opencl.rs).
 #![allow(non_camel_case_types)]
 
-use std::os::raw::{c_char, c_int, c_uint, c_ulonglong, c_void};
+use std::os::raw::{c_char, c_int, c_longlong, c_uint, c_ulonglong, c_void};
 
 pub const LLMRS_OK: c_int = 0;
 pub const LLMRS_F16: c_int = 0;
@@ -59,6 +59,31 @@ pub struct llmrs_config {
     pub scale_dtype: c_int,
     pub tp_rank: c_int,
     pub tp_size: c_int,
+}
+
+/// Paged 8-bit KV cache: int8 codes and one f32 scale per (page, KV head).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct llmrs_kv8 {
+    pub d_k_codes: *mut i8,
+    pub d_v_codes: *mut i8,
+    pub d_k_scales: *mut f32,
+    pub d_v_scales: *mut f32,
+    pub n_pages: c_int,
+    pub page_size: c_int,
+    pub n_kv_heads: c_int,
+    pub head_dim: c_int,
+}
+
+/// The packed new rows of a batch of sequences.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct llmrs_kv8_batch {
+    pub n_seqs: c_int,
+    pub d_row_start: *const c_int,
+    pub d_lens: *const c_int,
+    pub d_page_table: *const c_int,
+    pub max_pages: c_int,
 }
 
 #[link(name = "llmrs_cuda")]
@@ -123,6 +148,27 @@ extern "C" {
                                    d_rope_cos: *const f32, d_rope_sin: *const f32, d_out: *mut f32,
                                    n_rows: c_int, n_heads: c_int, n_kv_heads: c_int, head_dim: c_int,
                                    max_seq: c_int, start_pos: c_int) -> c_int;
+
+    // ---- paged 8-bit KV cache, drafted tokens (no counterpart in the reference) ----
+    pub fn llmrs_kv8_append(ctx: *mut llmrs_ctx, cache: *const llmrs_kv8, batch: *const llmrs_kv8_batch,
+                            d_k: *const c_void, d_v: *const c_void, dtype: c_int, ld: c_longlong, n_rows: c_int,
+                            d_rope_cos: *const f32, d_rope_sin: *const f32, n_pos: c_int) -> c_int;
+    pub fn llmrs_kv8_read(ctx: *mut llmrs_ctx, cache: *const llmrs_kv8, d_pages: *const c_int, n: c_int,
+                          d_k: *mut c_void, d_v: *mut c_void, dtype: c_int) -> c_int;
+    pub fn llmrs_kv8_attention_workspace(cache: *const llmrs_kv8, batch: *const llmrs_kv8_batch, n_heads: c_int,
+                                         n_rows: c_int, bytes: *mut usize) -> c_int;
+    pub fn llmrs_kv8_attention(ctx: *mut llmrs_ctx, cache: *const llmrs_kv8, batch: *const llmrs_kv8_batch,
+                               d_q: *const c_void, ld_q: c_longlong, d_out: *mut c_void, ld_out: c_longlong,
+                               dtype: c_int, n_rows: c_int, n_heads: c_int, d_rope_cos: *const f32,
+                               d_rope_sin: *const f32, n_pos: c_int, scale: f32, d_workspace: *mut c_void,
+                               workspace_bytes: usize) -> c_int;
+    pub fn llmrs_verify_draft_workspace(n_rows: c_int, vocab: c_int, bytes: *mut usize) -> c_int;
+    pub fn llmrs_verify_draft(ctx: *mut llmrs_ctx, d_logits: *const c_void, ld_logits: c_longlong, dtype: c_int,
+                              vocab: c_int, n_rows: c_int, n_seqs: c_int, d_row_start: *const c_int,
+                              d_draft_tokens: *const c_int, d_draft_probs: *const f32, ld_probs: c_longlong,
+                              d_uniforms: *const f32, d_temperature: *const f32, d_tokens: *mut c_int,
+                              d_accepted: *mut c_int, d_token_probs: *mut f32, d_workspace: *mut c_void,
+                              workspace_bytes: usize) -> c_int;
 
     // ---- model: device-resident weights + KV cache, fused token loop ----
     pub fn llmrs_model_create(ctx: *mut llmrs_ctx, cfg: *const llmrs_config, out: *mut *mut llmrs_model) -> c_int;
