@@ -1,106 +1,929 @@
 // kv8_attention.cu - causal attention of a ragged batch over the paged 8-bit
-// KV cache (sm_100a).
+// KV cache (sm_100a): the kernel for few rows per sequence, its merge, and the
+// launch of both paths.
 //
 // Row i of sequence s stands at position P = lens[s] + i and attends to the
 // positions 0 .. P of its pages (its own key and value are in the cache):
 //   o = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale * q.k_t - max),
-//   k_t = ks * kq_t,  v_t = vs * vq_t
+//   k_t = ks * kq_t,  v_t = vs * vq_t,  ks, vs the scales of t's page and head,
 // in one pass with the running maximum and sum of the softmax.  q is rotated
-// by its position here.  The reference's per-head loop (src/core/layer.rs:
-// 175-333) is the same formula over one sequence's contiguous f32 cache.
+// by its position on the way.  The reference's per-head loop
+// (src/core/layer.rs:175-333) is the same formula over one sequence's
+// contiguous f32 cache.
 //
-// One warp per (row, query head): lane = D/32 dims, one token at a time.
+// Few rows: bound by reading the codes once.  The (row, query head) vectors
+// that share a KV head are the columns of mma.sync.m16n8k16: S = K Q^T, then
+// O^T = V^T P, so a tile of 32 tokens is the long side and few vectors waste
+// little.  int8 codes are exact in f16.  f32 rows: q and the probabilities are
+// split into two f16 pieces (22 bits and more), the pieces are columns of
+// their own in the same instruction, so one pass over the codes serves both.
+//
+// Work: the tiles of all (sequence, vector group, KV head) pairs in one row,
+// cut into equal ranges, one per warp, whatever the lengths.  A warp streams
+// its range through its own ring of shared memory (TMA boxes, swizzled so that
+// both fragment patterns read without bank conflicts) and never waits for
+// another warp.  A pair that lies within one range is finished there; the
+// pieces of the others go to the workspace and a second kernel joins them in
+// order, so results do not depend on timing.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "attention_core.cuh"
+#include <algorithm>
+#include <mutex>
+
+#include "gemv.cuh"
 #include "kv8.cuh"
 
 namespace llmrs {
 
 namespace {
 
-__device__ __forceinline__ void put(float *p, float x) { *p = x; }
-__device__ __forceinline__ void put(__half *p, float x) { *p = __float2half_rn(x); }
-__device__ __forceinline__ void put(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
+constexpr int FT = 32;        // tokens of a tile
+constexpr int FW = 8;         // warps of a CTA
+constexpr int F_MAX_CTAS = 160;
+constexpr int F_WARPS = F_MAX_CTAS * FW;
+constexpr int JT = 128;       // threads of the joining kernel
+constexpr float P_SCALE = 16384.0f; // probabilities are split at this scale: p in [0, 1] keeps 22 bits down to 2^-13
 
-template <class T, int D>
-__global__ void __launch_bounds__(128) kv8_attention_kernel(Kv8Attn a)
+struct FewParams {
+    CUtensorMap tk, tv; // code pools as rows of D bytes
+    Kv8Attn a;
+    float *part;        // [warps][2][vectors][D + 2]
+    int4 *head;         // [warps][2] pieces: (sequence, group, KV head, state)
+    int many;           // sequences with more vectors per KV head than this are another kernel's
+};
+
+enum : int { PIECE_NONE = 0, PIECE_OPEN = 1, PIECE_END = 2 };
+
+// what a warp needs to know of one tile
+struct __align__(16) Tile {
+    int row0, row1;       // pool rows of its 16-token halves (row1: only for pages of 16); -1: not there
+    int s, group, g, tile; // pair, and the tile's index in it
+    int n_tiles, len, r0, n; // of the sequence: tiles, cached tokens, first row, rows
+    float ks0, ks1, vs0, vs1;
+    int pad0, pad1;
+};
+static_assert(sizeof(Tile) == 64, "four 16-byte words");
+
+template <int D>
+struct FewLay {
+    static constexpr int STAGES = D == 128 ? 3 : 6;
+    static constexpr int BOX = FT * D;            // bytes of K or V codes of a tile
+    static constexpr int RING = STAGES * 2 * BOX; // per warp
+    static constexpr int TILES = 64;              // tile records per warp: two batches of 32
+    static constexpr int tile_off = FW * RING;
+    static constexpr int bar_off = tile_off + FW * TILES * (int)sizeof(Tile);
+    static constexpr int bytes = bar_off + FW * STAGES * 8 + 1024; // + alignment slack
+    static_assert(bytes <= 232448, "shared memory of one CTA");
+};
+
+__device__ __forceinline__ void tma_box(void *dst, const CUtensorMap *map, int row, uint64_t *bar, uint64_t policy)
 {
-    constexpr int DL = D / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = blockIdx.x, h = blockIdx.y * 4 + warp;
-    if (h >= a.n_heads)
-        return;
-    int s = -1, r0 = 0, n = 0, len = 0;
-    for (int i = 0; i < a.b.n_seqs; i++) {
-        kv8_seq(a.b, i, a.err, r0, n, len);
-        if (n && row >= r0 && row < r0 + n) {
-            s = i;
-            break;
-        }
-    }
-    if (s < 0)
-        return;
-    const int pos = len + row - r0, g = h / (a.n_heads / a.c.n_kv);
-    const T *qp = reinterpret_cast<const T *>(a.q) + (size_t)row * a.ld_q + (size_t)h * D + lane * DL;
-    float q[DL], c[DL], sn[DL], acc[DL];
-#pragma unroll
-    for (int k = 0; k < DL; k++) {
-        q[k] = (float)qp[k];
-        acc[k] = 0.0f;
-    }
-    if (a.r.cos) {
-        rope_table_lane<D>(c, sn, lane, a.r.cos + (size_t)pos * (D / 2), a.r.sin + (size_t)pos * (D / 2));
-        rope_lane<D>(q, lane, c, sn);
-    }
-    float m = -INFINITY, l = 0.0f;
-    for (int t = 0; t <= pos; t++) {
-        const int id = kv8_page(a.b, a.c, s, t / a.c.page, a.err);
-        if (id < 0)
-            continue;
-        const size_t at = (size_t)id * a.c.n_kv + g, o = (at * a.c.page + t % a.c.page) * D + lane * DL;
-        float dot = 0.0f;
-#pragma unroll
-        for (int k = 0; k < DL; k++)
-            dot += q[k] * (float)a.c.kq[o + k];
-        const float x = warp_sum(dot) * (a.c.ks[at] * a.scale);
-        const float m_new = fmaxf(m, x), corr = expf(m - m_new), p = expf(x - m_new), vs = a.c.vs[at];
-        l = l * corr + p;
-#pragma unroll
-        for (int k = 0; k < DL; k++)
-            acc[k] = acc[k] * corr + p * vs * (float)a.c.vq[o + k];
-        m = m_new;
-    }
-    T *out = reinterpret_cast<T *>(a.out) + (size_t)row * a.ld_out + (size_t)h * D + lane * DL;
-#pragma unroll
-    for (int k = 0; k < DL; k++)
-        put(out + k, l == 0.0f ? 0.0f : acc[k] / l);
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(smem_addr(dst)),
+        "l"(map), "r"(0), "r"(row), "r"(smem_addr(bar)), "l"(policy)
+        : "memory");
 }
 
-template <class T>
-cudaError_t run(const Kv8Attn &a, cudaStream_t stream)
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1)
 {
-    const dim3 grid((unsigned)a.b.n_rows, (unsigned)((a.n_heads + 3) / 4));
-    return a.c.D == 128 ? launch(kv8_attention_kernel<T, 128>, grid, dim3(128), 0, stream, false, a)
-                        : launch(kv8_attention_kernel<T, 64>, grid, dim3(128), 0, stream, false, a);
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Two int8 codes, offset by 128 to unsigned bytes, as f16 values: the byte
+// under the exponent of 1024 is 1024 + code + 128, and the difference is exact.
+__device__ __forceinline__ uint32_t codes_f16(uint32_t biased, uint32_t select)
+{
+    const uint32_t w = __byte_perm(biased, 0x64646464u, select);
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&w), __floats2half2_rn(1152.0f, 1152.0f));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+__device__ __forceinline__ uint32_t pack16(float a, float b)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// N (a multiple of 16/sizeof(T) ... 16) consecutive floats to a row of T
+template <int N>
+__device__ __forceinline__ void store_row(float *p, const float (&x)[N])
+{
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+        *reinterpret_cast<float4 *>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+}
+template <int N>
+__device__ __forceinline__ void store_row(__half *p, const float (&x)[N])
+{
+#pragma unroll
+    for (int i = 0; i < N; i += 8)
+        *reinterpret_cast<uint4 *>(p + i) = make_uint4(pack16(x[i], x[i + 1]), pack16(x[i + 2], x[i + 3]),
+                                                       pack16(x[i + 4], x[i + 5]), pack16(x[i + 6], x[i + 7]));
+}
+template <int N>
+__device__ __forceinline__ void store_row(__nv_bfloat16 *p, const float (&x)[N])
+{
+#pragma unroll
+    for (int i = 0; i < N; i += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x[i + 2 * j], x[i + 2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        *reinterpret_cast<uint4 *>(p + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// (row, head) vectors of one KV head that a CTA's columns hold
+template <bool SPLIT, int NT>
+constexpr int group_vectors()
+{
+    return SPLIT ? 4 * NT : 8 * NT;
+}
+
+// tiles of all pairs of sequence s
+template <int GV>
+__device__ __forceinline__ long long seq_tiles(const FewParams &p, int n, int len, int &tiles, int &groups)
+{
+    const int vectors = n * (p.a.n_heads / p.a.c.n_kv);
+    tiles = (int)(((long long)len + n + FT - 1) / FT);
+    groups = vectors > p.many ? 0 : (vectors + GV - 1) / GV;
+    return (long long)tiles * groups * p.a.c.n_kv;
+}
+
+// T: type of the rows; SPLIT: two f16 pieces per value (f32 rows); NT: columns / 8
+template <class T, int D, bool SPLIT, int NT>
+__global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_constant__ FewParams p)
+{
+    using Lay = FewLay<D>;
+    constexpr int GV = group_vectors<SPLIT, NT>();
+    constexpr int KS = D / 16;    // k steps of q.k
+    constexpr int LD = D / 4;     // dims of q.k a lane holds: LD*t ..
+    constexpr int LV = D / 8;     // dims of the output a lane holds: LV*gl ..
+    constexpr int MT = D / 16;    // 16-dim tiles of the output
+    constexpr int ST = Lay::STAGES;
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t4 = lane & 3;
+    const Kv8Attn &a = p.a;
+    const int rep = a.n_heads / a.c.n_kv, page = a.c.page;
+    griddep_launch_dependents();
+
+    uint8_t *ring = smem + warp * Lay::RING;
+    Tile *rec = reinterpret_cast<Tile *>(smem + Lay::tile_off) + warp * Lay::TILES;
+    uint64_t *bar = reinterpret_cast<uint64_t *>(smem + Lay::bar_off) + warp * ST;
+    if (lane == 0) {
+        for (int i = 0; i < ST; i++)
+            mbar_init(&bar[i], 1);
+        fence_mbar_init();
+    }
+
+    // ---- this warp's range of tiles: warp `slot` of all warps, numbered so that
+    // few tiles spread over all SMs
+    __shared__ long long s_sum[FW], s_at[FW];
+    __shared__ int s_seq[FW];
+    auto tiles_of = [&](int s) -> long long {
+        int r0, n, len, tiles, groups;
+        if (s >= a.b.n_seqs)
+            return 0;
+        kv8_seq(a.b, s, a.err, r0, n, len);
+        return n ? seq_tiles<GV>(p, n, len, tiles, groups) : 0;
+    };
+    auto block_scan = [&](long long c, long long &all) { // exclusive sum over the threads, and the sum
+        long long x = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o)
+                x += y;
+        }
+        __syncthreads();
+        if (lane == 31)
+            s_sum[warp] = x;
+        __syncthreads();
+        all = 0;
+        long long before = 0;
+#pragma unroll
+        for (int w = 0; w < FW; w++) {
+            before += w < warp ? s_sum[w] : 0;
+            all += s_sum[w];
+        }
+        return before + x - c;
+    };
+    long long total = 0, all;
+    const long long c0 = tiles_of(threadIdx.x), e0 = block_scan(c0, all);
+    total = all;
+    for (int s0 = FW * 32; s0 < a.b.n_seqs; s0 += FW * 32) {
+        block_scan(tiles_of(s0 + threadIdx.x), all);
+        total += all;
+    }
+    const int slots = gridDim.x * FW;
+    const int active = (int)min((long long)slots, total);
+    if (threadIdx.x < FW)
+        s_seq[threadIdx.x] = 0;
+    __syncthreads();
+    long long base = 0;
+    for (int s0 = 0; s0 < a.b.n_seqs; s0 += FW * 32) { // the sequence that holds each warp's first tile
+        const int s = s0 + threadIdx.x;
+        const long long c = s0 ? tiles_of(s) : c0;
+        const long long e = base + (s0 ? block_scan(c, all) : e0);
+        if (s0 == 0 && a.b.n_seqs > FW * 32)
+            block_scan(c0, all);
+        for (int w = 0; w < FW; w++) {
+            const long long to = w * (long long)gridDim.x + blockIdx.x, u = to < active ? total * to / active : -1;
+            if (u >= e && u < e + c) {
+                s_seq[w] = s;
+                s_at[w] = e;
+            }
+        }
+        base += all;
+    }
+    __syncthreads();
+    const int slot = warp * gridDim.x + blockIdx.x;
+    const long long lo = slot < active ? total * slot / active : 0;
+    const long long hi = slot < active ? total * (slot + 1) / active : 0;
+    if (lane < 2)
+        p.head[slot * 2 + lane] = make_int4(0, 0, 0, PIECE_NONE);
+    if (lo == hi)
+        return;
+    int win_s = s_seq[warp];
+    long long win_base = s_at[warp]; // first tile of sequence win_s
+
+    // ---- tile records, 32 at a time: lane i describes tile `from + i`
+    int made = 0; // records made so far
+    auto describe = [&]() {
+        const long long from = lo + made;
+        int r0 = 0, n = 0, len = 0, tiles = 0, groups = 0;
+        long long c = 0, incl = 0;
+        for (;;) { // the window of 32 sequences that holds `from`
+            const int s = win_s + lane;
+            n = 0;
+            c = 0;
+            if (s < a.b.n_seqs) {
+                kv8_seq(a.b, s, a.err, r0, n, len);
+                c = n ? seq_tiles<GV>(p, n, len, tiles, groups) : 0;
+            }
+            incl = c;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o)
+                    incl += y;
+            }
+            const long long all = __shfl_sync(0xffffffffu, incl, 31);
+            if (from < win_base + all || win_s + 32 >= a.b.n_seqs)
+                break;
+            win_base += all;
+            win_s += 32;
+        }
+        const long long u = from + lane - win_base;
+        int j = 0; // sequences of the window that end at or before u
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const long long e = __shfl_sync(0xffffffffu, incl, j + o - 1);
+            if (e <= u)
+                j += o;
+        }
+        const long long window = __shfl_sync(0xffffffffu, incl, 31);
+        const bool here = from + lane < hi && u < window;
+        const int jj = j & 31;
+        const long long first = __shfl_sync(0xffffffffu, incl - c, jj);
+        Tile x;
+        x.s = win_s + jj;
+        x.n_tiles = __shfl_sync(0xffffffffu, tiles, jj);
+        x.len = __shfl_sync(0xffffffffu, len, jj);
+        x.r0 = __shfl_sync(0xffffffffu, r0, jj);
+        x.n = __shfl_sync(0xffffffffu, n, jj);
+        const int ng = __shfl_sync(0xffffffffu, groups, jj);
+        if (here) {
+            const long long r = u - first;
+            const int pair = (int)(r / x.n_tiles);
+            x.tile = (int)(r - (long long)pair * x.n_tiles);
+            x.g = pair / ng; // the groups of a KV head follow one another and share its codes in the L2
+            x.group = pair - x.g * ng;
+            const int t0 = x.tile * FT;
+            auto piece = [&](int pos, int &row, float &ks, float &vs) {
+                row = -1;
+                ks = vs = 0.0f;
+                if (pos >= x.len + x.n)
+                    return;
+                const int id = kv8_page(a.b, a.c, x.s, pos / page, a.err);
+                if (id < 0)
+                    return;
+                const size_t at = (size_t)id * a.c.n_kv + x.g;
+                row = (int)(at * page) + pos % page;
+                ks = a.c.ks[at];
+                vs = a.c.vs[at];
+            };
+            piece(t0, x.row0, x.ks0, x.vs0);
+            if (page == 16) {
+                piece(t0 + 16, x.row1, x.ks1, x.vs1);
+            } else {
+                x.row1 = x.row0;
+                x.ks1 = x.ks0;
+                x.vs1 = x.vs0;
+            }
+            x.pad0 = x.pad1 = 0;
+            const int4 *src = reinterpret_cast<const int4 *>(&x);
+            int4 *dst = reinterpret_cast<int4 *>(&rec[(made + lane) & (Lay::TILES - 1)]);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                dst[i] = src[i];
+        }
+        made += __popc(__ballot_sync(0xffffffffu, here));
+        __syncwarp();
+    };
+
+    const int mine = (int)(hi - lo);
+    const uint64_t policy = policy_evict_first();
+    auto issue = [&](int i) { // lane 0: tile i into stage i % ST
+        const Tile &x = rec[i & (Lay::TILES - 1)];
+        uint8_t *dst = ring + (i % ST) * 2 * Lay::BOX;
+        uint64_t *b = &bar[i % ST];
+        const int row0 = x.row0, row1 = x.row1;
+        if (page == 16) {
+            const uint32_t bytes = (row0 >= 0 ? Lay::BOX : 0) + (row1 >= 0 ? Lay::BOX : 0);
+            mbar_arrive_expect_tx(b, bytes);
+            if (row0 >= 0) {
+                tma_box(dst, &p.tk, row0, b, policy);
+                tma_box(dst + Lay::BOX, &p.tv, row0, b, policy);
+            }
+            if (row1 >= 0) {
+                tma_box(dst + Lay::BOX / 2, &p.tk, row1, b, policy);
+                tma_box(dst + Lay::BOX + Lay::BOX / 2, &p.tv, row1, b, policy);
+            }
+        } else {
+            mbar_arrive_expect_tx(b, row0 >= 0 ? 2 * Lay::BOX : 0);
+            if (row0 >= 0) {
+                tma_box(dst, &p.tk, row0, b, policy);
+                tma_box(dst + Lay::BOX, &p.tv, row0, b, policy);
+            }
+        }
+    };
+
+    // ---- the pair in progress
+    uint32_t qf[NT][KS][2];     // q as B fragments
+    float acc[MT][NT][4];       // O^T: (dim row gl / gl+8, column 2t4 / 2t4+1)
+    float m[NT][2], l[NT][2], fac[NT][2];
+    int lim[NT][2];             // last position the column's row attends to
+    auto begin = [&](const Tile &x) {
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const int v = x.group * GV + (SPLIT ? 4 * j + (gl & 3) : 8 * j + gl);
+            const int row = v / rep, head = x.g * rep + v % rep;
+            const bool live = row < x.n;
+            float q[LD];
+            float big = 0.0f;
+            if (live) {
+                const T *src = reinterpret_cast<const T *>(a.q) + (size_t)(x.r0 + row) * a.ld_q + (size_t)head * D;
+                constexpr int H = D / 2;
+                const int d0 = LD * t4, other = d0 ^ H;
+                const float sign = d0 < H ? -1.0f : 1.0f;
+                const size_t at = (size_t)(x.len + row) * H + (d0 & (H - 1));
+#pragma unroll
+                for (int i = 0; i < LD; i += 4) {
+                    const float4 w = kv8_load4(src + d0 + i);
+                    q[i] = w.x, q[i + 1] = w.y, q[i + 2] = w.z, q[i + 3] = w.w;
+                    if (a.r.cos) {
+                        const float4 o = kv8_load4(src + other + i), c = kv8_load4(a.r.cos + at + i),
+                                     s = kv8_load4(a.r.sin + at + i);
+                        // lower half: x c - y s; upper half: y s + x c
+                        q[i] = __fadd_rn(__fmul_rn(w.x, c.x), sign * __fmul_rn(o.x, s.x));
+                        q[i + 1] = __fadd_rn(__fmul_rn(w.y, c.y), sign * __fmul_rn(o.y, s.y));
+                        q[i + 2] = __fadd_rn(__fmul_rn(w.z, c.z), sign * __fmul_rn(o.z, s.z));
+                        q[i + 3] = __fadd_rn(__fmul_rn(w.w, c.w), sign * __fmul_rn(o.w, s.w));
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < LD; i++)
+                    big = fmaxf(big, fabsf(q[i]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < LD; i++)
+                    q[i] = 0.0f;
+            }
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            // a power of two brings the vector's largest value into [1, 2): f16 holds it with
+            // its eleven bits whatever q's magnitude
+            int e = (int)((__float_as_uint(big) >> 23) & 255u) - 127;
+            e = max(-126, min(126, e));
+            const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float x0 = q[4 * k + 2 * h] * down, x1 = q[4 * k + 2 * h + 1] * down;
+                    const uint32_t w = pack16(x0, x1);
+                    if constexpr (SPLIT) {
+                        const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+                        qf[j][k][h] = gl < 4 ? w : pack16(x0 - r.x, x1 - r.y);
+                    } else {
+                        qf[j][k][h] = w;
+                    }
+                }
+            const float f = up * a.scale * 1.4426950408889634f; // scores in powers of two
+            const int pos = live ? x.len + row : -1;
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const int from = (SPLIT ? (2 * t4 + c) & 3 : 2 * t4 + c) * 4;
+                fac[j][c] = __shfl_sync(0xffffffffu, f, from);
+                lim[j][c] = __shfl_sync(0xffffffffu, pos, from);
+                m[j][c] = -INFINITY;
+                l[j][c] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    acc[i][j][c] = 0.0f;
+        }
+    };
+
+    auto consume = [&](const Tile &x, const uint8_t *kb, const uint8_t *vb) {
+        float s[2][NT][4];
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++) {
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    s[mt][j][c] = 0.0f;
+            // the lane's LD codes of tokens gl and gl + 8, in 16-byte units
+#pragma unroll
+            for (int u = 0; u < LD / 16; u++) {
+                uint4 w[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int r = mt * 16 + h * 8 + gl;
+                    const int unit = (LD / 16) * t4 + u;
+                    const int sw = D == 128 ? unit ^ (r & 7) : unit ^ ((r >> 1) & 3);
+                    w[h] = *reinterpret_cast<const uint4 *>(kb + r * D + sw * 16);
+                }
+                const uint32_t w0[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, w1[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t x0 = w0[k] ^ 0x80808080u, x1 = w1[k] ^ 0x80808080u;
+                    const uint32_t a0 = codes_f16(x0, 0x4140), a2 = codes_f16(x0, 0x4342);
+                    const uint32_t a1 = codes_f16(x1, 0x4140), a3 = codes_f16(x1, 0x4342);
+#pragma unroll
+                    for (int j = 0; j < NT; j++)
+                        mma16816(s[mt][j], a0, a1, a2, a3, qf[j][4 * u + k][0], qf[j][4 * u + k][1]);
+                }
+            }
+        }
+        // values of the tile's tokens 2t4, 2t4+1, 2t4+8, 2t4+9 (each half): the lane's LV dims
+        const float vmax = fmaxf(x.vs0, x.vs1);
+        const float rel0 = page == 16 ? (vmax > 0.0f ? x.vs0 / vmax : 0.0f) * P_SCALE : P_SCALE;
+        const float rel1 = page == 16 ? (vmax > 0.0f ? x.vs1 / vmax : 0.0f) * P_SCALE : P_SCALE;
+        const float vscale = (page == 16 ? vmax : x.vs0) * (1.0f / P_SCALE);
+        const int t0 = x.tile * FT;
+        const bool whole = t0 + FT <= x.len + 1 && x.row0 >= 0 && x.row1 >= 0;
+        uint32_t pf[2][NT][2]; // P as B fragments
+        float corr[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            float tm[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++) {
+                const float ks = mt ? x.ks1 : x.ks0;
+                const bool there = (mt ? x.row1 : x.row0) >= 0;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    float y = s[mt][j][c];
+                    if constexpr (SPLIT)
+                        y += __shfl_xor_sync(0xffffffffu, y, 2);
+                    y *= ks * fac[j][c & 1];
+                    if (!whole && !(there && t0 + mt * 16 + (c >> 1) * 8 + gl <= lim[j][c & 1]))
+                        y = -INFINITY;
+                    s[mt][j][c] = y;
+                    tm[c & 1] = fmaxf(tm[c & 1], y);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1)
+                    tm[c] = fmaxf(tm[c], __shfl_xor_sync(0xffffffffu, tm[c], o));
+                const float mn = fmaxf(m[j][c], tm[c]);
+                const float ref = mn == -INFINITY ? 0.0f : mn; // nothing seen yet: every p is exp2(-inf)
+                corr[j][c] = ex2(m[j][c] - ref);
+                m[j][c] = mn;
+                tm[c] = ref;
+            }
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++) {
+                const float rel = mt ? rel1 : rel0;
+                float e[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    e[c] = ex2(s[mt][j][c] - tm[c & 1]);
+                    sum[c & 1] += e[c];
+                    e[c] *= rel;
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t w = pack16(e[2 * h], e[2 * h + 1]);
+                    if constexpr (SPLIT) {
+                        const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+                        const uint32_t rest = pack16(e[2 * h] - r.x, e[2 * h + 1] - r.y);
+                        w = t4 < 2 ? w : rest;
+                    }
+                    pf[mt][j][h] = transpose8x8(w);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; c++)
+                l[j][c] = l[j][c] * corr[j][c] + sum[c];
+        }
+        // O^T += V^T P: the tile's product in fresh accumulators, then one f32 step
+        constexpr int W = LV / 4; // 32-bit words of a token's LV codes
+        uint32_t vw[2][4][W];
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int r = mt * 16 + 2 * t4 + (i & 1) + (i >> 1) * 8;
+                if constexpr (D == 128) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(vb + r * D + ((gl ^ (r & 7)) << 4));
+                    vw[mt][i][0] = w.x, vw[mt][i][1] = w.y, vw[mt][i][2] = w.z, vw[mt][i][3] = w.w;
+                } else {
+                    const uint2 w = *reinterpret_cast<const uint2 *>(
+                        vb + r * D + (((gl >> 1) ^ ((r >> 1) & 3)) << 4) + (gl & 1) * 8);
+                    vw[mt][i][0] = w.x, vw[mt][i][1] = w.y;
+                }
+            }
+#pragma unroll
+        for (int k = 0; k < W; k++) {
+            float f[2][NT][4];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        f[i][j][c] = 0.0f;
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++) {
+                // bytes (token, dim) -> per dim the token pairs (0, 1) and (2, 3)
+                const uint32_t x01 = __byte_perm(vw[mt][0][k], vw[mt][1][k], 0x5140) ^ 0x80808080u;
+                const uint32_t y01 = __byte_perm(vw[mt][0][k], vw[mt][1][k], 0x7362) ^ 0x80808080u;
+                const uint32_t x23 = __byte_perm(vw[mt][2][k], vw[mt][3][k], 0x5140) ^ 0x80808080u;
+                const uint32_t y23 = __byte_perm(vw[mt][2][k], vw[mt][3][k], 0x7362) ^ 0x80808080u;
+                const uint32_t a0 = codes_f16(x01, 0x4140), a1 = codes_f16(x01, 0x4342);
+                const uint32_t a2 = codes_f16(x23, 0x4140), a3 = codes_f16(x23, 0x4342);
+                const uint32_t b0 = codes_f16(y01, 0x4140), b1 = codes_f16(y01, 0x4342);
+                const uint32_t b2 = codes_f16(y23, 0x4140), b3 = codes_f16(y23, 0x4342);
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    mma16816(f[0][j], a0, a1, a2, a3, pf[mt][j][0], pf[mt][j][1]);
+                    mma16816(f[1][j], b0, b1, b2, b3, pf[mt][j][0], pf[mt][j][1]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        acc[2 * k + i][j][c] = acc[2 * k + i][j][c] * corr[j][c & 1] + f[i][j][c] * vscale;
+        }
+    };
+
+    // the pair's segment is over: write it out, or keep it as a piece
+    auto finish = [&](const Tile &x, bool from_start, bool to_end) {
+        const bool done = from_start && to_end;
+        const int which = from_start ? 1 : 0;
+        float *part = p.part + ((size_t)slot * 2 + which) * GV * (D + 2);
+        if (!done && lane == 0)
+            p.head[slot * 2 + which] = make_int4(x.s, x.group, x.g, to_end ? PIECE_END : PIECE_OPEN);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                float sum = l[j][c];
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1)
+                    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                float o[LV]; // dims LV*gl ..
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        float y = acc[i][j][2 * h + c];
+                        if constexpr (SPLIT)
+                            y += __shfl_xor_sync(0xffffffffu, y, 2);
+                        o[2 * i + h] = y;
+                    }
+                const int vi = SPLIT ? 4 * j + 2 * t4 + c : 8 * j + 2 * t4 + c; // vector within the group
+                const int v = x.group * GV + vi;
+                if ((SPLIT && t4 >= 2) || v >= x.n * rep)
+                    continue;
+                if (done) {
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+                    for (int i = 0; i < LV; i++)
+                        o[i] *= inv;
+                    T *out = reinterpret_cast<T *>(a.out) + (size_t)(x.r0 + v / rep) * a.ld_out +
+                             (size_t)(x.g * rep + v % rep) * D + LV * gl;
+                    store_row<LV>(out, o);
+                } else {
+                    float *dst = part + (size_t)vi * D + LV * gl;
+                    store_row<LV>(dst, o);
+                    if (gl == 0) {
+                        part[(size_t)GV * D + vi] = m[j][c];
+                        part[(size_t)GV * (D + 1) + vi] = sum;
+                    }
+                }
+            }
+        }
+    };
+
+    describe();
+    int issued = 0;
+    if (lane == 0)
+        for (; issued < ST && issued < min(made, mine); issued++)
+            issue(issued);
+    issued = __shfl_sync(0xffffffffu, issued, 0);
+    bool ok = true, from_start = false;
+    int done = 0; // tiles consumed
+    for (int i = 0; i < mine; i++) {
+        // records ahead of the loads: a batch is made when the last one is half used
+        if (made < mine && made - i <= 32)
+            describe();
+        if (lane == 0)
+            for (; issued < min(made, mine) && issued < i + ST; issued++)
+                issue(issued);
+        const Tile x = rec[i & (Lay::TILES - 1)];
+        if (i == 0 || x.tile == 0) {
+            from_start = x.tile == 0;
+            begin(x);
+        }
+        if (ok)
+            ok = mbar_wait(&bar[i % ST], (uint32_t)((i / ST) & 1), a.err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok)
+            break;
+        const uint8_t *kb = ring + (i % ST) * 2 * Lay::BOX;
+        consume(x, kb, kb + Lay::BOX);
+        done++;
+        __syncwarp();
+        if (lane == 0) {
+            fence_proxy_async_smem(); // this warp's reads of the stage precede its refill
+            if (issued == i + ST && issued < min(made, mine)) {
+                issue(issued);
+                issued++;
+            }
+        }
+        const bool to_end = x.tile == x.n_tiles - 1;
+        if (to_end || i == mine - 1)
+            finish(x, from_start, to_end);
+    }
+    if (!ok && lane == 0) // copies in flight land before the shared memory goes
+        for (; done < issued; done++)
+            for (int it = 0; it < 100000 && !mbar_try_wait(&bar[done % ST], (uint32_t)((done / ST) & 1)); it++)
+                ;
+}
+
+// Join the pieces of each pair that no warp had to itself, in the order of its
+// tiles: the second slot of the warp that began it, then the first slots of the
+// warps behind, up to the one that ended it.  A task is one vector of one such
+// pair; every block lists the pairs and takes every gridDim.x-th task.
+template <class T, int D, int GV>
+__global__ void __launch_bounds__(JT) kv8_join_kernel(Kv8Attn a, const float *part, const int4 *head, int slots)
+{
+    __shared__ int s_owner[F_WARPS];
+    __shared__ float s_w[F_WARPS];
+    __shared__ int s_count, s_end;
+    __shared__ float s_red[JT / 32];
+    griddep_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rep = a.n_heads / a.c.n_kv;
+    const size_t stride = (size_t)GV * (D + 2);
+    int count = 0; // pairs begun and not ended by one warp, in order
+    for (int w0 = 0; w0 < slots; w0 += JT) {
+        const int w = w0 + threadIdx.x;
+        const bool open = w < slots && head[2 * w + 1].w == PIECE_OPEN;
+        const unsigned b = __ballot_sync(0xffffffffu, open);
+        __syncthreads();
+        if (lane == 0)
+            s_red[warp] = __int_as_float(__popc(b));
+        __syncthreads();
+        int at = count;
+        for (int i = 0; i < JT / 32; i++) {
+            at += i < warp ? __float_as_int(s_red[i]) : 0;
+            count += __float_as_int(s_red[i]);
+        }
+        if (open)
+            s_owner[at + __popc(b & ((1u << lane) - 1))] = w;
+    }
+    for (int task = blockIdx.x; task < count * GV; task += gridDim.x) {
+        __syncthreads();
+        const int w = s_owner[task / GV], vi = task % GV;
+        const int4 h = head[2 * w + 1];
+        int r0, n, len;
+        kv8_seq(a.b, h.x, a.err, r0, n, len);
+        const int v = h.y * GV + vi;
+        if (v >= n * rep)
+            continue;
+        if (threadIdx.x == 0)
+            s_end = slots - 1;
+        __syncthreads();
+        for (int i0 = w + 1; i0 < slots; i0 += JT) { // the warp that ended the pair
+            const int i = i0 + threadIdx.x;
+            const bool end = i < slots && head[2 * i].w == PIECE_END;
+            if (end)
+                atomicMin(&s_end, i);
+            if (__syncthreads_or(end))
+                break;
+        }
+        const int pieces = s_end - w + 1;
+        const float *first = part + (size_t)(2 * w + 1) * stride, *rest = part + (size_t)(2 * (w + 1)) * stride;
+        auto piece = [&](int i) { return i ? rest + (size_t)(i - 1) * 2 * stride : first; };
+        float m = -INFINITY;
+        for (int i = threadIdx.x; i < pieces; i += JT) {
+            s_w[i] = piece(i)[(size_t)GV * D + vi];
+            m = fmaxf(m, s_w[i]);
+        }
+        m = warp_max(m);
+        if (lane == 0)
+            s_red[warp] = m;
+        __syncthreads();
+        for (int i = 0; i < JT / 32; i++)
+            m = fmaxf(m, s_red[i]);
+        __syncthreads();
+        m = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f;
+        for (int i = threadIdx.x; i < pieces; i += JT) {
+            const float e = ex2(s_w[i] - m);
+            s_w[i] = e;
+            l += e * piece(i)[(size_t)GV * (D + 1) + vi];
+        }
+        l = warp_sum(l);
+        if (lane == 0)
+            s_red[warp] = l;
+        __syncthreads();
+        l = 0.0f;
+        for (int i = 0; i < JT / 32; i++)
+            l += s_red[i];
+        const int d = threadIdx.x;
+        if (d < D) {
+            float o = s_w[0] * first[(size_t)vi * D + d];
+            const float *src = rest + (size_t)vi * D + d;
+#pragma unroll 8
+            for (int i = 1; i < pieces; i++)
+                o += s_w[i] * src[(size_t)(i - 1) * 2 * stride];
+            T *out = reinterpret_cast<T *>(a.out) + (size_t)(r0 + v / rep) * a.ld_out +
+                     (size_t)(h.z * rep + v % rep) * D + d;
+            *out = T(l == 0.0f ? 0.0f : o / l);
+        }
+    }
+}
+
+// a code pool as rows of D bytes in swizzled boxes of `rows` rows
+int encode_codes(CUtensorMap *map, const int8_t *codes, const Kv8 &c, int rows)
+{
+    auto fn = tensor_map_encoder();
+    if (!fn)
+        return fail(LLMRS_ECUDA, "cuTensorMapEncodeTiled unavailable");
+    cuuint64_t dims[2] = {(cuuint64_t)c.D, (cuuint64_t)c.n_pages * c.n_kv * c.page};
+    cuuint64_t strides[1] = {(cuuint64_t)c.D};
+    cuuint32_t box[2] = {(cuuint32_t)c.D, (cuuint32_t)rows};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(codes), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          c.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(LLMRS_ECUDA, "cuTensorMapEncodeTiled (code pool) failed (%d)", (int)r);
+    return LLMRS_OK;
+}
+
+template <class T, int D, bool SPLIT, int NT>
+int run_few(const FewParams &p, int ctas, cudaStream_t stream)
+{
+    constexpr int GV = group_vectors<SPLIT, NT>();
+    LLMRS_CUDA_TRY(launch(kv8_few_kernel<T, D, SPLIT, NT>, dim3(ctas), dim3(FW * 32), FewLay<D>::bytes, stream, false,
+                          p));
+    LLMRS_CUDA_TRY(launch(kv8_join_kernel<T, D, GV>, dim3(2 * ctas), dim3(JT), 0, stream, true, p.a,
+                          (const float *)p.part, (const int4 *)p.head, ctas * FW));
+    return LLMRS_OK;
+}
+
+template <class T, int D, bool SPLIT>
+int run_nt(const FewParams &p, int nt, int ctas, cudaStream_t stream)
+{
+    if (nt == 1)
+        return run_few<T, D, SPLIT, 1>(p, ctas, stream);
+    if (nt == 2)
+        return run_few<T, D, SPLIT, 2>(p, ctas, stream);
+    return run_few<T, D, SPLIT, 4>(p, ctas, stream);
+}
+
+template <class T, bool SPLIT>
+int run_d(const FewParams &p, int nt, int ctas, cudaStream_t stream)
+{
+    return p.a.c.D == 128 ? run_nt<T, 128, SPLIT>(p, nt, ctas, stream) : run_nt<T, 64, SPLIT>(p, nt, ctas, stream);
+}
+
+template <class T, bool SPLIT, int D, int NT>
+cudaError_t prepare_few()
+{
+    return cudaFuncSetAttribute(kv8_few_kernel<T, D, SPLIT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                FewLay<D>::bytes);
+}
+
+template <class T, bool SPLIT>
+cudaError_t prepare_all()
+{
+    cudaError_t e = prepare_few<T, SPLIT, 128, 1>();
+    if (e == cudaSuccess)
+        e = prepare_few<T, SPLIT, 128, 2>();
+    if (e == cudaSuccess)
+        e = prepare_few<T, SPLIT, 128, 4>();
+    if (e == cudaSuccess)
+        e = prepare_few<T, SPLIT, 64, 1>();
+    if (e == cudaSuccess)
+        e = prepare_few<T, SPLIT, 64, 2>();
+    if (e == cudaSuccess)
+        e = prepare_few<T, SPLIT, 64, 4>();
+    return e;
+}
+
+// columns / 8 for the average sequence's vectors per KV head: a longer sequence
+// takes several groups.  A column more than needed costs its products and
+// registers, a group more reads the codes again (from the L2, mostly).
+int few_nt(long long vectors, int per)
+{
+    return vectors <= per ? 1 : vectors <= 2 * per ? 2 : 4;
+}
+
+long long mean_vectors(int rep, int n_rows, int n_seqs)
+{
+    return n_seqs > 0 ? ((long long)n_rows + n_seqs - 1) / n_seqs * rep : 0;
 }
 
 } // namespace
 
-size_t kv8_attention_workspace(int, int, int, int) { return 256; }
-
-int kv8_prepare(void) { return LLMRS_OK; }
-
-int kv8_attention(const Kv8Attn &a, void *, int, cudaStream_t stream)
+size_t kv8_attention_workspace(int rep, int head_dim, int n_rows, int n_seqs)
 {
-    if (a.dtype == LLMRS_F32)
-        LLMRS_CUDA_TRY(run<float>(a, stream));
-    else if (a.dtype == LLMRS_BF16)
-        LLMRS_CUDA_TRY(run<__nv_bfloat16>(a, stream));
-    else
-        LLMRS_CUDA_TRY(run<__half>(a, stream));
+    // two pieces a warp, of the vectors of a group (16-bit rows: eight to a column tile)
+    const int gv = 8 * few_nt(mean_vectors(rep, n_rows, n_seqs), 4);
+    return (size_t)F_WARPS * 2 * (sizeof(int4) + (size_t)gv * (head_dim + 2) * sizeof(float));
+}
+
+int kv8_prepare(void)
+{
+    cudaError_t e = prepare_all<float, true>();
+    if (e == cudaSuccess)
+        e = prepare_all<__half, false>();
+    if (e == cudaSuccess)
+        e = prepare_all<__nv_bfloat16, false>();
+    if (e != cudaSuccess)
+        return fail(LLMRS_ECUDA, "kv8 kernel attributes: %s", cudaGetErrorString(e));
     return LLMRS_OK;
+}
+
+int kv8_attention(const Kv8Attn &a, void *ws, int sms, cudaStream_t stream)
+{
+    FewParams p{};
+    p.a = a;
+    LLMRS_TRY(encode_codes(&p.tk, a.c.kq, a.c, std::min(a.c.page, FT)));
+    LLMRS_TRY(encode_codes(&p.tv, a.c.vq, a.c, std::min(a.c.page, FT)));
+    p.head = reinterpret_cast<int4 *>(ws);
+    p.part = reinterpret_cast<float *>(p.head + 2 * F_WARPS);
+    p.many = INT32_MAX;
+    const int nt = few_nt(mean_vectors(a.n_heads / a.c.n_kv, a.b.n_rows, a.b.n_seqs), a.dtype == LLMRS_F32 ? 4 : 8);
+    const int ctas = std::min(sms, F_MAX_CTAS);
+    if (a.dtype == LLMRS_F32)
+        return run_d<float, true>(p, nt, ctas, stream);
+    if (a.dtype == LLMRS_BF16)
+        return run_d<__nv_bfloat16, false>(p, nt, ctas, stream);
+    return run_d<__half, false>(p, nt, ctas, stream);
 }
 
 } // namespace llmrs

@@ -695,7 +695,7 @@ int llmrs_kv8_attention_workspace(const llmrs_kv8 *cache, const llmrs_kv8_batch 
     LLMRS_TRY(check_batch(cache, batch));
     LLMRS_CHECK_ARG(bytes && n_rows >= 0 && n_heads > 0 && n_heads % cache->n_kv_heads == 0,
                     "kv8_attention_workspace: bad arguments");
-    *bytes = llmrs::kv8_attention_workspace(n_heads, cache->head_dim, n_rows, batch->n_seqs);
+    *bytes = llmrs::kv8_attention_workspace(n_heads / cache->n_kv_heads, cache->head_dim, n_rows, batch->n_seqs);
     return LLMRS_OK;
 }
 
@@ -709,6 +709,8 @@ int llmrs_kv8_attention(llmrs_ctx *ctx, const llmrs_kv8 *cache, const llmrs_kv8_
     LLMRS_CHECK_ARG(n_heads > 0 && n_heads <= 65535 && n_heads % cache->n_kv_heads == 0,
                     "kv8_attention: bad head counts %d/%d", n_heads, cache->n_kv_heads);
     LLMRS_TRY(check_rows("kv8_attention", cache, d_q, dtype, ld_q, n_rows, n_heads));
+    LLMRS_CHECK_ARG((long long)n_rows * n_heads <= INT32_MAX, "kv8_attention: %d rows of %d heads (at most 2^31 - 1)",
+                    n_rows, n_heads);
     LLMRS_TRY(check_rows("kv8_attention", cache, d_out, dtype, ld_out, n_rows, n_heads));
     LLMRS_TRY(check_rope("kv8_attention", d_rope_cos, d_rope_sin, n_pos));
     LLMRS_CHECK_ARG(scale >= 0.0f && scale <= 3.0e38f, "kv8_attention: scale must be finite and not negative");
@@ -718,7 +720,7 @@ int llmrs_kv8_attention(llmrs_ctx *ctx, const llmrs_kv8 *cache, const llmrs_kv8_
     OnDevice on(ctx->device);
     void *ws = nullptr;
     LLMRS_TRY(take_workspace(ctx, "kv8_attention", d_workspace, workspace_bytes,
-                             llmrs::kv8_attention_workspace(n_heads, cache->head_dim, n_rows, batch->n_seqs), &ws));
+                             llmrs::kv8_attention_workspace(n_heads / cache->n_kv_heads, cache->head_dim, n_rows, batch->n_seqs), &ws));
     Kv8Attn a{};
     a.c = kv8_of(cache);
     a.b = batch_of(cache, batch, n_rows, d_rope_cos, n_pos);

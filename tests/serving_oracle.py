@@ -69,15 +69,15 @@ def append(pool, row_start, lens, table, k, v, cos=None, sin=None):
 
 
 def attend(pool, row_start, lens, table, q, n_rows, cos=None, sin=None, scale=None):
-    """(out [n_rows, H, D] f64 with NaN where no row is, tol/2^-24 weights): q f32 [rows, H, D].
-    Also returns, per row and head, the pieces a tolerance is made of: sum p|v| [rows, H, D],
+    """out [n_rows, H, D] f64 (NaN where no row is) for q f32 [rows, H, D], and per row and head
+    the pieces a tolerance is made of: sum p|v| and sum |v| [rows, H, D],
     S2 = max_t scale*sqrt(sum_d (q_d k_td)^2), X = max_t |score| and T."""
     n_pages, kv, page, d = pool["kq"].shape
     heads = q.shape[1]
     rep = heads // kv
     scale = 1.0 / np.sqrt(d) if scale is None else scale
     out = np.full((n_rows, heads, d), np.nan)
-    mass, s2, xs, ts = np.zeros_like(out), np.zeros((n_rows, heads)), np.zeros((n_rows, heads)), np.zeros(n_rows)
+    mass, floor, s2, xs, ts = np.zeros_like(out), np.zeros_like(out), np.zeros((n_rows, heads)), np.zeros((n_rows, heads)), np.zeros(n_rows)
     for s, length in enumerate(lens):
         a, n = row_start[s], row_start[s + 1] - row_start[s]
         if n == 0:
@@ -108,17 +108,21 @@ def attend(pool, row_start, lens, table, q, n_rows, cos=None, sin=None, scale=No
                 p = np.where(l > 0, p / np.where(l > 0, l, 1), 0)
                 out[a:a + n, hh] = p @ v
                 mass[a:a + n, hh] = p @ np.abs(v)
+                floor[a:a + n, hh] = ok @ np.abs(v)
         ts[a:a + n] = pos + 1
-    return out, mass, s2, xs, ts
+    return out, mass, floor, s2, xs, ts
 
 
-def attend_tolerance(dtype, ref, mass, s2, xs, ts, d):
+def attend_tolerance(dtype, ref, mass, floor, s2, xs, ts, d):
     """How far a row may be off, roundings counted as independent (four standard deviations
     or more): u = 2^-24 for each f32 operation of the sums over T positions and over D
     products and of the exponent; for 16-bit rows also the rounding of q and of the
-    probabilities to f16 (2^-11 each) and of the result to its type."""
+    probabilities to f16 (2^-11 each) and of the result to its type.  A probability far below
+    the row's largest is held by f16 pieces at a scale of 2^14: their smallest step is 2^-24,
+    so it is off by half of that, 2^-39 of the largest, however small it is itself; with the
+    sum of the probabilities at least the largest, that adds 2^-39 sum |v|."""
     ts, s2, xs = ts[:, None, None], s2[..., None], xs[..., None]
-    tol = 2.0 ** -24 * (32 + 2 * np.sqrt(ts) + 8 * np.sqrt(d) * s2 + 4 * xs) * mass + 1e-30
+    tol = 2.0 ** -24 * (32 + 2 * np.sqrt(ts) + 8 * np.sqrt(d) * s2 + 4 * xs) * mass + 2.0 ** -39 * floor + 1e-30
     if dtype == "f32":
         return tol
     half_step = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11}[dtype]
