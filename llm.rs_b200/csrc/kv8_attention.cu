@@ -32,7 +32,7 @@
 #include <mutex>
 
 #include "gemv.cuh"
-#include "kv8.cuh"
+#include "kv8_core.cuh"
 
 namespace llmrs {
 
@@ -40,20 +40,15 @@ namespace {
 
 constexpr int FT = 32;        // tokens of a tile
 constexpr int FW = 8;         // warps of a CTA
-constexpr int F_MAX_CTAS = 160;
-constexpr int F_WARPS = F_MAX_CTAS * FW;
-constexpr int JT = 128;       // threads of the joining kernel
-constexpr float P_SCALE = 16384.0f; // probabilities are split at this scale: p in [0, 1] keeps 22 bits down to 2^-13
+constexpr int F_MAX_CTAS = JOIN_SLOTS / FW;
 
 struct FewParams {
     CUtensorMap tk, tv; // code pools as rows of D bytes
     Kv8Attn a;
     float *part;        // [warps][2][vectors][D + 2]
-    int4 *head;         // [warps][2] pieces: (sequence, group, KV head, state)
+    int4 *head;         // [warps]: a pair begun but not ended: (sequence, group, KV head, pieces)
     int many;           // sequences with more vectors per KV head than this are another kernel's
 };
-
-enum : int { PIECE_NONE = 0, PIECE_OPEN = 1, PIECE_END = 2 };
 
 // what a warp needs to know of one tile
 struct __align__(16) Tile {
@@ -99,63 +94,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
-}
-
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Two int8 codes, offset by 128 to unsigned bytes, as f16 values: the byte
-// under the exponent of 1024 is 1024 + code + 128, and the difference is exact.
-__device__ __forceinline__ uint32_t codes_f16(uint32_t biased, uint32_t select)
-{
-    const uint32_t w = __byte_perm(biased, 0x64646464u, select);
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&w), __floats2half2_rn(1152.0f, 1152.0f));
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
-__device__ __forceinline__ uint32_t pack16(float a, float b)
-{
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-
-// N (a multiple of 16/sizeof(T) ... 16) consecutive floats to a row of T
-template <int N>
-__device__ __forceinline__ void store_row(float *p, const float (&x)[N])
-{
-#pragma unroll
-    for (int i = 0; i < N; i += 4)
-        *reinterpret_cast<float4 *>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-}
-template <int N>
-__device__ __forceinline__ void store_row(__half *p, const float (&x)[N])
-{
-#pragma unroll
-    for (int i = 0; i < N; i += 8)
-        *reinterpret_cast<uint4 *>(p + i) = make_uint4(pack16(x[i], x[i + 1]), pack16(x[i + 2], x[i + 3]),
-                                                       pack16(x[i + 4], x[i + 5]), pack16(x[i + 6], x[i + 7]));
-}
-template <int N>
-__device__ __forceinline__ void store_row(__nv_bfloat16 *p, const float (&x)[N])
-{
-#pragma unroll
-    for (int i = 0; i < N; i += 8) {
-        uint32_t w[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(x[i + 2 * j], x[i + 2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t *>(&h);
-        }
-        *reinterpret_cast<uint4 *>(p + i) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
 }
 
 // (row, head) vectors of one KV head that a CTA's columns hold
@@ -266,8 +204,8 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
     const int slot = warp * gridDim.x + blockIdx.x;
     const long long lo = slot < active ? total * slot / active : 0;
     const long long hi = slot < active ? total * (slot + 1) / active : 0;
-    if (lane < 2)
-        p.head[slot * 2 + lane] = make_int4(0, 0, 0, PIECE_NONE);
+    if (lane == 0)
+        p.head[slot] = make_int4(0, 0, 0, 0);
     if (lo == hi)
         return;
     int win_s = s_seq[warp];
@@ -620,8 +558,10 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
         const bool done = from_start && to_end;
         const int which = from_start ? 1 : 0;
         float *part = p.part + ((size_t)slot * 2 + which) * GV * (D + 2);
-        if (!done && lane == 0)
-            p.head[slot * 2 + which] = make_int4(x.s, x.group, x.g, to_end ? PIECE_END : PIECE_OPEN);
+        if (from_start && !to_end && lane == 0) { // hi - 1 is tile x.tile; the range that holds the pair's last one
+            const long long end = hi - 1 + (x.n_tiles - 1 - x.tile);
+            p.head[slot] = make_int4(x.s, x.group, x.g, (int)(((end + 1) * active - 1) / total) - slot + 1);
+        }
 #pragma unroll
         for (int j = 0; j < NT; j++) {
 #pragma unroll
@@ -710,100 +650,6 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
                 ;
 }
 
-// Join the pieces of each pair that no warp had to itself, in the order of its
-// tiles: the second slot of the warp that began it, then the first slots of the
-// warps behind, up to the one that ended it.  A task is one vector of one such
-// pair; every block lists the pairs and takes every gridDim.x-th task.
-template <class T, int D, int GV>
-__global__ void __launch_bounds__(JT) kv8_join_kernel(Kv8Attn a, const float *part, const int4 *head, int slots)
-{
-    __shared__ int s_owner[F_WARPS];
-    __shared__ float s_w[F_WARPS];
-    __shared__ int s_count, s_end;
-    __shared__ float s_red[JT / 32];
-    griddep_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rep = a.n_heads / a.c.n_kv;
-    const size_t stride = (size_t)GV * (D + 2);
-    int count = 0; // pairs begun and not ended by one warp, in order
-    for (int w0 = 0; w0 < slots; w0 += JT) {
-        const int w = w0 + threadIdx.x;
-        const bool open = w < slots && head[2 * w + 1].w == PIECE_OPEN;
-        const unsigned b = __ballot_sync(0xffffffffu, open);
-        __syncthreads();
-        if (lane == 0)
-            s_red[warp] = __int_as_float(__popc(b));
-        __syncthreads();
-        int at = count;
-        for (int i = 0; i < JT / 32; i++) {
-            at += i < warp ? __float_as_int(s_red[i]) : 0;
-            count += __float_as_int(s_red[i]);
-        }
-        if (open)
-            s_owner[at + __popc(b & ((1u << lane) - 1))] = w;
-    }
-    for (int task = blockIdx.x; task < count * GV; task += gridDim.x) {
-        __syncthreads();
-        const int w = s_owner[task / GV], vi = task % GV;
-        const int4 h = head[2 * w + 1];
-        int r0, n, len;
-        kv8_seq(a.b, h.x, a.err, r0, n, len);
-        const int v = h.y * GV + vi;
-        if (v >= n * rep)
-            continue;
-        if (threadIdx.x == 0)
-            s_end = slots - 1;
-        __syncthreads();
-        for (int i0 = w + 1; i0 < slots; i0 += JT) { // the warp that ended the pair
-            const int i = i0 + threadIdx.x;
-            const bool end = i < slots && head[2 * i].w == PIECE_END;
-            if (end)
-                atomicMin(&s_end, i);
-            if (__syncthreads_or(end))
-                break;
-        }
-        const int pieces = s_end - w + 1;
-        const float *first = part + (size_t)(2 * w + 1) * stride, *rest = part + (size_t)(2 * (w + 1)) * stride;
-        auto piece = [&](int i) { return i ? rest + (size_t)(i - 1) * 2 * stride : first; };
-        float m = -INFINITY;
-        for (int i = threadIdx.x; i < pieces; i += JT) {
-            s_w[i] = piece(i)[(size_t)GV * D + vi];
-            m = fmaxf(m, s_w[i]);
-        }
-        m = warp_max(m);
-        if (lane == 0)
-            s_red[warp] = m;
-        __syncthreads();
-        for (int i = 0; i < JT / 32; i++)
-            m = fmaxf(m, s_red[i]);
-        __syncthreads();
-        m = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f;
-        for (int i = threadIdx.x; i < pieces; i += JT) {
-            const float e = ex2(s_w[i] - m);
-            s_w[i] = e;
-            l += e * piece(i)[(size_t)GV * (D + 1) + vi];
-        }
-        l = warp_sum(l);
-        if (lane == 0)
-            s_red[warp] = l;
-        __syncthreads();
-        l = 0.0f;
-        for (int i = 0; i < JT / 32; i++)
-            l += s_red[i];
-        const int d = threadIdx.x;
-        if (d < D) {
-            float o = s_w[0] * first[(size_t)vi * D + d];
-            const float *src = rest + (size_t)vi * D + d;
-#pragma unroll 8
-            for (int i = 1; i < pieces; i++)
-                o += s_w[i] * src[(size_t)(i - 1) * 2 * stride];
-            T *out = reinterpret_cast<T *>(a.out) + (size_t)(r0 + v / rep) * a.ld_out +
-                     (size_t)(h.z * rep + v % rep) * D + d;
-            *out = T(l == 0.0f ? 0.0f : o / l);
-        }
-    }
-}
-
 // a code pool as rows of D bytes in swizzled boxes of `rows` rows
 int encode_codes(CUtensorMap *map, const int8_t *codes, const Kv8 &c, int rows)
 {
@@ -830,7 +676,7 @@ int run_few(const FewParams &p, int ctas, cudaStream_t stream)
     LLMRS_CUDA_TRY(launch(kv8_few_kernel<T, D, SPLIT, NT>, dim3(ctas), dim3(FW * 32), FewLay<D>::bytes, stream, false,
                           p));
     LLMRS_CUDA_TRY(launch(kv8_join_kernel<T, D, GV>, dim3(2 * ctas), dim3(JT), 0, stream, true, p.a,
-                          (const float *)p.part, (const int4 *)p.head, ctas * FW));
+                          (const float *)p.part, (const int4 *)p.head, ctas * FW, 0));
     return LLMRS_OK;
 }
 
@@ -893,7 +739,7 @@ size_t kv8_attention_workspace(int rep, int head_dim, int n_rows, int n_seqs)
 {
     // two pieces a warp, of the vectors of a group (16-bit rows: eight to a column tile)
     const int gv = 8 * few_nt(mean_vectors(rep, n_rows, n_seqs), 4);
-    return (size_t)F_WARPS * 2 * (sizeof(int4) + (size_t)gv * (head_dim + 2) * sizeof(float));
+    return JOIN_SLOTS * (sizeof(int4) + 2 * (size_t)gv * (head_dim + 2) * sizeof(float));
 }
 
 int kv8_prepare(void)
@@ -915,7 +761,7 @@ int kv8_attention(const Kv8Attn &a, void *ws, int sms, cudaStream_t stream)
     LLMRS_TRY(encode_codes(&p.tk, a.c.kq, a.c, std::min(a.c.page, FT)));
     LLMRS_TRY(encode_codes(&p.tv, a.c.vq, a.c, std::min(a.c.page, FT)));
     p.head = reinterpret_cast<int4 *>(ws);
-    p.part = reinterpret_cast<float *>(p.head + 2 * F_WARPS);
+    p.part = reinterpret_cast<float *>(p.head + JOIN_SLOTS);
     p.many = INT32_MAX;
     const int nt = few_nt(mean_vectors(a.n_heads / a.c.n_kv, a.b.n_rows, a.b.n_seqs), a.dtype == LLMRS_F32 ? 4 : 8);
     const int ctas = std::min(sms, F_MAX_CTAS);
