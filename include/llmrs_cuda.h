@@ -194,7 +194,8 @@ int llmrs_quantize_q4(llmrs_ctx *ctx, const float *d_w, size_t n, uint8_t *d_qs,
  * the reference (one sequence, contiguous f32 cache, src/core/layer.rs:114-128).
  *
  * Keys and values are int8 codes with one f32 scale for each (page, KV head);
- * a cached value is code * scale.  The caller owns every buffer.  All calls run
+ * a cached value is code * scale (scales are not negative).  The caller owns
+ * every buffer.  All calls run
  * on the context's stream on the context's device; none of them synchronises,
  * and with a workspace of the caller's none allocates, so they can be captured
  * into CUDA graphs (graphs that may run at the same time need a workspace

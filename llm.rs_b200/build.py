@@ -16,7 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libllmrs_cuda.so")
 SOURCES = ["prefill.cu", "sample.cu", "gemv.cu", "attention.cu", "ops.cu", "runtime.cu",
-           "kv8_cache.cu", "kv8_attention.cu", "verify.cu"]
+           "kv8_cache.cu", "kv8_attention.cu", "kv8_many.cu", "verify.cu"]
 
 
 def nvcc():

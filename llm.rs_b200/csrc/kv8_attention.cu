@@ -17,6 +17,8 @@
 // little.  int8 codes are exact in f16.  f32 rows: q and the probabilities are
 // split into two f16 pieces (22 bits and more), the pieces are columns of
 // their own in the same instruction, so one pass over the codes serves both.
+// f16 rows are split too: with one piece each, the roundings of q and P put
+// 3.4e-4 on the result where rounding the result itself costs 2.1e-4.
 //
 // Work: the tiles of all (sequence, vector group, KV head) pairs in one row,
 // cut into equal ranges, one per warp, whatever the lengths.  A warp streams
@@ -33,6 +35,7 @@
 
 #include "gemv.cuh"
 #include "kv8_core.cuh"
+#include "kv8_many.cuh"
 
 namespace llmrs {
 
@@ -435,10 +438,8 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
             }
         }
         // values of the tile's tokens 2t4, 2t4+1, 2t4+8, 2t4+9 (each half): the lane's LV dims
-        const float vmax = fmaxf(x.vs0, x.vs1);
-        const float rel0 = page == 16 ? (vmax > 0.0f ? x.vs0 / vmax : 0.0f) * P_SCALE : P_SCALE;
-        const float rel1 = page == 16 ? (vmax > 0.0f ? x.vs1 / vmax : 0.0f) * P_SCALE : P_SCALE;
-        const float vscale = (page == 16 ? vmax : x.vs0) * (1.0f / P_SCALE);
+        const float vs0 = x.vs0 * (1.0f / P_SCALE), vs1 = x.vs1 * (1.0f / P_SCALE);
+        const bool half = page == 16;
         const int t0 = x.tile * FT;
         const bool whole = t0 + FT <= x.len + 1 && x.row0 >= 0 && x.row1 >= 0;
         uint32_t pf[2][NT][2]; // P as B fragments
@@ -476,13 +477,12 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
             float sum[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int mt = 0; mt < 2; mt++) {
-                const float rel = mt ? rel1 : rel0;
                 float e[4];
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     e[c] = ex2(s[mt][j][c] - tm[c & 1]);
                     sum[c & 1] += e[c];
-                    e[c] *= rel;
+                    e[c] *= P_SCALE;
                 }
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
@@ -542,6 +542,17 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
                     mma16816(f[0][j], a0, a1, a2, a3, pf[mt][j][0], pf[mt][j][1]);
                     mma16816(f[1][j], b0, b1, b2, b3, pf[mt][j][0], pf[mt][j][1]);
                 }
+                if (half && mt == 0) { // pages of 16: the two halves have scales of their own
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+#pragma unroll
+                        for (int j = 0; j < NT; j++)
+#pragma unroll
+                            for (int c = 0; c < 4; c++) {
+                                acc[2 * k + i][j][c] = acc[2 * k + i][j][c] * corr[j][c & 1] + f[i][j][c] * vs0;
+                                f[i][j][c] = 0.0f;
+                            }
+                }
             }
 #pragma unroll
             for (int i = 0; i < 2; i++)
@@ -549,7 +560,8 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
                 for (int j = 0; j < NT; j++)
 #pragma unroll
                     for (int c = 0; c < 4; c++)
-                        acc[2 * k + i][j][c] = acc[2 * k + i][j][c] * corr[j][c & 1] + f[i][j][c] * vscale;
+                        acc[2 * k + i][j][c] = (half ? acc[2 * k + i][j][c] : acc[2 * k + i][j][c] * corr[j][c & 1]) +
+                                               f[i][j][c] * vs1;
         }
     };
 
@@ -733,43 +745,58 @@ long long mean_vectors(int rep, int n_rows, int n_seqs)
     return n_seqs > 0 ? ((long long)n_rows + n_seqs - 1) / n_seqs * rep : 0;
 }
 
+// vectors per KV head from which on a sequence goes to the kernel for many rows
+constexpr int MANY = 64;
+
+// whether a sequence may have that many: with no more rows than sequences (a
+// decode step) every sequence is taken to have few, which is right for any
+bool some_many(int rep, int n_rows, int n_seqs)
+{
+    return rep <= MANY_MAX_REP && n_rows > n_seqs && (long long)n_rows * rep > MANY;
+}
+
 } // namespace
 
 size_t kv8_attention_workspace(int rep, int head_dim, int n_rows, int n_seqs)
 {
     // two pieces a warp, of the vectors of a group (16-bit rows: eight to a column tile)
     const int gv = 8 * few_nt(mean_vectors(rep, n_rows, n_seqs), 4);
-    return JOIN_SLOTS * (sizeof(int4) + 2 * (size_t)gv * (head_dim + 2) * sizeof(float));
+    const size_t few = JOIN_SLOTS * (sizeof(int4) + 2 * (size_t)gv * (head_dim + 2) * sizeof(float));
+    return some_many(rep, n_rows, n_seqs) ? std::max(few, kv8_many_workspace(head_dim)) : few;
 }
 
 int kv8_prepare(void)
 {
     cudaError_t e = prepare_all<float, true>();
     if (e == cudaSuccess)
-        e = prepare_all<__half, false>();
+        e = prepare_all<__half, true>();
     if (e == cudaSuccess)
         e = prepare_all<__nv_bfloat16, false>();
     if (e != cudaSuccess)
         return fail(LLMRS_ECUDA, "kv8 kernel attributes: %s", cudaGetErrorString(e));
-    return LLMRS_OK;
+    return kv8_many_prepare();
 }
 
 int kv8_attention(const Kv8Attn &a, void *ws, int sms, cudaStream_t stream)
 {
+    const int rep = a.n_heads / a.c.n_kv;
+    const bool both = some_many(rep, a.b.n_rows, a.b.n_seqs);
+    if (both)
+        LLMRS_TRY(kv8_many(a, MANY, ws, sms, stream));
     FewParams p{};
     p.a = a;
     LLMRS_TRY(encode_codes(&p.tk, a.c.kq, a.c, std::min(a.c.page, FT)));
     LLMRS_TRY(encode_codes(&p.tv, a.c.vq, a.c, std::min(a.c.page, FT)));
     p.head = reinterpret_cast<int4 *>(ws);
     p.part = reinterpret_cast<float *>(p.head + JOIN_SLOTS);
-    p.many = INT32_MAX;
-    const int nt = few_nt(mean_vectors(a.n_heads / a.c.n_kv, a.b.n_rows, a.b.n_seqs), a.dtype == LLMRS_F32 ? 4 : 8);
+    p.many = both ? MANY : INT32_MAX;
+    const int nt = few_nt(mean_vectors(rep, a.b.n_rows, a.b.n_seqs), a.dtype == LLMRS_BF16 ? 8 : 4);
     const int ctas = std::min(sms, F_MAX_CTAS);
     if (a.dtype == LLMRS_F32)
         return run_d<float, true>(p, nt, ctas, stream);
     if (a.dtype == LLMRS_BF16)
         return run_d<__nv_bfloat16, false>(p, nt, ctas, stream);
-    return run_d<__half, false>(p, nt, ctas, stream);
+    return run_d<__half, true>(p, nt, ctas, stream);
 }
 
 } // namespace llmrs

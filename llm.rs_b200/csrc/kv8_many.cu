@@ -1,0 +1,797 @@
+// kv8_many.cu - causal attention over the paged 8-bit KV cache for many rows
+// per sequence (prompts, chunks of them): tcgen05 tensor cores (sm_100a).
+//
+// A CTA's tile is 128 vectors (row, query head) of one KV head by 128 tokens:
+//   S = Q K^T (128 x 128, K = D), P = exp2(S * ks - max) * vs, O = P V,
+// f16 operands, f32 accumulators in TMEM.  The codes are exact in f16.  f32
+// rows: Q and P are two f16 pieces each (22 bits and more), so the products
+// run twice; f16 rows: Q in two pieces, P in one; bf16 rows: one each.  Every
+// tile's O is a fresh product that registers add up in f32, with the change of
+// the maximum and the value scales applied there: long sums do not pass
+// through the tensor core's accumulator.
+//
+// Warpgroups: 0 softmax (thread = row; also rotates, scales and splits Q),
+// 1 output (thread = row, D accumulators), 2 codes to f16 in shared memory
+// (keys K-major, values MN-major, both 128-byte swizzled: the same image),
+// 3: one warp issues the products, one looks up pages and scales ahead.
+// S and O are double buffered (4 x 128 columns: all of TMEM), P lies over the S
+// it came from, K and V tiles are double buffered, so the product of tile i + 1
+// runs while tile i is in the softmax.
+//
+// Work: the tiles of all (sequence, KV head, tile of rows) in one row, cut into
+// equal consecutive ranges, one per CTA; pieces of a softmax that a range cuts
+// are joined by a second kernel (kv8_core.cuh).
+#include "gemv.cuh"
+#include "kv8_core.cuh"
+#include "kv8_many.cuh"
+
+namespace llmrs {
+
+namespace {
+
+constexpr int MB = 128;          // vectors, and tokens, of a tile
+constexpr int MANY_THREADS = 512;
+constexpr int INFO = 8;          // tile descriptions in flight
+constexpr int RING = 4;          // softmax -> output hand-overs in flight
+
+struct ManyTile {
+    int row[8];                  // pool rows of the tile's 16-token groups; -1: not there
+    float ks[8];                 // key scales
+    float lvs[8];                // log2 of the value scales (-inf: zero)
+    int first, last, masked;     // of the pair within this range; some row does not see all tokens
+    int tile, s, g, mt;          // which
+    int r0, n, len;              // of the sequence
+    int from_start, to_end, pieces;
+    int pad[3];
+};
+static_assert(sizeof(ManyTile) == 160, "16-byte words");
+
+struct ManyParams {
+    Kv8Attn a;
+    float *part;
+    int4 *head;
+    int many; // sequences with at most this many vectors per KV head are another kernel's
+};
+
+template <int D, int QP>
+struct ManyLay {
+    static constexpr int Q = MB * D * 2;   // bytes of one piece of Q; of an f16 K or V tile
+    static constexpr int k_off = QP * Q;
+    static constexpr int v_off = k_off + 2 * Q;
+    static constexpr int info_off = v_off + 2 * Q;
+    static constexpr int ring_off = info_off + INFO * (int)sizeof(ManyTile);
+    static constexpr int bar_off = ring_off + RING * 4 * MB * 4;
+    static constexpr int bytes = bar_off + 512 + 1024; // + alignment slack
+    static_assert(bytes <= 232448 - 256, "shared memory of one CTA");
+};
+
+enum : int { // barriers
+    B_INFO_FULL = 0,
+    B_INFO_EMPTY = B_INFO_FULL + INFO,
+    B_K_FULL = B_INFO_EMPTY + INFO,
+    B_K_EMPTY = B_K_FULL + 2,
+    B_V_FULL = B_K_EMPTY + 2,
+    B_V_EMPTY = B_V_FULL + 2,
+    B_S_FULL = B_V_EMPTY + 2,
+    B_P_FULL = B_S_FULL + 2,
+    B_O_FULL = B_P_FULL + 2,
+    B_O_EMPTY = B_O_FULL + 2,
+    B_Q_FULL = B_O_EMPTY + 2,
+    B_COUNT = B_Q_FULL + 1,
+};
+static_assert(B_COUNT * 8 <= 512, "barrier space");
+
+// ------------------------------------------------------------ tcgen05
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tc_commit(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                 : "memory");
+}
+
+// Operand tile in 128-byte-swizzled atoms of 8 rows x 128 bytes, 1024 bytes
+// apart.  K-major: rows are M or N, 64 K values each (lead unused).  MN-major:
+// rows are K, 64 M or N values each, `lead` bytes to the next 64.
+__device__ __forceinline__ uint64_t sw128(uint32_t saddr, uint32_t lead)
+{
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
+           ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+}
+
+// kind::f16: f16 x f16 -> f32, M = 128; B K-major or MN-major
+__host__ __device__ constexpr uint32_t idesc_f16(int n, bool b_mn)
+{
+    return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(MB >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, bool acc)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                 "l"(ad), "l"(bd), "r"(idesc), "r"((int)acc)
+                 : "memory");
+}
+
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t at, uint64_t bd, uint32_t idesc, bool acc)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+                 "r"(at), "l"(bd), "r"(idesc), "r"((int)acc)
+                 : "memory");
+}
+
+#define R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), \
+                 "=r"(r[o + 6]), "=r"(r[o + 7])
+#define T8(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), \
+                 "+r"(r[o + 6]), "+r"(r[o + 7])
+#define I8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), \
+                 "r"(r[o + 6]), "r"(r[o + 7])
+
+// 32 consecutive columns of this thread's TMEM lane; tm_wait makes them usable
+__device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+                 "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : R8(r, 0), R8(r, 8), R8(r, 16), R8(r, 24)
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tm_wait(uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : T8(r, 0), T8(r, 8), T8(r, 16), T8(r, 24) : : "memory");
+}
+__device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+                 "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::I8(r, 0),
+                 I8(r, 8), I8(r, 16), I8(r, 24), "r"(addr)
+                 : "memory");
+}
+#undef R8
+#undef T8
+#undef I8
+
+template <int N>
+__device__ __forceinline__ void regs_up()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// ------------------------------------------------------------ the tiles of a sequence
+// Tile of rows mt holds rows [mt*R, (mt+1)*R), whole rows of rep vectors each;
+// vector r of it is row mt*R + r / rep, head r % rep.  It needs the tokens up
+// to its last row's position.
+__device__ __forceinline__ int row_tiles(int n, int R) { return (n + R - 1) / R; }
+__device__ __forceinline__ int token_tiles(int len, int n, int R, int mt) { return (len + min(n, (mt + 1) * R) - 1) / MB + 1; }
+
+__device__ __forceinline__ long long head_tiles(int len, int n, int R)
+{
+    long long t = 0;
+    for (int mt = 0, m = row_tiles(n, R); mt < m; mt++)
+        t += token_tiles(len, n, R, mt);
+    return t;
+}
+
+// codes of 16 dims to f16, 32 bytes
+__device__ __forceinline__ void widen(uint4 w, uint4 &lo, uint4 &hi)
+{
+    const uint32_t x = w.x ^ 0x80808080u, y = w.y ^ 0x80808080u, z = w.z ^ 0x80808080u, t = w.w ^ 0x80808080u;
+    lo = make_uint4(codes_f16(x, 0x4140), codes_f16(x, 0x4342), codes_f16(y, 0x4140), codes_f16(y, 0x4342));
+    hi = make_uint4(codes_f16(z, 0x4140), codes_f16(z, 0x4342), codes_f16(t, 0x4140), codes_f16(t, 0x4342));
+}
+
+// QP, PP: f16 pieces of Q and of P
+template <class T, int D, int QP, int PP>
+__global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_constant__ ManyParams p)
+{
+    using Lay = ManyLay<D, QP>;
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    ManyTile *info = reinterpret_cast<ManyTile *>(smem + Lay::info_off);
+    float *ring = reinterpret_cast<float *>(smem + Lay::ring_off); // [RING][corr | scale of O | sum | max][MB]
+    uint64_t *bar = reinterpret_cast<uint64_t *>(smem + Lay::bar_off);
+    __shared__ uint32_t s_tmem;
+    __shared__ long long s_sum[MANY_THREADS / 32];
+    __shared__ long long s_at;
+    __shared__ int s_seq;
+    const Kv8Attn &a = p.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2;
+    const int rep = a.n_heads / a.c.n_kv, R = MB / rep;
+    griddep_launch_dependents();
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < INFO; i++) {
+            mbar_init(&bar[B_INFO_FULL + i], 1);
+            mbar_init(&bar[B_INFO_EMPTY + i], 13); // 12 warps and the issuing thread
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&bar[B_K_FULL + i], 128);
+            mbar_init(&bar[B_K_EMPTY + i], 1);
+            mbar_init(&bar[B_V_FULL + i], 128);
+            mbar_init(&bar[B_V_EMPTY + i], 1);
+            mbar_init(&bar[B_S_FULL + i], 1);
+            mbar_init(&bar[B_P_FULL + i], 128);
+            mbar_init(&bar[B_O_FULL + i], 1);
+            mbar_init(&bar[B_O_EMPTY + i], 128);
+        }
+        mbar_init(&bar[B_Q_FULL], 128);
+        fence_mbar_init();
+        s_seq = 0;
+    }
+
+    // ---- this CTA's range of tiles
+    auto tiles_of = [&](int s) -> long long {
+        int r0, n, len;
+        if (s >= a.b.n_seqs)
+            return 0;
+        kv8_seq(a.b, s, a.err, r0, n, len);
+        return (long long)n * rep > p.many ? a.c.n_kv * head_tiles(len, n, R) : 0;
+    };
+    auto block_scan = [&](long long c, long long &all) {
+        long long x = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o)
+                x += y;
+        }
+        __syncthreads();
+        if (lane == 31)
+            s_sum[warp] = x;
+        __syncthreads();
+        all = 0;
+        long long before = 0;
+#pragma unroll
+        for (int w = 0; w < MANY_THREADS / 32; w++) {
+            before += w < warp ? s_sum[w] : 0;
+            all += s_sum[w];
+        }
+        return before + x - c;
+    };
+    long long total, all;
+    const long long c0 = tiles_of(threadIdx.x), e0 = block_scan(c0, all), all0 = all;
+    total = all;
+    for (int s0 = MANY_THREADS; s0 < a.b.n_seqs; s0 += MANY_THREADS) {
+        block_scan(tiles_of(s0 + threadIdx.x), all);
+        total += all;
+    }
+    const int slot = blockIdx.x, active = (int)min((long long)gridDim.x, total);
+    const long long lo = slot < active ? total * slot / active : 0;
+    const long long hi = slot < active ? total * (slot + 1) / active : 0;
+    if (threadIdx.x == 0)
+        p.head[slot] = make_int4(0, 0, 0, 0);
+    if (lo == hi)
+        return;
+    long long base = 0;
+    for (int s0 = 0; s0 < a.b.n_seqs; s0 += MANY_THREADS) {
+        const long long c = s0 ? tiles_of(s0 + threadIdx.x) : c0;
+        const long long e = base + (s0 ? block_scan(c, all) : e0);
+        if (lo >= e && lo < e + c) {
+            s_seq = s0 + threadIdx.x;
+            s_at = lo - e;
+        }
+        base += s0 ? all : all0;
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_before();
+    }
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = s_tmem;
+    const int mine = (int)(hi - lo);
+    auto wait = [&](int b, int use) { return mbar_wait(&bar[b], (uint32_t)(use & 1), a.err); };
+    bool ok = true;
+
+    if (wg == 0) {
+        // ================================================= softmax: thread = row
+        regs_up<168>();
+        const int r = threadIdx.x;
+        const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+        float m = -INFINITY, l = 0.0f, fac = 0.0f;
+        int lim = -1;
+        bool busy = false; // some row of this warp is there
+        for (int i = 0; i < mine && ok; i++) {
+            const ManyTile &x = info[i % INFO];
+            if (!(ok = wait(B_INFO_FULL + i % INFO, i / INFO)))
+                break;
+            if (x.first) {
+                // rotate, scale and split the row's q; its last use was the products of the
+                // tile before, which this warpgroup has waited for
+                const int row = x.mt * R + r / rep, head = x.g * rep + r % rep;
+                const bool live = r < R * rep && row < x.n;
+                constexpr int H = D / 2;
+                float q[D];
+                float big = 0.0f;
+                if (live) {
+                    const T *src = reinterpret_cast<const T *>(a.q) + (size_t)(x.r0 + row) * a.ld_q + (size_t)head * D;
+                    const size_t at = (size_t)(x.len + row) * H;
+#pragma unroll
+                    for (int d = 0; d < H; d += 4) {
+                        const float4 u = kv8_load4(src + d), v = kv8_load4(src + H + d);
+                        float4 c = make_float4(1.0f, 1.0f, 1.0f, 1.0f), s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (a.r.cos) {
+                            c = kv8_load4(a.r.cos + at + d);
+                            s = kv8_load4(a.r.sin + at + d);
+                        }
+                        const float uu[4] = {u.x, u.y, u.z, u.w}, vv[4] = {v.x, v.y, v.z, v.w};
+                        const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            q[d + k] = a.r.cos ? __fsub_rn(__fmul_rn(uu[k], cc[k]), __fmul_rn(vv[k], ss[k])) : uu[k];
+                            q[H + d + k] = a.r.cos ? __fadd_rn(__fmul_rn(uu[k], ss[k]), __fmul_rn(vv[k], cc[k])) : vv[k];
+                        }
+                    }
+#pragma unroll
+                    for (int d = 0; d < D; d++)
+                        big = fmaxf(big, fabsf(q[d]));
+                } else {
+#pragma unroll
+                    for (int d = 0; d < D; d++)
+                        q[d] = 0.0f;
+                }
+                int e = (int)((__float_as_uint(big) >> 23) & 255u) - 127;
+                e = max(-126, min(126, e)); // a power of two brings the largest value into [1, 2)
+                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+                fac = __uint_as_float((uint32_t)(127 + e) << 23) * a.scale * 1.4426950408889634f;
+                lim = live ? x.len + row : -1;
+                busy = __any_sync(0xffffffffu, live);
+                m = -INFINITY;
+                l = 0.0f;
+#pragma unroll
+                for (int u = 0; u < D / 8; u++) { // 16-byte units of the swizzled K-major image
+                    uint32_t w[4], w2[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float x0 = q[8 * u + 2 * k] * down, x1 = q[8 * u + 2 * k + 1] * down;
+                        w[k] = pack16(x0, x1);
+                        if constexpr (QP == 2) {
+                            const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
+                            w2[k] = pack16(x0 - h.x, x1 - h.y);
+                        }
+                    }
+                    const int o = (u / 8) * (MB * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4);
+                    *reinterpret_cast<uint4 *>(smem + o) = make_uint4(w[0], w[1], w[2], w[3]);
+                    if constexpr (QP == 2)
+                        *reinterpret_cast<uint4 *>(smem + Lay::Q + o) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(&bar[B_Q_FULL]);
+            }
+            if (!(ok = wait(B_S_FULL + (i & 1), i >> 1)))
+                break;
+            tc_after();
+            const uint32_t sp = lanes + (uint32_t)(i & 1) * MB;
+            float corr = 1.0f, oscale = 0.0f;
+            if (busy) {
+                uint32_t s[4][32];
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    tm_ld32(sp + 32 * k, s[k]);
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    tm_wait(s[k]);
+                float kf[8];
+                float top = -INFINITY, ref2 = -INFINITY;
+#pragma unroll
+                for (int g = 0; g < 8; g++)
+                    kf[g] = fac * x.ks[g];
+                if (x.masked) { // scores themselves, the unseen ones at -inf
+#pragma unroll
+                    for (int g = 0; g < 8; g++) {
+                        const int last = x.row[g] >= 0 ? lim - x.tile * MB - 16 * g : -1;
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            uint32_t &w = s[g / 2][(g & 1) * 16 + j];
+                            w = __float_as_uint(j <= last ? __uint_as_float(w) * kf[g] : -INFINITY);
+                        }
+                        kf[g] = 1.0f;
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < 8; g++) {
+                    float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        t0 = fmaxf(t0, __uint_as_float(s[g / 2][(g & 1) * 16 + j]));
+                        t1 = fmaxf(t1, __uint_as_float(s[g / 2][(g & 1) * 16 + j + 1]));
+                    }
+                    t0 = fmaxf(t0, t1) * kf[g]; // kf >= 0
+                    top = fmaxf(top, t0);
+                    ref2 = fmaxf(ref2, t0 + x.lvs[g]);
+                }
+                const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.0f : mn;
+                corr = ex2(m - ref);
+                m = mn;
+                // P = p * vs against the row's own largest p * vs of the tile: f16 keeps its bits
+                // whatever the scales of pages that the row hardly sees
+                const bool none = ref2 == -INFINITY; // no seen page has a scale above 0
+                ref2 = none ? 0.0f : ref2 - P_SCALE_LOG2;
+                oscale = none ? 0.0f : ex2(ref2 - ref);
+                float sum = 0.0f;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t ph[32], pl[32];
+#pragma unroll
+                    for (int gg = 0; gg < 4; gg++) {
+                        const int g = 4 * h + gg;
+                        // a scale of zero: f16 holds the probabilities as zero, the sum keeps them
+                        const bool zero = x.lvs[g] == -INFINITY;
+                        const float add = zero ? -60.0f - ref : x.lvs[g] - ref2;
+                        const float back = zero ? 0x1p60f : ex2(fminf(ref2 - x.lvs[g] - ref, 120.0f));
+                        float g0 = 0.0f, g1 = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) {
+                            const float e0 = ex2(fmaf(__uint_as_float(s[g / 2][(g & 1) * 16 + j]), kf[g], add));
+                            const float e1 = ex2(fmaf(__uint_as_float(s[g / 2][(g & 1) * 16 + j + 1]), kf[g], add));
+                            g0 += e0;
+                            g1 += e1;
+                            const uint32_t w = pack16(e0, e1);
+                            ph[gg * 8 + j / 2] = w;
+                            if constexpr (PP == 2) {
+                                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+                                pl[gg * 8 + j / 2] = pack16(e0 - f.x, e1 - f.y);
+                            }
+                        }
+                        sum += (g0 + g1) * back;
+                    }
+                    tm_st32(sp + 32 * h, ph);
+                    if constexpr (PP == 2)
+                        tm_st32(sp + 64 + 32 * h, pl);
+                }
+                l = l * corr + sum;
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            }
+            float *hand = ring + (i % RING) * 4 * MB;
+            hand[r] = corr;
+            hand[MB + r] = oscale;
+            if (x.last) {
+                hand[2 * MB + r] = l;
+                hand[3 * MB + r] = m;
+            }
+            tc_before();
+            mbar_arrive(&bar[B_P_FULL + (i & 1)]);
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
+        }
+    } else if (wg == 1) {
+        // ================================================= output: thread = row
+        regs_up<176>();
+        const int r = threadIdx.x - 128;
+        const uint32_t lanes = tmem + 2 * MB + ((uint32_t)((warp & 3) * 32) << 16);
+        float acc[D];
+        for (int i = 0; i < mine && ok; i++) {
+            const ManyTile &x = info[i % INFO];
+            if (!(ok = wait(B_INFO_FULL + i % INFO, i / INFO) && wait(B_O_FULL + (i & 1), i >> 1)))
+                break;
+            tc_after();
+            const float *hand = ring + (i % RING) * 4 * MB;
+            const float corr = x.first ? 0.0f : hand[r], oscale = hand[MB + r];
+            float l = 0.0f, m = 0.0f;
+            if (x.last) {
+                l = hand[2 * MB + r];
+                m = hand[3 * MB + r];
+            }
+            if (x.first) {
+#pragma unroll
+                for (int d = 0; d < D; d++)
+                    acc[d] = 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < D / 32; k++) {
+                uint32_t o[32];
+                tm_ld32(lanes + (uint32_t)(i & 1) * MB + 32 * k, o);
+                tm_wait(o);
+                if (k == D / 32 - 1) {
+                    tc_before();
+                    mbar_arrive(&bar[B_O_EMPTY + (i & 1)]);
+                }
+#pragma unroll
+                for (int d = 0; d < 32; d++)
+                    acc[32 * k + d] = acc[32 * k + d] * corr + __uint_as_float(o[d]) * oscale;
+            }
+            if (x.last) {
+                const int row = x.mt * R + r / rep, head = x.g * rep + r % rep;
+                const bool done = x.from_start && x.to_end, live = r < R * rep && row < x.n;
+                if (!done && x.from_start && r == 0)
+                    p.head[slot] = make_int4(x.s, x.mt, x.g, x.pieces);
+                if (live && done) {
+                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                    T *out = reinterpret_cast<T *>(a.out) + (size_t)(x.r0 + row) * a.ld_out + (size_t)head * D;
+#pragma unroll
+                    for (int d = 0; d < D; d += 16) {
+                        float o[16];
+#pragma unroll
+                        for (int j = 0; j < 16; j++)
+                            o[j] = acc[d + j] * inv;
+                        store_row<16>(out + d, o);
+                    }
+                } else if (live) {
+                    float *part = p.part + ((size_t)slot * 2 + (x.from_start ? 1 : 0)) * MB * (D + 2);
+#pragma unroll
+                    for (int d = 0; d < D; d += 16) {
+                        float o[16];
+#pragma unroll
+                        for (int j = 0; j < 16; j++)
+                            o[j] = acc[d + j];
+                        store_row<16>(part + (size_t)r * D + d, o);
+                    }
+                    part[(size_t)MB * D + r] = m;
+                    part[(size_t)MB * (D + 1) + r] = l;
+                }
+            }
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
+        }
+    } else if (wg == 2) {
+        // ================================================= codes to f16
+        regs_down<112>();
+        constexpr int U = D / 16;            // 16-code units of a token
+        constexpr int N = MB * U / 128;      // units a thread widens per tile and operand
+        const int t = threadIdx.x - 256, j = t & 7;
+        // D = 128: eight lanes take half the units of two tokens, crosswise, so that
+        // the eight 16-byte stores of a pass fall into eight bank groups
+        auto place = [&](int n, int &tok, int &unit) {
+            if constexpr (D == 128) {
+                const int half = n & 1;
+                tok = 2 * ((t >> 3) + 16 * (n >> 1)) + (j >> 2);
+                unit = 4 * (half ^ (j >> 2)) + (j & 3);
+            } else {
+                tok = 2 * ((t >> 3) + 16 * n) + (j >> 2);
+                unit = j & 3;
+            }
+        };
+        auto load = [&](const int8_t *codes, const ManyTile &x, uint4 (&w)[N]) {
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                int tok, unit;
+                place(n, tok, unit);
+                const int row = x.row[tok >> 4];
+                w[n] = make_uint4(0, 0, 0, 0);
+                if (row >= 0)
+                    w[n] = __ldg(reinterpret_cast<const uint4 *>(codes + ((size_t)row + (tok & 15)) * D + unit * 16));
+            }
+        };
+        auto store = [&](uint8_t *dst, const uint4 (&w)[N]) {
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                int tok, unit;
+                place(n, tok, unit);
+                uint4 a0, a1;
+                widen(w[n], a0, a1);
+                uint8_t *b = dst + (unit >> 2) * (MB * 128) + tok * 128;
+                const int u = 2 * (unit & 3), sw = tok & 7;
+                *reinterpret_cast<uint4 *>(b + ((u ^ sw) << 4)) = a0;
+                *reinterpret_cast<uint4 *>(b + (((u + 1) ^ sw) << 4)) = a1;
+            }
+        };
+        uint4 kw[N], vw[N];
+        ok = wait(B_INFO_FULL, 0);
+        if (ok)
+            load(a.c.kq, info[0], kw);
+        for (int i = 0; i < mine && ok; i++) {
+            load(a.c.vq, info[i % INFO], vw);
+            if (!(ok = i < 2 || wait(B_K_EMPTY + (i & 1), (i >> 1) - 1)))
+                break;
+            store(smem + Lay::k_off + (i & 1) * Lay::Q, kw);
+            fence_proxy_async_smem();
+            mbar_arrive(&bar[B_K_FULL + (i & 1)]);
+            if (i + 1 < mine) {
+                if (!(ok = wait(B_INFO_FULL + (i + 1) % INFO, (i + 1) / INFO)))
+                    break;
+                load(a.c.kq, info[(i + 1) % INFO], kw);
+            }
+            if (!(ok = i < 2 || wait(B_V_EMPTY + (i & 1), (i >> 1) - 1)))
+                break;
+            store(smem + Lay::v_off + (i & 1) * Lay::Q, vw);
+            fence_proxy_async_smem();
+            mbar_arrive(&bar[B_V_FULL + (i & 1)]);
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
+        }
+    } else {
+        regs_down<56>();
+        if (warp == 12 && lane == 0) {
+            // ============================================= the products
+            constexpr uint32_t QK = idesc_f16(MB, false), PV = idesc_f16(D, true);
+            const uint32_t sq = smem_addr(smem), sk = smem_addr(smem + Lay::k_off), sv = smem_addr(smem + Lay::v_off);
+            auto qk = [&](int i, bool first, int item) {
+                if (first && !(ok = wait(B_Q_FULL, item)))
+                    return;
+                // S lies under the P of tile i - 2, which that tile's product has read
+                if (!(ok = wait(B_K_FULL + (i & 1), i >> 1) && (i < 2 || wait(B_O_FULL + (i & 1), (i >> 1) - 1))))
+                    return;
+                tc_after();
+#pragma unroll
+                for (int c = 0; c < QP; c++)
+#pragma unroll
+                    for (int k = 0; k < D / 16; k++) {
+                        const uint32_t o = (uint32_t)((k >> 2) * MB * 128 + (k & 3) * 32);
+                        mma_ss(tmem + (uint32_t)(i & 1) * MB, sw128(sq + c * Lay::Q + o, 16),
+                               sw128(sk + (i & 1) * Lay::Q + o, 16), QK, c || k);
+                    }
+                tc_commit(&bar[B_K_EMPTY + (i & 1)]);
+                tc_commit(&bar[B_S_FULL + (i & 1)]);
+            };
+            auto pv = [&](int i) {
+                if (!(ok = wait(B_P_FULL + (i & 1), i >> 1) && wait(B_V_FULL + (i & 1), i >> 1) &&
+                           (i < 2 || wait(B_O_EMPTY + (i & 1), (i >> 1) - 1))))
+                    return;
+                tc_after();
+#pragma unroll
+                for (int c = 0; c < PP; c++)
+#pragma unroll
+                    for (int k = 0; k < MB / 16; k++)
+                        mma_ts(tmem + 2 * MB + (uint32_t)(i & 1) * MB, tmem + (uint32_t)(i & 1) * MB + 64 * c + 8 * k,
+                               sw128(sv + (i & 1) * Lay::Q + k * 2048, MB * 128), PV, c || k);
+                tc_commit(&bar[B_V_EMPTY + (i & 1)]);
+                tc_commit(&bar[B_O_FULL + (i & 1)]);
+            };
+            int item = 0;
+            for (int i = 0; i < mine && ok; i++) {
+                if (!(ok = wait(B_INFO_FULL + i % INFO, i / INFO)))
+                    break;
+                const bool first = info[i % INFO].first;
+                mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
+                if (i && first) // the next rows' Q comes after the last softmax of these
+                    pv(i - 1);
+                if (ok)
+                    qk(i, first, item);
+                item += first;
+                if (ok && i && !first)
+                    pv(i - 1);
+            }
+            if (ok)
+                pv(mine - 1);
+            for (int i = max(0, mine - 2); i < mine && ok; i++) // every arrival lands before the barriers go
+                ok = wait(B_K_EMPTY + (i & 1), i >> 1) && wait(B_V_EMPTY + (i & 1), i >> 1);
+        } else if (warp == 13) {
+            // ============================================= pages and scales, ahead
+            int s = s_seq, r0, n, len;
+            kv8_seq(a.b, s, a.err, r0, n, len);
+            long long ht = head_tiles(len, n, R), off = s_at;
+            int g = (int)(off / ht), mt = 0, nt;
+            off -= g * ht;
+            for (; off >= (nt = token_tiles(len, n, R, mt)); mt++)
+                off -= nt;
+            int tile = (int)off;
+            bool from_start = tile == 0;
+            for (int i = 0; i < mine && ok; i++) {
+                const int pos = tile * MB + (lane & 7) * 16, need = len + min(n, (mt + 1) * R);
+                int row = -1;
+                float ks = 0.0f, vs = 0.0f;
+                if (pos < need) {
+                    const int id = kv8_page(a.b, a.c, s, pos / a.c.page, a.err);
+                    if (id >= 0) {
+                        const size_t at = (size_t)id * a.c.n_kv + g;
+                        row = (int)(at * a.c.page) + pos % a.c.page;
+                        ks = a.c.ks[at];
+                        vs = a.c.vs[at];
+                    }
+                }
+                const float lvs = log2f(vs);
+                const bool hole = __any_sync(0xffffffffu, row < 0);
+                if (i >= INFO && !(ok = wait(B_INFO_EMPTY + i % INFO, i / INFO - 1)))
+                    break;
+                ManyTile &x = info[i % INFO];
+                if (lane < 8) {
+                    x.row[lane] = row;
+                    x.ks[lane] = ks;
+                    x.lvs[lane] = lvs;
+                }
+                if (lane == 0) {
+                    x.first = i == 0 || tile == 0;
+                    x.to_end = tile == nt - 1;
+                    x.last = x.to_end || i == mine - 1;
+                    x.masked = hole || tile * MB + MB > len + mt * R + 1;
+                    x.tile = tile;
+                    x.s = s;
+                    x.g = g;
+                    x.mt = mt;
+                    x.r0 = r0;
+                    x.n = n;
+                    x.len = len;
+                    x.from_start = from_start;
+                    x.pieces = (int)(((lo + i + (nt - 1 - tile) + 1) * active - 1) / total) - slot + 1;
+                }
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&bar[B_INFO_FULL + i % INFO]);
+                if (++tile == nt && i + 1 < mine) { // next rows, KV head, sequence
+                    tile = 0;
+                    from_start = true;
+                    if (++mt == row_tiles(n, R)) {
+                        mt = 0;
+                        if (++g == a.c.n_kv) {
+                            g = 0;
+                            do {
+                                s++;
+                                kv8_seq(a.b, s, a.err, r0, n, len);
+                            } while ((long long)n * rep <= p.many);
+                        }
+                    }
+                    nt = token_tiles(len, n, R, mt);
+                }
+            }
+        }
+    }
+    if (!ok) // let products in flight end before their memory goes
+        for (int i = 0; i < 64; i++)
+            __nanosleep(1000);
+    __syncthreads();
+    if (warp == 12)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+template <class T, int D, int QP, int PP>
+int run(const ManyParams &p, int ctas, cudaStream_t stream)
+{
+    const int rep = p.a.n_heads / p.a.c.n_kv;
+    LLMRS_CUDA_TRY(launch(kv8_many_kernel<T, D, QP, PP>, dim3(ctas), dim3(MANY_THREADS), ManyLay<D, QP>::bytes, stream,
+                          false, p));
+    LLMRS_CUDA_TRY(launch(kv8_join_kernel<T, D, MB>, dim3(2 * ctas), dim3(JT), 0, stream, true, p.a,
+                          (const float *)p.part, (const int4 *)p.head, ctas, MB / rep));
+    return LLMRS_OK;
+}
+
+template <class T, int D, int QP, int PP>
+cudaError_t prepare()
+{
+    return cudaFuncSetAttribute(kv8_many_kernel<T, D, QP, PP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                ManyLay<D, QP>::bytes);
+}
+
+} // namespace
+
+size_t kv8_many_workspace(int head_dim)
+{
+    return (size_t)MANY_CTAS * (sizeof(int4) + 2 * (size_t)MB * (head_dim + 2) * sizeof(float));
+}
+
+int kv8_many_prepare(void)
+{
+    cudaError_t e = prepare<float, 128, 2, 2>();
+    if (e == cudaSuccess)
+        e = prepare<float, 64, 2, 2>();
+    if (e == cudaSuccess)
+        e = prepare<__half, 128, 2, 1>();
+    if (e == cudaSuccess)
+        e = prepare<__half, 64, 2, 1>();
+    if (e == cudaSuccess)
+        e = prepare<__nv_bfloat16, 128, 1, 1>();
+    if (e == cudaSuccess)
+        e = prepare<__nv_bfloat16, 64, 1, 1>();
+    if (e != cudaSuccess)
+        return fail(LLMRS_ECUDA, "kv8 kernel attributes: %s", cudaGetErrorString(e));
+    return LLMRS_OK;
+}
+
+int kv8_many(const Kv8Attn &a, int many, void *ws, int sms, cudaStream_t stream)
+{
+    ManyParams p{};
+    p.a = a;
+    p.head = reinterpret_cast<int4 *>(ws);
+    p.part = reinterpret_cast<float *>(p.head + MANY_CTAS);
+    p.many = many;
+    const int ctas = sms < MANY_CTAS ? sms : MANY_CTAS;
+    if (a.dtype == LLMRS_F32)
+        return a.c.D == 128 ? run<float, 128, 2, 2>(p, ctas, stream) : run<float, 64, 2, 2>(p, ctas, stream);
+    if (a.dtype == LLMRS_F16)
+        return a.c.D == 128 ? run<__half, 128, 2, 1>(p, ctas, stream) : run<__half, 64, 2, 1>(p, ctas, stream);
+    return a.c.D == 128 ? run<__nv_bfloat16, 128, 1, 1>(p, ctas, stream)
+                        : run<__nv_bfloat16, 64, 1, 1>(p, ctas, stream);
+}
+
+} // namespace llmrs
