@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
             begin(x);
         }
         if (ok)
-            ok = mbar_wait(&bar[i % ST], (uint32_t)((i / ST) & 1), a.err);
+            ok = kv8_wait(&bar[i % ST], (uint32_t)((i / ST) & 1), a.err);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok)
             break;

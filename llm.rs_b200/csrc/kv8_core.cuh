@@ -76,6 +76,53 @@ __device__ __forceinline__ void store_row(__nv_bfloat16 *p, const float (&x)[N])
     }
 }
 
+// Wait for a barrier's phase, like mbar_wait, in few instructions: a try may
+// suspend for a microsecond, and a million tries without the phase set the
+// error word.
+__device__ __forceinline__ bool kv8_wait(uint64_t *bar, uint32_t parity, uint32_t *err)
+{
+    for (uint32_t left = 1u << 20; left; left--) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\t"
+                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+                     "selp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done)
+                     : "r"(smem_addr(bar)), "r"(parity), "r"(1000)
+                     : "memory");
+        if (done)
+            return true;
+    }
+    atomicCAS(err, 0u, (uint32_t)DEV_ERR_MBAR_TIMEOUT);
+    return false;
+}
+
+// packed f32 pairs
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 c;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t &>(c))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return c;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 c;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t &>(c))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return c;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t &>(d))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)),
+          "l"(reinterpret_cast<uint64_t &>(c)));
+    return d;
+}
+
 // Join the pieces of each pair that no range had to itself.  The tiles of all
 // pairs are cut into `slots` consecutive ranges; a range that begins a pair and
 // does not end it keeps its piece in its second slot and notes the pair and its

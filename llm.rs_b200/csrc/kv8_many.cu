@@ -10,13 +10,16 @@
 // the maximum and the value scales applied there: long sums do not pass
 // through the tensor core's accumulator.
 //
-// Warpgroups: 0 softmax (thread = row; also rotates, scales and splits Q),
-// 1 output (thread = row, D accumulators), 2 codes to f16 in shared memory
-// (keys K-major, values MN-major, both 128-byte swizzled: the same image),
-// 3: one warp issues the products, one looks up pages and scales ahead.
+// Warpgroups: 0 softmax (thread = row), 1 output (thread = row, D accumulators),
+// 2 codes to f16 in shared memory (keys K-major, values MN-major, both 128-byte
+// swizzled: the same image), 3: one warp issues the products, one looks up pages
+// and scales ahead, 4 rotates, scales and splits the next rows' Q.
 // S and O are double buffered (4 x 128 columns: all of TMEM), P lies over the S
-// it came from, K and V tiles are double buffered, so the product of tile i + 1
-// runs while tile i is in the softmax.
+// it came from, Q is double buffered, K and V too where Q is one piece, so the
+// product of tile i + 1 runs while tile i is in the softmax.  The softmax reads
+// S from TMEM twice, 32 columns at a time in a rolled loop: unrolled over 128
+// registers (with Q's preparation in line) a third of all stalls were
+// instruction fetches.
 //
 // Work: the tiles of all (sequence, KV head, tile of rows) in one row, cut into
 // equal consecutive ranges, one per CTA; pieces of a softmax that a range cuts
@@ -30,7 +33,7 @@ namespace llmrs {
 namespace {
 
 constexpr int MB = 128;          // vectors, and tokens, of a tile
-constexpr int MANY_THREADS = 512;
+constexpr int MANY_THREADS = 640;
 constexpr int INFO = 8;          // tile descriptions in flight
 constexpr int RING = 4;          // softmax -> output hand-overs in flight
 
@@ -55,12 +58,14 @@ struct ManyParams {
 
 template <int D, int QP>
 struct ManyLay {
-    static constexpr int Q = MB * D * 2;   // bytes of one piece of Q; of an f16 K or V tile
-    static constexpr int k_off = QP * Q;
-    static constexpr int v_off = k_off + 2 * Q;
-    static constexpr int info_off = v_off + 2 * Q;
+    static constexpr int KVS = QP == 1 ? 2 : 1; // buffers of K and of V
+    static constexpr int T = MB * D * 2;        // bytes of one piece of Q, of an f16 K or V tile
+    static constexpr int k_off = 2 * QP * T;    // Q: [2 buffers][QP pieces]
+    static constexpr int v_off = k_off + KVS * T;
+    static constexpr int info_off = v_off + KVS * T;
     static constexpr int ring_off = info_off + INFO * (int)sizeof(ManyTile);
-    static constexpr int bar_off = ring_off + RING * 4 * MB * 4;
+    static constexpr int fac_off = ring_off + RING * 4 * MB * 4; // [2][MB] score factors of the rows
+    static constexpr int bar_off = fac_off + 2 * MB * 4;
     static constexpr int bytes = bar_off + 512 + 1024; // + alignment slack
     static_assert(bytes <= 232448 - 256, "shared memory of one CTA");
 };
@@ -77,7 +82,8 @@ enum : int { // barriers
     B_O_FULL = B_P_FULL + 2,
     B_O_EMPTY = B_O_FULL + 2,
     B_Q_FULL = B_O_EMPTY + 2,
-    B_COUNT = B_Q_FULL + 1,
+    B_Q_EMPTY = B_Q_FULL + 2,
+    B_COUNT = B_Q_EMPTY + 2,
 };
 static_assert(B_COUNT * 8 <= 512, "barrier space");
 
@@ -87,7 +93,8 @@ __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_
 
 __device__ __forceinline__ void tc_commit(uint64_t *bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar))
                  : "memory");
 }
 
@@ -106,18 +113,21 @@ __host__ __device__ constexpr uint32_t idesc_f16(int n, bool b_mn)
     return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(MB >> 4) << 24);
 }
 
+// Whole warp, one elected lane issues: operands stay in uniform registers (under
+// a divergent branch every product paid for moving its descriptors there, 200
+// cycles each)
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, bool acc)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+    asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
                  "l"(ad), "l"(bd), "r"(idesc), "r"((int)acc)
                  : "memory");
 }
 
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t at, uint64_t bd, uint32_t idesc, bool acc)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+    asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
                  "r"(at), "l"(bd), "r"(idesc), "r"((int)acc)
                  : "memory");
 }
@@ -147,6 +157,25 @@ __device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t (&r)[32])
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
                  "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::I8(r, 0),
                  I8(r, 8), I8(r, 16), I8(r, 24), "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tm_ld16(uint32_t addr, uint32_t (&r)[16])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+                 "%14, %15}, [%16];"
+                 : R8(r, 0), R8(r, 8)
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tm_wait(uint32_t (&r)[16])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : T8(r, 0), T8(r, 8) : : "memory");
+}
+__device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t (&r)[16])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+                 "%13, %14, %15};" ::I8(r, 0),
+                 I8(r, 8), "r"(addr)
                  : "memory");
 }
 #undef R8
@@ -179,6 +208,36 @@ __device__ __forceinline__ long long head_tiles(int len, int n, int R)
     return t;
 }
 
+// The (sequence, KV head, tile of rows) pairs in their order
+struct Walk {
+    int s, r0, n, len, g, mt, nt; // nt: tiles of tokens
+    __device__ __forceinline__ int start(const ManyParams &p, int s_, long long off, int R) // returns the tile at `off`
+    {
+        s = s_;
+        kv8_seq(p.a.b, s, p.a.err, r0, n, len);
+        const long long ht = head_tiles(len, n, R);
+        g = (int)(off / ht);
+        off -= g * ht;
+        for (mt = 0; off >= (nt = token_tiles(len, n, R, mt)); mt++)
+            off -= nt;
+        return (int)off;
+    }
+    __device__ __forceinline__ void next(const ManyParams &p, int rep, int R)
+    {
+        if (++mt == row_tiles(n, R)) {
+            mt = 0;
+            if (++g == p.a.c.n_kv) {
+                g = 0;
+                do {
+                    s++;
+                    kv8_seq(p.a.b, s, p.a.err, r0, n, len);
+                } while ((long long)n * rep <= p.many);
+            }
+        }
+        nt = token_tiles(len, n, R, mt);
+    }
+};
+
 // codes of 16 dims to f16, 32 bytes
 __device__ __forceinline__ void widen(uint4 w, uint4 &lo, uint4 &hi)
 {
@@ -195,14 +254,15 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
     extern __shared__ __align__(128) uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     ManyTile *info = reinterpret_cast<ManyTile *>(smem + Lay::info_off);
-    float *ring = reinterpret_cast<float *>(smem + Lay::ring_off); // [RING][corr | scale of O | sum | max][MB]
+    float *ring = reinterpret_cast<float *>(smem + Lay::ring_off); // [RING][change of max | scale of O | sum | max][MB]
+    float *facs = reinterpret_cast<float *>(smem + Lay::fac_off);
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + Lay::bar_off);
     __shared__ uint32_t s_tmem;
     __shared__ long long s_sum[MANY_THREADS / 32];
     __shared__ long long s_at;
     __shared__ int s_seq;
     const Kv8Attn &a = p.a;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, wg = warp >> 2;
     const int rep = a.n_heads / a.c.n_kv, R = MB / rep;
     griddep_launch_dependents();
 
@@ -220,8 +280,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
             mbar_init(&bar[B_P_FULL + i], 128);
             mbar_init(&bar[B_O_FULL + i], 1);
             mbar_init(&bar[B_O_EMPTY + i], 128);
+            mbar_init(&bar[B_Q_FULL + i], 128);
+            mbar_init(&bar[B_Q_EMPTY + i], 5); // the products and the softmax warps
         }
-        mbar_init(&bar[B_Q_FULL], 128);
         fence_mbar_init();
         s_seq = 0;
     }
@@ -289,83 +350,37 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
     tc_after();
     const uint32_t tmem = s_tmem;
     const int mine = (int)(hi - lo);
-    auto wait = [&](int b, int use) { return mbar_wait(&bar[b], (uint32_t)(use & 1), a.err); };
+    auto wait = [&](int b, int use) { // whole warp
+        return __all_sync(0xffffffffu, kv8_wait(&bar[b], (uint32_t)(use & 1), a.err));
+    };
     bool ok = true;
 
     if (wg == 0) {
         // ================================================= softmax: thread = row
-        regs_up<168>();
+        regs_up<104>();
         const int r = threadIdx.x;
         const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
         float m = -INFINITY, l = 0.0f, fac = 0.0f;
-        int lim = -1;
+        int lim = -1, item = 0;
         bool busy = false; // some row of this warp is there
         for (int i = 0; i < mine && ok; i++) {
             const ManyTile &x = info[i % INFO];
             if (!(ok = wait(B_INFO_FULL + i % INFO, i / INFO)))
                 break;
             if (x.first) {
-                // rotate, scale and split the row's q; its last use was the products of the
-                // tile before, which this warpgroup has waited for
-                const int row = x.mt * R + r / rep, head = x.g * rep + r % rep;
+                const int row = x.mt * R + r / rep;
                 const bool live = r < R * rep && row < x.n;
-                constexpr int H = D / 2;
-                float q[D];
-                float big = 0.0f;
-                if (live) {
-                    const T *src = reinterpret_cast<const T *>(a.q) + (size_t)(x.r0 + row) * a.ld_q + (size_t)head * D;
-                    const size_t at = (size_t)(x.len + row) * H;
-#pragma unroll
-                    for (int d = 0; d < H; d += 4) {
-                        const float4 u = kv8_load4(src + d), v = kv8_load4(src + H + d);
-                        float4 c = make_float4(1.0f, 1.0f, 1.0f, 1.0f), s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (a.r.cos) {
-                            c = kv8_load4(a.r.cos + at + d);
-                            s = kv8_load4(a.r.sin + at + d);
-                        }
-                        const float uu[4] = {u.x, u.y, u.z, u.w}, vv[4] = {v.x, v.y, v.z, v.w};
-                        const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            q[d + k] = a.r.cos ? __fsub_rn(__fmul_rn(uu[k], cc[k]), __fmul_rn(vv[k], ss[k])) : uu[k];
-                            q[H + d + k] = a.r.cos ? __fadd_rn(__fmul_rn(uu[k], ss[k]), __fmul_rn(vv[k], cc[k])) : vv[k];
-                        }
-                    }
-#pragma unroll
-                    for (int d = 0; d < D; d++)
-                        big = fmaxf(big, fabsf(q[d]));
-                } else {
-#pragma unroll
-                    for (int d = 0; d < D; d++)
-                        q[d] = 0.0f;
-                }
-                int e = (int)((__float_as_uint(big) >> 23) & 255u) - 127;
-                e = max(-126, min(126, e)); // a power of two brings the largest value into [1, 2)
-                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                fac = __uint_as_float((uint32_t)(127 + e) << 23) * a.scale * 1.4426950408889634f;
                 lim = live ? x.len + row : -1;
                 busy = __any_sync(0xffffffffu, live);
                 m = -INFINITY;
                 l = 0.0f;
-#pragma unroll
-                for (int u = 0; u < D / 8; u++) { // 16-byte units of the swizzled K-major image
-                    uint32_t w[4], w2[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const float x0 = q[8 * u + 2 * k] * down, x1 = q[8 * u + 2 * k + 1] * down;
-                        w[k] = pack16(x0, x1);
-                        if constexpr (QP == 2) {
-                            const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
-                            w2[k] = pack16(x0 - h.x, x1 - h.y);
-                        }
-                    }
-                    const int o = (u / 8) * (MB * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4);
-                    *reinterpret_cast<uint4 *>(smem + o) = make_uint4(w[0], w[1], w[2], w[3]);
-                    if constexpr (QP == 2)
-                        *reinterpret_cast<uint4 *>(smem + Lay::Q + o) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
-                }
-                fence_proxy_async_smem();
-                mbar_arrive(&bar[B_Q_FULL]);
+                if (!(ok = wait(B_Q_FULL + (item & 1), item >> 1)))
+                    break;
+                fac = facs[(item & 1) * MB + r];
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&bar[B_Q_EMPTY + (item & 1)]);
+                item++;
             }
             if (!(ok = wait(B_S_FULL + (i & 1), i >> 1)))
                 break;
@@ -373,41 +388,51 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
             const uint32_t sp = lanes + (uint32_t)(i & 1) * MB;
             float corr = 1.0f, oscale = 0.0f;
             if (busy) {
-                uint32_t s[4][32];
+                const bool masked = x.masked;
+                if (masked) { // S becomes the scores themselves, the unseen ones at -inf
+#pragma unroll 1
+                    for (int k = 0; k < 4; k++) {
+                        uint32_t s[32];
+                        tm_ld32(sp + 32 * k, s);
+                        tm_wait(s);
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    tm_ld32(sp + 32 * k, s[k]);
+                        for (int h = 0; h < 2; h++) {
+                            const int last = x.row[2 * k + h] >= 0 ? lim - x.tile * MB - 32 * k - 16 * h : -1;
+                            const float kf = fac * x.ks[2 * k + h];
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    tm_wait(s[k]);
-                float kf[8];
-                float top = -INFINITY, ref2 = -INFINITY;
-#pragma unroll
-                for (int g = 0; g < 8; g++)
-                    kf[g] = fac * x.ks[g];
-                if (x.masked) { // scores themselves, the unseen ones at -inf
-#pragma unroll
-                    for (int g = 0; g < 8; g++) {
-                        const int last = x.row[g] >= 0 ? lim - x.tile * MB - 16 * g : -1;
-#pragma unroll
-                        for (int j = 0; j < 16; j++) {
-                            uint32_t &w = s[g / 2][(g & 1) * 16 + j];
-                            w = __float_as_uint(j <= last ? __uint_as_float(w) * kf[g] : -INFINITY);
+                            for (int j = 0; j < 16; j++)
+                                s[16 * h + j] =
+                                    __float_as_uint(j <= last ? __uint_as_float(s[16 * h + j]) * kf : -INFINITY);
                         }
-                        kf[g] = 1.0f;
+                        tm_st32(sp + 32 * k, s);
                     }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
+                // 32 scores of the row as two groups of 16, and what they are multiplied by
+                auto scores = [&](int k, uint32_t(&s)[32], float(&kf)[2]) {
+                    tm_ld32(sp + 32 * k, s);
+                    kf[0] = masked ? 1.0f : fac * x.ks[2 * k];
+                    kf[1] = masked ? 1.0f : fac * x.ks[2 * k + 1];
+                    tm_wait(s);
+                };
+                float top = -INFINITY, ref2 = -INFINITY;
+#pragma unroll 1
+                for (int k = 0; k < 4; k++) {
+                    uint32_t s[32];
+                    float kf[2];
+                    scores(k, s, kf);
 #pragma unroll
-                for (int g = 0; g < 8; g++) {
-                    float t0 = -INFINITY, t1 = -INFINITY;
+                    for (int h = 0; h < 2; h++) {
+                        float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        t0 = fmaxf(t0, __uint_as_float(s[g / 2][(g & 1) * 16 + j]));
-                        t1 = fmaxf(t1, __uint_as_float(s[g / 2][(g & 1) * 16 + j + 1]));
+                        for (int j = 0; j < 16; j += 4) {
+                            t0 = fmaxf(fmaxf(t0, __uint_as_float(s[16 * h + j])), __uint_as_float(s[16 * h + j + 1]));
+                            t1 = fmaxf(fmaxf(t1, __uint_as_float(s[16 * h + j + 2])), __uint_as_float(s[16 * h + j + 3]));
+                        }
+                        t0 = fmaxf(t0, t1) * kf[h]; // kf >= 0
+                        top = fmaxf(top, t0);
+                        ref2 = fmaxf(ref2, t0 + x.lvs[2 * k + h]);
                     }
-                    t0 = fmaxf(t0, t1) * kf[g]; // kf >= 0
-                    top = fmaxf(top, t0);
-                    ref2 = fmaxf(ref2, t0 + x.lvs[g]);
                 }
                 const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.0f : mn;
                 corr = ex2(m - ref);
@@ -418,35 +443,38 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                 ref2 = none ? 0.0f : ref2 - P_SCALE_LOG2;
                 oscale = none ? 0.0f : ex2(ref2 - ref);
                 float sum = 0.0f;
+#pragma unroll 1
+                for (int k = 0; k < 4; k++) {
+                    uint32_t s[32], ph[16], pl[16];
+                    float kf[2];
+                    scores(k, s, kf);
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t ph[32], pl[32];
-#pragma unroll
-                    for (int gg = 0; gg < 4; gg++) {
-                        const int g = 4 * h + gg;
+                    for (int h = 0; h < 2; h++) {
+                        const float lvs = x.lvs[2 * k + h];
                         // a scale of zero: f16 holds the probabilities as zero, the sum keeps them
-                        const bool zero = x.lvs[g] == -INFINITY;
-                        const float add = zero ? -60.0f - ref : x.lvs[g] - ref2;
-                        const float back = zero ? 0x1p60f : ex2(fminf(ref2 - x.lvs[g] - ref, 120.0f));
-                        float g0 = 0.0f, g1 = 0.0f;
+                        const bool zero = lvs == -INFINITY;
+                        const float add = zero ? -60.0f - ref : lvs - ref2;
+                        const float back = zero ? 0x1p60f : ex2(fminf(ref2 - lvs - ref, 120.0f));
+                        float2 g01 = make_float2(0.0f, 0.0f);
 #pragma unroll
                         for (int j = 0; j < 16; j += 2) {
-                            const float e0 = ex2(fmaf(__uint_as_float(s[g / 2][(g & 1) * 16 + j]), kf[g], add));
-                            const float e1 = ex2(fmaf(__uint_as_float(s[g / 2][(g & 1) * 16 + j + 1]), kf[g], add));
-                            g0 += e0;
-                            g1 += e1;
+                            const float2 y = fma2(make_float2(__uint_as_float(s[16 * h + j]), __uint_as_float(s[16 * h + j + 1])),
+                                                  make_float2(kf[h], kf[h]), make_float2(add, add));
+                            const float e0 = ex2(y.x), e1 = ex2(y.y);
+                            g01 = add2(g01, make_float2(e0, e1));
                             const uint32_t w = pack16(e0, e1);
-                            ph[gg * 8 + j / 2] = w;
+                            ph[8 * h + j / 2] = w;
                             if constexpr (PP == 2) {
                                 const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-                                pl[gg * 8 + j / 2] = pack16(e0 - f.x, e1 - f.y);
+                                pl[8 * h + j / 2] = pack16(e0 - f.x, e1 - f.y);
                             }
                         }
-                        sum += (g0 + g1) * back;
+                        sum += (g01.x + g01.y) * back;
                     }
-                    tm_st32(sp + 32 * h, ph);
+                    // over the 32 columns just read: 16 of the first piece, 16 of the second
+                    tm_st16(sp + 32 * k, ph);
                     if constexpr (PP == 2)
-                        tm_st32(sp + 64 + 32 * h, pl);
+                        tm_st16(sp + 32 * k + 16, pl);
                 }
                 l = l * corr + sum;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -466,10 +494,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
         }
     } else if (wg == 1) {
         // ================================================= output: thread = row
-        regs_up<176>();
+        regs_up<160>();
         const int r = threadIdx.x - 128;
         const uint32_t lanes = tmem + 2 * MB + ((uint32_t)((warp & 3) * 32) << 16);
-        float acc[D];
+        float2 acc[D / 2];
         for (int i = 0; i < mine && ok; i++) {
             const ManyTile &x = info[i % INFO];
             if (!(ok = wait(B_INFO_FULL + i % INFO, i / INFO) && wait(B_O_FULL + (i & 1), i >> 1)))
@@ -484,50 +512,50 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
             }
             if (x.first) {
 #pragma unroll
-                for (int d = 0; d < D; d++)
-                    acc[d] = 0.0f;
+                for (int d = 0; d < D / 2; d++)
+                    acc[d] = make_float2(0.0f, 0.0f);
             }
+            const float2 corr2 = make_float2(corr, corr), scale2 = make_float2(oscale, oscale);
 #pragma unroll
-            for (int k = 0; k < D / 32; k++) {
-                uint32_t o[32];
-                tm_ld32(lanes + (uint32_t)(i & 1) * MB + 32 * k, o);
+            for (int k = 0; k < D / 16; k++) {
+                uint32_t o[16];
+                tm_ld16(lanes + (uint32_t)(i & 1) * MB + 16 * k, o);
                 tm_wait(o);
-                if (k == D / 32 - 1) {
+                if (k == D / 16 - 1) {
                     tc_before();
                     mbar_arrive(&bar[B_O_EMPTY + (i & 1)]);
                 }
 #pragma unroll
-                for (int d = 0; d < 32; d++)
-                    acc[32 * k + d] = acc[32 * k + d] * corr + __uint_as_float(o[d]) * oscale;
+                for (int d = 0; d < 8; d++)
+                    acc[8 * k + d] = fma2(acc[8 * k + d], corr2,
+                                          mul2(make_float2(__uint_as_float(o[2 * d]), __uint_as_float(o[2 * d + 1])), scale2));
             }
             if (x.last) {
                 const int row = x.mt * R + r / rep, head = x.g * rep + r % rep;
                 const bool done = x.from_start && x.to_end, live = r < R * rep && row < x.n;
                 if (!done && x.from_start && r == 0)
                     p.head[slot] = make_int4(x.s, x.mt, x.g, x.pieces);
-                if (live && done) {
-                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                if (live) {
+                    const float inv = !done ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
                     T *out = reinterpret_cast<T *>(a.out) + (size_t)(x.r0 + row) * a.ld_out + (size_t)head * D;
-#pragma unroll
-                    for (int d = 0; d < D; d += 16) {
-                        float o[16];
-#pragma unroll
-                        for (int j = 0; j < 16; j++)
-                            o[j] = acc[d + j] * inv;
-                        store_row<16>(out + d, o);
-                    }
-                } else if (live) {
                     float *part = p.part + ((size_t)slot * 2 + (x.from_start ? 1 : 0)) * MB * (D + 2);
 #pragma unroll
                     for (int d = 0; d < D; d += 16) {
                         float o[16];
 #pragma unroll
-                        for (int j = 0; j < 16; j++)
-                            o[j] = acc[d + j];
-                        store_row<16>(part + (size_t)r * D + d, o);
+                        for (int j = 0; j < 8; j++) {
+                            o[2 * j] = acc[d / 2 + j].x * inv;
+                            o[2 * j + 1] = acc[d / 2 + j].y * inv;
+                        }
+                        if (done)
+                            store_row<16>(out + d, o);
+                        else
+                            store_row<16>(part + (size_t)r * D + d, o);
                     }
-                    part[(size_t)MB * D + r] = m;
-                    part[(size_t)MB * (D + 1) + r] = l;
+                    if (!done) {
+                        part[(size_t)MB * D + r] = m;
+                        part[(size_t)MB * (D + 1) + r] = l;
+                    }
                 }
             }
             __syncwarp();
@@ -536,149 +564,142 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
         }
     } else if (wg == 2) {
         // ================================================= codes to f16
-        regs_down<112>();
-        constexpr int U = D / 16;            // 16-code units of a token
-        constexpr int N = MB * U / 128;      // units a thread widens per tile and operand
-        const int t = threadIdx.x - 256, j = t & 7;
-        // D = 128: eight lanes take half the units of two tokens, crosswise, so that
-        // the eight 16-byte stores of a pass fall into eight bank groups
-        auto place = [&](int n, int &tok, int &unit) {
-            if constexpr (D == 128) {
-                const int half = n & 1;
-                tok = 2 * ((t >> 3) + 16 * (n >> 1)) + (j >> 2);
-                unit = 4 * (half ^ (j >> 2)) + (j & 3);
-            } else {
-                tok = 2 * ((t >> 3) + 16 * n) + (j >> 2);
-                unit = j & 3;
-            }
-        };
-        auto load = [&](const int8_t *codes, const ManyTile &x, uint4 (&w)[N]) {
+        // Eight lanes take eight 16-code units: for D = 128 half the units of two tokens,
+        // crosswise, for D = 64 two tokens, so that the eight 16-byte stores of a pass fall
+        // into eight bank groups.  Unit n of a thread: token tok + 32 * (n / PER), column
+        // unit0 or unit1.
+        constexpr int PER = D / 64;      // units of a token pair row that a thread takes
+        constexpr int N = 4 * PER;       // units a thread widens per half tile (K or V)
+        const int t = threadIdx.x - 256, j = t & 7, odd = j >> 2;
+        const int tok = 2 * (t >> 3) + odd;
+        const int unit0 = D == 128 ? 4 * odd + (j & 3) : j & 3, unit1 = unit0 ^ 4;
+        const int sw = tok & 7;          // the same for every token of the thread
+        auto place = [&](int unit) { return (unit >> 2) * (MB * 128) + tok * 128 + (((2 * (unit & 3)) ^ sw) << 4); };
+        const int at0 = place(unit0), at1 = place(unit1);
+        uint4 cur[N], nxt[N];
+        auto load = [&](int h) { // half tile h: keys of tile h / 2, then its values
+            const ManyTile &x = info[(h >> 1) % INFO];
+            const int8_t *codes = (h & 1 ? a.c.vq : a.c.kq) + (tok & 15) * D;
 #pragma unroll
-            for (int n = 0; n < N; n++) {
-                int tok, unit;
-                place(n, tok, unit);
-                const int row = x.row[tok >> 4];
-                w[n] = make_uint4(0, 0, 0, 0);
-                if (row >= 0)
-                    w[n] = __ldg(reinterpret_cast<const uint4 *>(codes + ((size_t)row + (tok & 15)) * D + unit * 16));
-            }
-        };
-        auto store = [&](uint8_t *dst, const uint4 (&w)[N]) {
+            for (int n = 0; n < 4; n++) {
+                const int row = x.row[(tok >> 4) + 2 * n];
+                const int8_t *src = codes + (size_t)row * D;
 #pragma unroll
-            for (int n = 0; n < N; n++) {
-                int tok, unit;
-                place(n, tok, unit);
-                uint4 a0, a1;
-                widen(w[n], a0, a1);
-                uint8_t *b = dst + (unit >> 2) * (MB * 128) + tok * 128;
-                const int u = 2 * (unit & 3), sw = tok & 7;
-                *reinterpret_cast<uint4 *>(b + ((u ^ sw) << 4)) = a0;
-                *reinterpret_cast<uint4 *>(b + (((u + 1) ^ sw) << 4)) = a1;
+                for (int u = 0; u < PER; u++)
+                    nxt[n * PER + u] = row >= 0 ? __ldg(reinterpret_cast<const uint4 *>(src + (u ? unit1 : unit0) * 16))
+                                                : make_uint4(0, 0, 0, 0);
             }
         };
-        uint4 kw[N], vw[N];
         ok = wait(B_INFO_FULL, 0);
         if (ok)
-            load(a.c.kq, info[0], kw);
-        for (int i = 0; i < mine && ok; i++) {
-            load(a.c.vq, info[i % INFO], vw);
-            if (!(ok = i < 2 || wait(B_K_EMPTY + (i & 1), (i >> 1) - 1)))
-                break;
-            store(smem + Lay::k_off + (i & 1) * Lay::Q, kw);
-            fence_proxy_async_smem();
-            mbar_arrive(&bar[B_K_FULL + (i & 1)]);
-            if (i + 1 < mine) {
-                if (!(ok = wait(B_INFO_FULL + (i + 1) % INFO, (i + 1) / INFO)))
+            load(0);
+#pragma unroll 1
+        for (int h = 0; h < 2 * mine && ok; h++) {
+            const int i = h >> 1, b = i % Lay::KVS, use = i / Lay::KVS, v = h & 1;
+#pragma unroll
+            for (int n = 0; n < N; n++)
+                cur[n] = nxt[n];
+            if (h + 1 < 2 * mine) {
+                if (v && !(ok = wait(B_INFO_FULL + (i + 1) % INFO, (i + 1) / INFO)))
                     break;
-                load(a.c.kq, info[(i + 1) % INFO], kw);
+                load(h + 1);
             }
-            if (!(ok = i < 2 || wait(B_V_EMPTY + (i & 1), (i >> 1) - 1)))
+            if (!(ok = use == 0 || wait((v ? B_V_EMPTY : B_K_EMPTY) + b, use - 1)))
                 break;
-            store(smem + Lay::v_off + (i & 1) * Lay::Q, vw);
+            uint8_t *dst = smem + (v ? Lay::v_off : Lay::k_off) + b * Lay::T;
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                uint4 a0, a1;
+                widen(cur[n], a0, a1);
+                uint8_t *o = dst + (n % PER ? at1 : at0) + (n / PER) * 32 * 128;
+                *reinterpret_cast<uint4 *>(o) = a0;
+                *reinterpret_cast<uint4 *>(dst + ((n % PER ? at1 : at0) ^ 16) + (n / PER) * 32 * 128) = a1;
+            }
             fence_proxy_async_smem();
-            mbar_arrive(&bar[B_V_FULL + (i & 1)]);
-            __syncwarp();
-            if (lane == 0)
-                mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
+            mbar_arrive(&bar[(v ? B_V_FULL : B_K_FULL) + b]);
+            if (v) {
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
+            }
         }
-    } else {
-        regs_down<56>();
-        if (warp == 12 && lane == 0) {
+    } else if (wg == 3) {
+        regs_down<48>();
+        if (warp == 12) {
             // ============================================= the products
             constexpr uint32_t QK = idesc_f16(MB, false), PV = idesc_f16(D, true);
             const uint32_t sq = smem_addr(smem), sk = smem_addr(smem + Lay::k_off), sv = smem_addr(smem + Lay::v_off);
-            auto qk = [&](int i, bool first, int item) {
-                if (first && !(ok = wait(B_Q_FULL, item)))
-                    return;
+            int item = -1;
+            auto qk = [&](int i, bool first, bool last) {
+                item += first;
+                const int b = i % Lay::KVS;
                 // S lies under the P of tile i - 2, which that tile's product has read
-                if (!(ok = wait(B_K_FULL + (i & 1), i >> 1) && (i < 2 || wait(B_O_FULL + (i & 1), (i >> 1) - 1))))
+                if (!(ok = (!first || wait(B_Q_FULL + (item & 1), item >> 1)) && wait(B_K_FULL + b, i / Lay::KVS) &&
+                           (i < 2 || wait(B_O_FULL + (i & 1), (i >> 1) - 1))))
                     return;
                 tc_after();
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < QP; c++)
-#pragma unroll
+#pragma unroll 4
                     for (int k = 0; k < D / 16; k++) {
                         const uint32_t o = (uint32_t)((k >> 2) * MB * 128 + (k & 3) * 32);
-                        mma_ss(tmem + (uint32_t)(i & 1) * MB, sw128(sq + c * Lay::Q + o, 16),
-                               sw128(sk + (i & 1) * Lay::Q + o, 16), QK, c || k);
+                        mma_ss(tmem + (uint32_t)(i & 1) * MB, sw128(sq + ((item & 1) * QP + c) * Lay::T + o, 16),
+                               sw128(sk + b * Lay::T + o, 16), QK, c || k);
                     }
-                tc_commit(&bar[B_K_EMPTY + (i & 1)]);
+                tc_commit(&bar[B_K_EMPTY + b]);
+                if (last)
+                    tc_commit(&bar[B_Q_EMPTY + (item & 1)]);
                 tc_commit(&bar[B_S_FULL + (i & 1)]);
             };
             auto pv = [&](int i) {
-                if (!(ok = wait(B_P_FULL + (i & 1), i >> 1) && wait(B_V_FULL + (i & 1), i >> 1) &&
+                const int b = i % Lay::KVS;
+                if (!(ok = wait(B_P_FULL + (i & 1), i >> 1) && wait(B_V_FULL + b, i / Lay::KVS) &&
                            (i < 2 || wait(B_O_EMPTY + (i & 1), (i >> 1) - 1))))
                     return;
                 tc_after();
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < PP; c++)
-#pragma unroll
+#pragma unroll 4
                     for (int k = 0; k < MB / 16; k++)
-                        mma_ts(tmem + 2 * MB + (uint32_t)(i & 1) * MB, tmem + (uint32_t)(i & 1) * MB + 64 * c + 8 * k,
-                               sw128(sv + (i & 1) * Lay::Q + k * 2048, MB * 128), PV, c || k);
-                tc_commit(&bar[B_V_EMPTY + (i & 1)]);
+                        mma_ts(tmem + 2 * MB + (uint32_t)(i & 1) * MB,
+                               tmem + (uint32_t)(i & 1) * MB + 32 * (k >> 1) + 16 * c + 8 * (k & 1),
+                               sw128(sv + b * Lay::T + k * 2048, MB * 128), PV, c || k);
+                tc_commit(&bar[B_V_EMPTY + b]);
                 tc_commit(&bar[B_O_FULL + (i & 1)]);
             };
-            int item = 0;
-            for (int i = 0; i < mine && ok; i++) {
-                if (!(ok = wait(B_INFO_FULL + i % INFO, i / INFO)))
-                    break;
-                const bool first = info[i % INFO].first;
-                mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
-                if (i && first) // the next rows' Q comes after the last softmax of these
-                    pv(i - 1);
-                if (ok)
-                    qk(i, first, item);
-                item += first;
-                if (ok && i && !first)
+#pragma unroll 1
+            for (int i = 0; i <= mine && ok; i++) { // the scores of tile i, then the output of tile i - 1
+                if (i < mine) {
+                    if (!(ok = wait(B_INFO_FULL + i % INFO, i / INFO)))
+                        break;
+                    const bool first = __shfl_sync(0xffffffffu, info[i % INFO].first, 0);
+                    const bool last = __shfl_sync(0xffffffffu, info[i % INFO].last, 0);
+                    if (lane == 0)
+                        mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
+                    qk(i, first, last);
+                }
+                if (ok && i)
                     pv(i - 1);
             }
-            if (ok)
-                pv(mine - 1);
-            for (int i = max(0, mine - 2); i < mine && ok; i++) // every arrival lands before the barriers go
-                ok = wait(B_K_EMPTY + (i & 1), i >> 1) && wait(B_V_EMPTY + (i & 1), i >> 1);
+            // every arrival lands before the barriers go
+            const int b = (mine - 1) % Lay::KVS, use = (mine - 1) / Lay::KVS;
+            ok = ok && wait(B_K_EMPTY + b, use) && wait(B_V_EMPTY + b, use) && wait(B_Q_EMPTY + (item & 1), item >> 1);
         } else if (warp == 13) {
             // ============================================= pages and scales, ahead
-            int s = s_seq, r0, n, len;
-            kv8_seq(a.b, s, a.err, r0, n, len);
-            long long ht = head_tiles(len, n, R), off = s_at;
-            int g = (int)(off / ht), mt = 0, nt;
-            off -= g * ht;
-            for (; off >= (nt = token_tiles(len, n, R, mt)); mt++)
-                off -= nt;
-            int tile = (int)off;
+            Walk at;
+            int tile = at.start(p, s_seq, s_at, R);
             bool from_start = tile == 0;
             for (int i = 0; i < mine && ok; i++) {
-                const int pos = tile * MB + (lane & 7) * 16, need = len + min(n, (mt + 1) * R);
+                const int pos = tile * MB + (lane & 7) * 16, need = at.len + min(at.n, (at.mt + 1) * R);
                 int row = -1;
                 float ks = 0.0f, vs = 0.0f;
                 if (pos < need) {
-                    const int id = kv8_page(a.b, a.c, s, pos / a.c.page, a.err);
+                    const int id = kv8_page(a.b, a.c, at.s, pos / a.c.page, a.err);
                     if (id >= 0) {
-                        const size_t at = (size_t)id * a.c.n_kv + g;
-                        row = (int)(at * a.c.page) + pos % a.c.page;
-                        ks = a.c.ks[at];
-                        vs = a.c.vs[at];
+                        const size_t o = (size_t)id * a.c.n_kv + at.g;
+                        row = (int)(o * a.c.page) + pos % a.c.page;
+                        ks = a.c.ks[o];
+                        vs = a.c.vs[o];
                     }
                 }
                 const float lvs = log2f(vs);
@@ -693,38 +714,117 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                 }
                 if (lane == 0) {
                     x.first = i == 0 || tile == 0;
-                    x.to_end = tile == nt - 1;
+                    x.to_end = tile == at.nt - 1;
                     x.last = x.to_end || i == mine - 1;
-                    x.masked = hole || tile * MB + MB > len + mt * R + 1;
+                    x.masked = hole || tile * MB + MB > at.len + at.mt * R + 1;
                     x.tile = tile;
-                    x.s = s;
-                    x.g = g;
-                    x.mt = mt;
-                    x.r0 = r0;
-                    x.n = n;
-                    x.len = len;
+                    x.s = at.s;
+                    x.g = at.g;
+                    x.mt = at.mt;
+                    x.r0 = at.r0;
+                    x.n = at.n;
+                    x.len = at.len;
                     x.from_start = from_start;
-                    x.pieces = (int)(((lo + i + (nt - 1 - tile) + 1) * active - 1) / total) - slot + 1;
+                    x.pieces = (int)(((lo + i + (at.nt - 1 - tile) + 1) * active - 1) / total) - slot + 1;
                 }
                 __syncwarp();
                 if (lane == 0)
                     mbar_arrive(&bar[B_INFO_FULL + i % INFO]);
-                if (++tile == nt && i + 1 < mine) { // next rows, KV head, sequence
+                if (++tile == at.nt && i + 1 < mine) {
                     tile = 0;
                     from_start = true;
-                    if (++mt == row_tiles(n, R)) {
-                        mt = 0;
-                        if (++g == a.c.n_kv) {
-                            g = 0;
-                            do {
-                                s++;
-                                kv8_seq(a.b, s, a.err, r0, n, len);
-                            } while ((long long)n * rep <= p.many);
-                        }
-                    }
-                    nt = token_tiles(len, n, R, mt);
+                    at.next(p, rep, R);
                 }
             }
+        }
+    } else {
+        // ================================================= Q of the next rows
+        regs_down<72>();
+        constexpr int L = D / 8; // lanes of a vector: four dims of each half
+        constexpr int H = D / 2;
+        const int t = threadIdx.x - 512, j = t % L;
+        Walk at;
+        int begun = at.start(p, s_seq, s_at, R), left = mine; // tiles of the pair in front of this range; tiles left
+        for (int item = 0; left > 0 && ok; item++) {
+            if (!(ok = item < 2 || wait(B_Q_EMPTY + (item & 1), (item >> 1) - 1)))
+                break;
+            uint8_t *dst = smem + (item & 1) * QP * Lay::T;
+            // The rows come in with asynchronous copies, all at once, each into the 128-byte
+            // lines that its own f16 pieces will take: f32 rows four, 16-bit rows two
+            constexpr int UNITS = D * (int)sizeof(T) / 16;
+            auto line = [&](int r, int unit) { // unit of row r: line unit / 8 of the row's lines, natural order
+                return dst + (unit >> 3) * (MB * 128) + r * 128 + (unit & 7) * 16;
+            };
+#pragma unroll 1
+            for (int r = t / L; r < MB; r += 128 / L) {
+                const int row = at.mt * R + r / rep, head = at.g * rep + r % rep;
+                if (r < R * rep && row < at.n) {
+                    const uint8_t *src = reinterpret_cast<const uint8_t *>(reinterpret_cast<const T *>(a.q) +
+                                                                           (size_t)(at.r0 + row) * a.ld_q + (size_t)head * D);
+#pragma unroll
+                    for (int u = j; u < UNITS; u += L)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(line(r, u))),
+                                     "l"(src + u * 16)
+                                     : "memory");
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
+#pragma unroll 1
+            for (int r = t / L; r < MB; r += 128 / L) {
+                const int row = at.mt * R + r / rep;
+                const bool live = r < R * rep && row < at.n;
+                float4 u = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = u;
+                if (live) {
+                    constexpr int B = (int)sizeof(T);
+                    u = kv8_load4(reinterpret_cast<const T *>(line(r, 4 * j * B / 16) + 4 * j * B % 16));
+                    v = kv8_load4(reinterpret_cast<const T *>(line(r, (H + 4 * j) * B / 16) + (H + 4 * j) * B % 16));
+                    if (a.r.cos) {
+                        const size_t o = (size_t)(at.len + row) * H + 4 * j;
+                        const float4 c = kv8_load4(a.r.cos + o), s = kv8_load4(a.r.sin + o), w = u;
+                        u.x = __fsub_rn(__fmul_rn(w.x, c.x), __fmul_rn(v.x, s.x));
+                        u.y = __fsub_rn(__fmul_rn(w.y, c.y), __fmul_rn(v.y, s.y));
+                        u.z = __fsub_rn(__fmul_rn(w.z, c.z), __fmul_rn(v.z, s.z));
+                        u.w = __fsub_rn(__fmul_rn(w.w, c.w), __fmul_rn(v.w, s.w));
+                        v.x = __fadd_rn(__fmul_rn(w.x, s.x), __fmul_rn(v.x, c.x));
+                        v.y = __fadd_rn(__fmul_rn(w.y, s.y), __fmul_rn(v.y, c.y));
+                        v.z = __fadd_rn(__fmul_rn(w.z, s.z), __fmul_rn(v.z, c.z));
+                        v.w = __fadd_rn(__fmul_rn(w.w, s.w), __fmul_rn(v.w, c.w));
+                    }
+                }
+                float big = fmaxf(fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(u.z), fabsf(u.w))),
+                                  fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+#pragma unroll
+                for (int o = 1; o < L; o <<= 1) // and every lane of the row has read its part
+                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                int e = (int)((__float_as_uint(big) >> 23) & 255u) - 127;
+                e = max(-126, min(126, e)); // a power of two brings the largest value into [1, 2)
+                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+                if (j == 0)
+                    facs[(item & 1) * MB + r] = __uint_as_float((uint32_t)(127 + e) << 23) * a.scale * 1.4426950408889634f;
+                __syncwarp();
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float x[4] = {(h ? v.x : u.x) * down, (h ? v.y : u.y) * down, (h ? v.z : u.z) * down,
+                                        (h ? v.w : u.w) * down};
+                    const int unit = (h * H + 4 * j) / 8;
+                    uint8_t *b = dst + (unit / 8) * (MB * 128) + r * 128 + (((unit & 7) ^ (r & 7)) << 4) + (j & 1) * 8;
+                    const uint32_t w0 = pack16(x[0], x[1]), w1 = pack16(x[2], x[3]);
+                    *reinterpret_cast<uint2 *>(b) = make_uint2(w0, w1);
+                    if constexpr (QP == 2) {
+                        const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&w0));
+                        const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&w1));
+                        *reinterpret_cast<uint2 *>(b + Lay::T) =
+                            make_uint2(pack16(x[0] - f0.x, x[1] - f0.y), pack16(x[2] - f1.x, x[3] - f1.y));
+                    }
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&bar[B_Q_FULL + (item & 1)]);
+            left -= at.nt - begun;
+            begun = 0;
+            if (left > 0)
+                at.next(p, rep, R);
         }
     }
     if (!ok) // let products in flight end before their memory goes
