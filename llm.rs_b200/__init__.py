@@ -301,12 +301,22 @@ class QuantWeight:
 
 
 # element types of device arrays: DeviceTensor's numpy dtypes (bfloat16 as its
-# uint16 bits), and torch's by name
-_DTYPES = {np.dtype(np.float32): F32, np.dtype(np.float16): F16, np.dtype(np.uint16): BF16,
-           "torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
-_INT32 = (np.dtype(np.int32), "torch.int32")
-_INT8 = (np.dtype(np.int8), "torch.int8")
-_F32 = (np.dtype(np.float32), "torch.float32")
+# uint16 bits); torch's are added when the first tensor of torch's comes in
+_DTYPES = {np.dtype(np.float32): F32, np.dtype(np.float16): F16, np.dtype(np.uint16): BF16}
+_INT32 = {np.dtype(np.int32): 0}
+_INT8 = {np.dtype(np.int8): 0}
+_F32 = {np.dtype(np.float32): 0}
+
+
+def _learn_torch(dtype, kinds, what):
+    """The code of a dtype that `kinds` does not have yet; TypeError when it is none of them."""
+    if str(dtype).startswith("torch.") and dtype not in _DTYPES:
+        import torch
+        _DTYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+        _INT32[torch.int32] = _INT8[torch.int8] = _F32[torch.float32] = 0
+    if dtype not in kinds:
+        raise TypeError("%s: dtype %s" % (what, dtype))
+    return kinds[dtype]
 
 
 def _address(x):
@@ -314,38 +324,37 @@ def _address(x):
     return x.ptr.value if isinstance(x, DeviceTensor) else x.data_ptr()
 
 
-def _type(x):
-    return x.dtype if isinstance(x, DeviceTensor) else str(x.dtype)
-
-
-def _array(x, types, what):
-    """Address of a contiguous array of one of `types`."""
-    if _type(x) not in types:
-        raise TypeError("%s: dtype %s" % (what, x.dtype))
-    if not isinstance(x, DeviceTensor) and not x.is_contiguous():
+def _array(x, kinds, what):
+    """Address of a contiguous array of one of the element types `kinds`."""
+    if x.dtype not in kinds:
+        _learn_torch(x.dtype, kinds, what)
+    if isinstance(x, DeviceTensor):
+        return x.ptr.value
+    if not x.is_contiguous():
         raise ValueError("%s must be contiguous" % what)
-    return _address(x)
+    return x.data_ptr()
 
 
 def _rows(x, width, what):
     """(address, dtype code, rows, row stride) of rows of `width` elements: [n, width]
     or [n, heads, D], the elements of a row next to each other."""
-    t = _type(x)
-    if t not in _DTYPES:
-        raise TypeError("%s: dtype %s" % (what, x.dtype))
-    n, size = x.shape[0], 1
-    for s in x.shape[1:]:
-        size *= s
+    kind = _DTYPES.get(x.dtype)
+    if kind is None:
+        kind = _learn_torch(x.dtype, _DTYPES, what)
+    shape = x.shape
+    n, size = shape[0], shape[1] if len(shape) == 2 else int(np.prod(shape[1:]))
     if size != width:
         raise ValueError("%s: rows of %d elements, not %d" % (what, size, width))
     if isinstance(x, DeviceTensor):
-        return x.ptr.value, _DTYPES[t], n, width
+        return x.ptr.value, kind, n, width
     strides, inner = x.stride(), 1
-    for s, st in zip(reversed(x.shape[1:]), reversed(strides[1:])):
+    if len(shape) == 2 and strides[1] == 1:
+        return x.data_ptr(), kind, n, strides[0] if n > 1 else width
+    for s, st in zip(reversed(shape[1:]), reversed(strides[1:])):
         if s != 1 and st != inner:
             raise ValueError("%s: the elements of a row must lie next to each other" % what)
         inner *= s
-    return x.data_ptr(), _DTYPES[t], n, strides[0] if n > 1 else max(strides[0], width)
+    return x.data_ptr(), kind, n, strides[0] if n > 1 else width
 
 
 class Kv8Cache:
@@ -525,11 +534,11 @@ class CudaBackend:
         """The values of `pages` (int32 [n]) into k_out, v_out [n, n_kv_heads, page_size, head_dim]."""
         n = pages.shape[0]
         shape = (n,) + cache.shape[1:]
-        if tuple(k_out.shape) != shape or tuple(v_out.shape) != shape or _type(k_out) != _type(v_out):
+        if tuple(k_out.shape) != shape or tuple(v_out.shape) != shape or k_out.dtype != v_out.dtype:
             raise ValueError("kv8_read: outputs must be two arrays of shape %s" % (shape,))
-        check(lib().llmrs_kv8_read(self.ctx.h, cache._ref, _array(pages, _INT32, "pages"), n,
-                                   _array(k_out, _DTYPES, "k_out"), _array(v_out, _DTYPES, "v_out"),
-                                   _DTYPES[_type(k_out)]))
+        kp, vp = _array(k_out, _DTYPES, "k_out"), _array(v_out, _DTYPES, "v_out")
+        check(lib().llmrs_kv8_read(self.ctx.h, cache._ref, _array(pages, _INT32, "pages"), n, kp, vp,
+                                   _DTYPES[k_out.dtype]))
 
     def kv8_attention_workspace(self, cache, batch, n_heads, n_rows):
         """A workspace for kv8_attention of this many heads and rows (one call at a time)."""
@@ -541,9 +550,7 @@ class CudaBackend:
         """Causal attention of the batch's rows q [n, n_heads*head_dim] over the cache,
         after kv8_append of the same batch; writes and returns `out`."""
         d = cache.shape[3]
-        width = 1
-        for s in q.shape[1:]:
-            width *= s
+        width = q.shape[1] if len(q.shape) == 2 else int(np.prod(q.shape[1:]))
         n_heads = width // d
         if n_heads * d != width:
             raise ValueError("kv8_attention: q rows of %d elements are no heads of %d" % (width, d))

@@ -76,22 +76,13 @@ __device__ __forceinline__ void store_row(__nv_bfloat16 *p, const float (&x)[N])
     }
 }
 
-// Wait for a barrier's phase, like mbar_wait, in few instructions: a try may
-// suspend for a microsecond, and a million tries without the phase set the
-// error word.
+// Wait for a barrier's phase, like mbar_wait, in few instructions: a try suspends
+// the warp for a while, and a million tries without the phase set the error word.
 __device__ __forceinline__ bool kv8_wait(uint64_t *bar, uint32_t parity, uint32_t *err)
 {
-    for (uint32_t left = 1u << 20; left; left--) {
-        uint32_t done;
-        asm volatile("{\n\t.reg .pred p;\n\t"
-                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-                     "selp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(done)
-                     : "r"(smem_addr(bar)), "r"(parity), "r"(1000)
-                     : "memory");
-        if (done)
+    for (uint32_t left = 1u << 20; left; left--)
+        if (mbar_try_wait(bar, parity))
             return true;
-    }
     atomicCAS(err, 0u, (uint32_t)DEV_ERR_MBAR_TIMEOUT);
     return false;
 }

@@ -13,12 +13,14 @@
 // one token at a time on the host (src/main.rs:192-305).
 //
 // Two kernels.  verify_rows: every row's maximum and sum of exponentials, one
-// CTA per (row, chunk of VCHUNK tokens); bound by reading the logits once.
-// verify_pick: a cluster of PICK_CTAS CTAs per sequence decides the
-// acceptances, then walks the one row that the next token comes from, with
-// exponentials and sums in 64 bits: a draw next to the border of two tokens
-// would otherwise be decided by the rounding of a 32-bit running sum over the
-// whole vocabulary.
+// CTA per (row, chunk of VCHUNK tokens), all of a thread's 16-byte loads in
+// flight at once; bound by reading the logits once.  verify_pick: a cluster of
+// PICK_CTAS CTAs per sequence decides the acceptances, then walks the one row
+// that the next token comes from, with exponentials and sums in 64 bits: a draw
+// next to the border of two tokens would otherwise be decided by the rounding of
+// a 32-bit running sum over the whole vocabulary.  Its exponentials stay in
+// registers between the row's sum and the residual's (vocabularies up to
+// PICK_SPAN; longer ones compute them again).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -39,8 +41,11 @@ constexpr int VT = 256;         // threads of verify_rows
 constexpr int VPER = 32;        // logits a thread holds
 constexpr int VCHUNK = VT * VPER;
 constexpr int PICK_CTAS = 8;
-constexpr int PT = 512;
+constexpr int PT = 1024;
 constexpr int PW = PT / 32;
+constexpr int PWARPS = PICK_CTAS * PW;
+constexpr int PPER = 16;        // exponentials a thread holds
+constexpr int PICK_SPAN = PICK_CTAS * PT * PPER;
 
 // a chunk's part of its row's statistics
 struct RowPart {
@@ -52,6 +57,13 @@ struct RowPart {
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // a logit that is no number has no weight; infinite ones share it
 __device__ __forceinline__ float clean(float l)
@@ -81,18 +93,17 @@ __device__ __forceinline__ void warp_best(float &m, int &at)
     }
 }
 
-// sequence of a packed row, -1 behind the last one
-__device__ __forceinline__ int seq_of_row(const int *row_start, int n_seqs, int row)
+// exp(x) for x <= 0, whole warp; table: 2^(lane / 32).  x = n ln2/32 + r with
+// |r| <= ln2/64, exp(x) = 2^(n/32) (1 + r + r^2/2 + r^3/6 + r^4/24), off by
+// r^5/120 < 1.3e-12 of itself; below -700 (and for NaN) 0.
+__device__ __forceinline__ double exp64(double x, double table)
 {
-    int lo = 0, hi = n_seqs; // the last s with row_start[s] <= row
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (row_start[mid] <= row)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    return row >= row_start[lo] && row < row_start[lo + 1] ? lo : -1;
+    const bool some = x > -700.0;
+    x = some ? x : 0.0;
+    const int n = __double2int_rn(x * 46.166241308446828384);
+    const double r = fma((double)n, -0.021660849392498290195, x);
+    const double y = fma(fma(fma(fma(r, 1.0 / 24, 1.0 / 6), r, 0.5), r, 1.0), r, 1.0) * __shfl_sync(0xffffffffu, table, n & 31);
+    return some ? __hiloint2double(__double2hiint(y) + ((n >> 5) << 20), __double2loint(y)) : 0.0;
 }
 
 template <class T>
@@ -101,23 +112,47 @@ __global__ void __launch_bounds__(VT) verify_rows_kernel(VerifyParams p, RowPart
     __shared__ float s_m[VT / 32];
     __shared__ int s_at[VT / 32];
     __shared__ double s_s[VT / 32];
+    constexpr int E = 16 / (int)sizeof(T); // logits of a 16-byte load
     const int row = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const T *x = reinterpret_cast<const T *>(p.logits) + (size_t)row * p.ld;
-    const int c0 = chunk * VCHUNK, c1 = min(p.vocab, c0 + VCHUNK);
+    griddep_launch_dependents();
+    // loads on 16-byte boundaries whatever the row's: load v of the row covers the tokens E*v - skew ..
+    const int skew = (int)(((uintptr_t)x & 15) / sizeof(T)), c0 = chunk * VCHUNK - skew;
     float l[VPER];
+#pragma unroll
+    for (int i = 0; i < VPER / E; i++) {
+        const int t = c0 + (i * VT + (int)threadIdx.x) * E;
+        if (t >= 0 && t + E <= p.vocab) {
+            const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(x + t));
+            T v[E];
+            memcpy(v, &w, 16);
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                l[i * E + e] = to_float(v[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                l[i * E + e] = t + e >= 0 && t + e < p.vocab ? to_float(x[t + e]) : -INFINITY;
+        }
+    }
+    // the row's sequence, for its temperature: how many sequences end at or before the row
+    int seq = 0;
+    for (int s0 = 0; p.temperature && s0 < p.n_seqs; s0 += VT) {
+        const int s = s0 + (int)threadIdx.x;
+        seq += __syncthreads_count(s < p.n_seqs && p.row_start[s + 1] <= row);
+    }
+    const float T_ = p.temperature && seq < p.n_seqs ? p.temperature[seq] : 1.0f;
+    const float inv = T_ > 0.0f ? 1.4426950408889634f / T_ : 0.0f;
     float m = -INFINITY;
     int at = INT_MAX;
 #pragma unroll
     for (int i = 0; i < VPER; i++) {
-        const int t = c0 + i * VT + threadIdx.x;
-        l[i] = t < c1 ? clean(to_float(x[t])) : -INFINITY;
-    }
-#pragma unroll
-    for (int i = 0; i < VPER; i++)
+        l[i] = clean(l[i]);
         if (l[i] > m) {
             m = l[i];
-            at = c0 + i * VT + threadIdx.x;
+            at = c0 + ((i / E) * VT + (int)threadIdx.x) * E + i % E;
         }
+    }
     warp_best(m, at);
     if (lane == 0) {
         s_m[warp] = m;
@@ -130,13 +165,10 @@ __global__ void __launch_bounds__(VT) verify_rows_kernel(VerifyParams p, RowPart
             m = s_m[w];
             at = s_at[w];
         }
-    const int seq = seq_of_row(p.row_start, p.n_seqs, row);
-    const float T_ = seq >= 0 && p.temperature ? p.temperature[seq] : 1.0f;
-    const float inv = T_ > 0.0f ? 1.0f / T_ : 0.0f;
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < VPER; i++)
-        sum += l[i] > -INFINITY ? expf((l[i] - m) * inv) : 0.0f;
+        sum += l[i] > -INFINITY ? ex2((l[i] - m) * inv) : 0.0f;
     const double d = warp_sum_d((double)sum);
     if (lane == 0)
         s_s[warp] = d;
@@ -181,9 +213,10 @@ __global__ void __cluster_dims__(PICK_CTAS, 1, 1) __launch_bounds__(PT)
     cg::cluster_group cluster = cg::this_cluster();
     __shared__ int s_first;                       // first rejected draft
     __shared__ double s_z[PICK_CTAS];             // each CTA's share of the row's sum
-    __shared__ double s_w[2][PICK_CTAS * PW];     // each warp's share: of max(p - q, 0), of p
-    __shared__ int s_final[2][PICK_CTAS * PW];    // last token with weight in each warp's range
+    __shared__ double s_w[2][PWARPS];     // each warp's share: of max(p - q, 0), of p
+    __shared__ int s_final[2][PWARPS];    // last token with weight in each warp's range
     __shared__ double s_red[PW];
+    griddep_wait();
     const int seq = blockIdx.x / PICK_CTAS, rank = (int)cluster.block_rank();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int r0 = p.row_start[seq], r1 = p.row_start[seq + 1], n = r1 - r0;
@@ -264,17 +297,32 @@ __global__ void __cluster_dims__(PICK_CTAS, 1, 1) __launch_bounds__(PT)
     const bool rest = a < k;
     const float *q = rest && p.q ? p.q + (size_t)(d0 + a) * p.ldq : nullptr;
     const int gone = rest && !p.q ? p.draft[d0 + a] : -1; // a certain draft's own token
-    // warp `gw` of the cluster's warps owns the tokens [t0, t1)
+    // warp `gw` of the cluster's warps owns the tokens [t0, t1): lane + 32 k + PSTEP b
     const int gw = rank * PW + warp;
-    const int per = (p.vocab + PICK_CTAS * PW - 1) / (PICK_CTAS * PW);
+    const int per = (p.vocab + PWARPS - 1) / PWARPS;
     const int t0 = min(p.vocab, gw * per), t1 = min(p.vocab, t0 + per);
-    auto weight = [&](int t) { // exp((l - m) / T) in 64 bits
-        const float l = clean(to_float(x[t]));
-        return l > -INFINITY ? exp(((double)l - (double)r.m) * inv) : 0.0;
+    constexpr int PSTEP = 32 * PPER;
+    const double table = exp2((double)lane / 32);
+    double e[PPER]; // exp((l - m) / T) of tokens b + lane, b + lane + 32, ..
+    auto weights = [&](int b) {
+        float v[PPER];
+#pragma unroll
+        for (int k = 0; k < PPER; k++) {
+            const int t = b + lane + 32 * k;
+            v[k] = t < t1 ? clean(to_float(x[t])) : -INFINITY;
+        }
+#pragma unroll
+        for (int k = 0; k < PPER; k++)
+            e[k] = exp64(((double)v[k] - (double)r.m) * inv, table);
     };
+    const bool one = per <= PSTEP; // the exponentials stay in registers
     double z = 0.0;
-    for (int t = t0 + lane; t < t1; t += 32)
-        z += weight(t);
+    for (int b = t0; b < t1; b += PSTEP) {
+        weights(b);
+#pragma unroll
+        for (int k = 0; k < PPER; k++)
+            z += e[k];
+    }
     z = warp_sum_d(z);
     if (lane == 0)
         s_red[warp] = z;
@@ -290,18 +338,30 @@ __global__ void __cluster_dims__(PICK_CTAS, 1, 1) __launch_bounds__(PT)
     for (int c = 0; c < PICK_CTAS; c++)
         z += s_z[c];
     const double invz = 1.0 / z;
-    auto residual = [&](int t, double pt) {
-        const double w = t == gone ? 0.0 : q ? pt - (double)q[t] : pt;
+    // what is left of token t: max(p - q, 0), without a certain draft's own token
+    auto residual = [&](int t, double pt, float qt) {
+        const double w = t == gone ? 0.0 : pt - (double)qt;
         return w > 0.0 ? w : 0.0;
     };
+    auto q_of = [&](int t) { return q && t < t1 ? q[t] : 0.0f; };
     double sw = 0.0, sp = 0.0;
     int fw = -1, fp = -1;
-    for (int t = t0 + lane; t < t1; t += 32) {
-        const double pt = weight(t) * invz, w = residual(t, pt);
-        sw += w;
-        sp += pt;
-        fw = w > 0.0 ? t : fw;
-        fp = pt > 0.0 ? t : fp;
+    for (int b = t0; b < t1; b += PSTEP) {
+        if (!one)
+            weights(b);
+        float qt[PPER];
+#pragma unroll
+        for (int k = 0; k < PPER; k++)
+            qt[k] = q_of(b + lane + 32 * k);
+#pragma unroll
+        for (int k = 0; k < PPER; k++) {
+            const int t = b + lane + 32 * k;
+            const double pt = e[k] * invz, w = residual(t, pt, qt[k]);
+            sw += w;
+            sp += pt;
+            fw = w > 0.0 ? t : fw;
+            fp = pt > 0.0 ? t : fp;
+        }
     }
     sw = warp_sum_d(sw);
     sp = warp_sum_d(sp);
@@ -314,39 +374,53 @@ __global__ void __cluster_dims__(PICK_CTAS, 1, 1) __launch_bounds__(PT)
         cluster.map_shared_rank(&s_final[1][0], lane)[gw] = fp;
     }
     cluster.sync(); // the last access to another CTA's shared memory
-    double total = 0.0;
-    for (int w = 0; w < PICK_CTAS * PW; w++)
-        total += s_w[0][w];
-    const int use = total > 0.0 ? 0 : 1; // p equals q: nothing is left over, draw from p
-    if (use) {
-        total = 0.0;
-        for (int w = 0; w < PICK_CTAS * PW; w++)
-            total += s_w[1][w];
+    // the warp whose range the draw falls into: lane i looks at warps PWARPS/32 * i ..
+    constexpr int WL = PWARPS / 32;
+    double own[2] = {0.0, 0.0};
+    for (int i = 0; i < WL; i++) {
+        own[0] += s_w[0][lane * WL + i];
+        own[1] += s_w[1][lane * WL + i];
     }
-    const double target = (double)p.u[r1 - 1] * total;
-    double before = 0.0;
-    int owner = -1, last = -1; // the warp whose range the target falls into
-    for (int w = 0; w < PICK_CTAS * PW; w++) {
-        if (s_final[use][w] >= 0)
+    const int use = warp_sum_d(own[0]) > 0.0 ? 0 : 1; // p equals q: nothing is left over, draw from p
+    double before = use ? own[1] : own[0];            // inclusive sum over the lanes
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o)
+            before += y;
+    }
+    const double target = (double)p.u[r1 - 1] * __shfl_sync(0xffffffffu, before, 31);
+    before -= use ? own[1] : own[0];
+    int owner = -1, last = -1;
+    double until = 0.0; // the sum in front of the owner
+    for (int i = 0; i < WL; i++) {
+        const int w = lane * WL + i;
+        if (s_final[use][w] >= 0) {
             last = w;
-        if (owner < 0) {
-            if (s_final[use][w] >= 0 && before + s_w[use][w] > target)
+            if (owner < 0 && before + s_w[use][w] > target) {
                 owner = w;
-            else
-                before += s_w[use][w];
+                until = before;
+            }
         }
+        before += s_w[use][w];
     }
-    const bool past = owner < 0; // the draw lies behind the rounded sum
-    if (past)
-        owner = last;
+    last = __reduce_max_sync(0xffffffffu, last);
+    const unsigned found = __ballot_sync(0xffffffffu, owner >= 0);
+    const bool past = !found; // the draw lies behind the rounded sum
+    const int from = past ? 0 : __ffs(found) - 1;
+    owner = past ? last : __shfl_sync(0xffffffffu, owner, from);
+    until = __shfl_sync(0xffffffffu, until, from);
     if (gw != owner)
         return;
     int token = -1;
-    if (!past)
-        for (int b = t0; b < t1 && token < 0; b += 32) {
-            const int t = b + lane;
-            const double pt = t < t1 ? weight(t) * invz : 0.0;
-            const double w = t < t1 ? (use ? pt : residual(t, pt)) : 0.0;
+    double pick = 0.0; // its probability
+    for (int b = t0; b < t1 && token < 0; b += PSTEP) {
+        if (!one)
+            weights(b);
+#pragma unroll
+        for (int k = 0; k < PPER; k++) {
+            const int t = b + lane + 32 * k;
+            const double pt = e[k] * invz, w = use ? pt : residual(t, pt, q_of(t));
             double c = w;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -354,28 +428,37 @@ __global__ void __cluster_dims__(PICK_CTAS, 1, 1) __launch_bounds__(PT)
                 if (lane >= o)
                     c += y;
             }
-            const unsigned hit = __ballot_sync(0xffffffffu, w > 0.0 && before + c > target);
-            if (hit)
-                token = b + __ffs(hit) - 1;
-            before += __shfl_sync(0xffffffffu, c, 31);
+            // behind the sum: the last token with weight
+            const unsigned hit = __ballot_sync(0xffffffffu, past ? t == s_final[use][owner] : w > 0.0 && until + c > target);
+            if (hit && token < 0) {
+                token = b + 32 * k + __ffs(hit) - 1;
+                pick = __shfl_sync(0xffffffffu, pt, __ffs(hit) - 1);
+            }
+            until += __shfl_sync(0xffffffffu, c, 31);
         }
-    if (token < 0)
+    }
+    if (token < 0) { // the warp's own sum was rounded otherwise: its last token with weight
         token = s_final[use][owner];
+        pick = exp(((double)clean(to_float(x[token])) - (double)r.m) * inv) * invz;
+    }
     if (lane == 0) {
         p.tokens[row] = token;
         if (p.probs)
-            p.probs[row] = (float)(weight(token) * invz);
+            p.probs[row] = (float)pick;
     }
 }
+
+// a row that starts off a 16-byte boundary reaches up to 7 tokens further
+int chunks(int vocab) { return (vocab + 7 + VCHUNK - 1) / VCHUNK; }
 
 template <class T>
 int run(const VerifyParams &p, RowPart *part, cudaStream_t stream)
 {
-    const int n_chunks = (p.vocab + VCHUNK - 1) / VCHUNK;
+    const int n_chunks = chunks(p.vocab);
     if (p.n_rows > 0)
         LLMRS_CUDA_TRY(launch(verify_rows_kernel<T>, dim3(n_chunks, p.n_rows), dim3(VT), 0, stream, false, p, part,
                               n_chunks));
-    LLMRS_CUDA_TRY(launch(verify_pick_kernel<T>, dim3(p.n_seqs * PICK_CTAS), dim3(PT), 0, stream, false, p,
+    LLMRS_CUDA_TRY(launch(verify_pick_kernel<T>, dim3(p.n_seqs * PICK_CTAS), dim3(PT), 0, stream, p.n_rows > 0, p,
                           (const RowPart *)part, n_chunks));
     return LLMRS_OK;
 }
@@ -384,7 +467,7 @@ int run(const VerifyParams &p, RowPart *part, cudaStream_t stream)
 
 size_t verify_workspace(int n_rows, int vocab)
 {
-    return (size_t)n_rows * ((vocab + VCHUNK - 1) / VCHUNK) * sizeof(RowPart);
+    return (size_t)n_rows * chunks(vocab) * sizeof(RowPart);
 }
 
 int verify_launch(const VerifyParams &p, void *ws, cudaStream_t stream)
