@@ -236,6 +236,8 @@ int llmrs_ctx_create(int device, llmrs_ctx **out)
         rc = prefill_prepare();
     if (rc == LLMRS_OK)
         rc = kv8_prepare();
+    if (rc == LLMRS_OK)
+        rc = verify_prepare();
     if (rc != LLMRS_OK) {
         cudaFree(c->d_err);
         cudaStreamDestroy(c->own);

@@ -14,13 +14,18 @@
 //
 // Two kernels.  verify_rows: every row's maximum and sum of exponentials, one
 // CTA per (row, chunk of VCHUNK tokens), all of a thread's 16-byte loads in
-// flight at once; bound by reading the logits once.  verify_pick: a cluster of
-// PICK_CTAS CTAs per sequence decides the acceptances, then walks the one row
-// that the next token comes from, with exponentials and sums in 64 bits: a draw
-// next to the border of two tokens would otherwise be decided by the rounding of
-// a 32-bit running sum over the whole vocabulary.  Its exponentials stay in
-// registers between the row's sum and the residual's (vocabularies up to
-// PICK_SPAN; longer ones compute them again).
+// flight at once; bound by reading the logits once (35 us for 148 MB, 288 rows
+// of 128256 f32 logits).  verify_pick: a cluster of CTAs per sequence decides
+// the acceptances, then takes the one row that the next token comes from twice,
+// for its sum and for what is left of it, each warp a range of consecutive
+// tokens; the CTA whose warp holds the draw looks through that range once more.
+// Exponentials and sums are in 64 bits here: a draw next to the border of two
+// tokens would otherwise be decided by the rounding of a 32-bit running sum
+// over the whole vocabulary.  54 us for 64 such sequences, of which 4 for the
+// acceptances, 20 and 27 for the two passes (half of it conversions and 64-bit
+// arithmetic) and 2 for the end; a warp alone in its range's last look took 40.
+// (64-bit exponentials of every row in verify_rows save the first pass here
+// and cost more: 31 us.)
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -40,12 +45,9 @@ namespace {
 constexpr int VT = 256;         // threads of verify_rows
 constexpr int VPER = 32;        // logits a thread holds
 constexpr int VCHUNK = VT * VPER;
-constexpr int PICK_CTAS = 8;
-constexpr int PT = 1024;
+constexpr int PT = 512;         // threads of verify_pick
 constexpr int PW = PT / 32;
-constexpr int PWARPS = PICK_CTAS * PW;
-constexpr int PPER = 16;        // exponentials a thread holds
-constexpr int PICK_SPAN = PICK_CTAS * PT * PPER;
+constexpr int PPER = 16;        // tokens of a thread in flight
 
 // a chunk's part of its row's statistics
 struct RowPart {
@@ -206,16 +208,65 @@ __device__ __forceinline__ RowPart row_stats(const RowPart *part, int n_chunks, 
     return r;
 }
 
+// Four logits of a row from token t on, -inf outside of [0, vocab); t lies on a
+// boundary of four elements of the row's memory.
 template <class T>
-__global__ void __cluster_dims__(PICK_CTAS, 1, 1) __launch_bounds__(PT)
-    verify_pick_kernel(VerifyParams p, const RowPart *part, int n_chunks)
+__device__ __forceinline__ void load4(const T *x, int t, int vocab, float (&v)[4])
 {
+    if (t >= 0 && t + 4 <= vocab) {
+        T w[4];
+        if constexpr (sizeof(T) == 4) {
+            const uint4 raw = *reinterpret_cast<const uint4 *>(x + t);
+            memcpy(w, &raw, 16);
+        } else {
+            const uint2 raw = *reinterpret_cast<const uint2 *>(x + t);
+            memcpy(w, &raw, 8);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            v[e] = clean(to_float(w[e]));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            v[e] = t + e >= 0 && t + e < vocab ? clean(to_float(x[t + e])) : -INFINITY;
+    }
+}
+
+// the same tokens of a row of draft probabilities, of any alignment; 0 outside
+__device__ __forceinline__ void load_q4(const float *q, int t, int vocab, bool wide, float (&v)[4])
+{
+    if (wide && t >= 0 && t + 4 <= vocab) {
+        const float4 w = __ldcs(reinterpret_cast<const float4 *>(q + t));
+        v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            v[e] = t + e >= 0 && t + e < vocab ? q[t + e] : 0.0f;
+    }
+}
+
+// the sum over the CTA, in every thread; s_red: PW + 1 places, free at entry
+__device__ __forceinline__ double cta_sum(double v, double *s_red)
+{
+    const int lane = threadIdx.x & 31;
+    v = warp_sum_d(v);
+    if (lane == 0)
+        s_red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return warp_sum_d(lane < PW ? s_red[lane] : 0.0);
+}
+
+template <class T, int PICK_CTAS>
+__global__ void __launch_bounds__(PT, 2) verify_pick_kernel(VerifyParams p, const RowPart *part, int n_chunks)
+{
+    constexpr int PWARPS = PICK_CTAS * PW;
     cg::cluster_group cluster = cg::this_cluster();
-    __shared__ int s_first;                       // first rejected draft
-    __shared__ double s_z[PICK_CTAS];             // each CTA's share of the row's sum
-    __shared__ double s_w[2][PWARPS];     // each warp's share: of max(p - q, 0), of p
-    __shared__ int s_final[2][PWARPS];    // last token with weight in each warp's range
+    __shared__ int s_first;                   // first rejected draft
     __shared__ double s_red[PW];
+    __shared__ double s_z[PICK_CTAS];         // each CTA's share of the row's sum
+    __shared__ double s_w[2][PWARPS];         // each warp's share: of max(p - q, 0), of p
+    __shared__ int s_final[2][PWARPS];        // last token with weight in each warp's range
+    __shared__ int s_hit;
     griddep_wait();
     const int seq = blockIdx.x / PICK_CTAS, rank = (int)cluster.block_rank();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -293,46 +344,33 @@ __global__ void __cluster_dims__(PICK_CTAS, 1, 1) __launch_bounds__(PT)
         }
         return;
     }
+    cluster.barrier_arrive(); // every CTA has begun before another writes to its shared memory
     const T *x = reinterpret_cast<const T *>(p.logits) + (size_t)row * p.ld;
     const bool rest = a < k;
     const float *q = rest && p.q ? p.q + (size_t)(d0 + a) * p.ldq : nullptr;
     const int gone = rest && !p.q ? p.draft[d0 + a] : -1; // a certain draft's own token
-    // warp `gw` of the cluster's warps owns the tokens [t0, t1): lane + 32 k + PSTEP b
-    const int gw = rank * PW + warp;
-    const int per = (p.vocab + PWARPS - 1) / PWARPS;
-    const int t0 = min(p.vocab, gw * per), t1 = min(p.vocab, t0 + per);
-    constexpr int PSTEP = 32 * PPER;
+    // warp `gw` of the cluster's warps owns the tokens [t0, t1); the ranges' ends lie on
+    // boundaries of four elements in memory, the row's own ends mask the rest
+    const int skew = (int)(((uintptr_t)x / sizeof(T)) & 3), gw = rank * PW + warp;
+    const int per = ((p.vocab + skew + 3) / 4 + PWARPS - 1) / PWARPS * 4;
+    const int t0 = min(p.vocab, gw * per - skew), t1 = min(p.vocab, (gw + 1) * per - skew);
+    const bool wide = q && ((uintptr_t)(q - skew) & 15) == 0;
     const double table = exp2((double)lane / 32);
-    double e[PPER]; // exp((l - m) / T) of tokens b + lane, b + lane + 32, ..
-    auto weights = [&](int b) {
-        float v[PPER];
-#pragma unroll
-        for (int k = 0; k < PPER; k++) {
-            const int t = b + lane + 32 * k;
-            v[k] = t < t1 ? clean(to_float(x[t])) : -INFINITY;
-        }
-#pragma unroll
-        for (int k = 0; k < PPER; k++)
-            e[k] = exp64(((double)v[k] - (double)r.m) * inv, table);
-    };
-    const bool one = per <= PSTEP; // the exponentials stay in registers
+    auto weight = [&](float l) { return exp64(((double)l - (double)r.m) * inv, table); };
     double z = 0.0;
-    for (int b = t0; b < t1; b += PSTEP) {
-        weights(b);
+    for (int b = t0; b < t1; b += 32 * PPER) {
+        float v[PPER / 4][4];
+#pragma unroll
+        for (int k = 0; k < PPER / 4; k++)
+            load4(x, b + (k * 32 + lane) * 4, t1, v[k]);
 #pragma unroll
         for (int k = 0; k < PPER; k++)
-            z += e[k];
+            z += weight(v[k / 4][k % 4]);
     }
-    z = warp_sum_d(z);
-    if (lane == 0)
-        s_red[warp] = z;
-    __syncthreads();
-    if (threadIdx.x < PICK_CTAS) {
-        double c = 0.0;
-        for (int w = 0; w < PW; w++)
-            c += s_red[w];
-        cluster.map_shared_rank(s_z, threadIdx.x)[rank] = c;
-    }
+    z = cta_sum(z, s_red);
+    cluster.barrier_wait();
+    if (threadIdx.x < PICK_CTAS)
+        cluster.map_shared_rank(s_z, threadIdx.x)[rank] = z;
     cluster.sync();
     z = 0.0;
     for (int c = 0; c < PICK_CTAS; c++)
@@ -343,20 +381,21 @@ __global__ void __cluster_dims__(PICK_CTAS, 1, 1) __launch_bounds__(PT)
         const double w = t == gone ? 0.0 : pt - (double)qt;
         return w > 0.0 ? w : 0.0;
     };
-    auto q_of = [&](int t) { return q && t < t1 ? q[t] : 0.0f; };
     double sw = 0.0, sp = 0.0;
     int fw = -1, fp = -1;
-    for (int b = t0; b < t1; b += PSTEP) {
-        if (!one)
-            weights(b);
-        float qt[PPER];
+    for (int b = t0; b < t1; b += 32 * PPER) {
+        float v[PPER / 4][4], qt[PPER / 4][4] = {};
 #pragma unroll
-        for (int k = 0; k < PPER; k++)
-            qt[k] = q_of(b + lane + 32 * k);
+        for (int k = 0; k < PPER / 4; k++) {
+            const int t = b + (k * 32 + lane) * 4;
+            load4(x, t, t1, v[k]);
+            if (q)
+                load_q4(q, t, t1, wide, qt[k]);
+        }
 #pragma unroll
         for (int k = 0; k < PPER; k++) {
-            const int t = b + lane + 32 * k;
-            const double pt = e[k] * invz, w = residual(t, pt, qt[k]);
+            const int t = b + (k / 4 * 32 + lane) * 4 + k % 4;
+            const double pt = weight(v[k / 4][k % 4]) * invz, w = residual(t, pt, qt[k / 4][k % 4]);
             sw += w;
             sp += pt;
             fw = w > 0.0 ? t : fw;
@@ -374,25 +413,30 @@ __global__ void __cluster_dims__(PICK_CTAS, 1, 1) __launch_bounds__(PT)
         cluster.map_shared_rank(&s_final[1][0], lane)[gw] = fp;
     }
     cluster.sync(); // the last access to another CTA's shared memory
-    // the warp whose range the draw falls into: lane i looks at warps PWARPS/32 * i ..
+    // the warp whose range the draw falls into: lane i looks at warps WL * i ..
     constexpr int WL = PWARPS / 32;
     double own[2] = {0.0, 0.0};
+#pragma unroll
     for (int i = 0; i < WL; i++) {
         own[0] += s_w[0][lane * WL + i];
         own[1] += s_w[1][lane * WL + i];
     }
     const int use = warp_sum_d(own[0]) > 0.0 ? 0 : 1; // p equals q: nothing is left over, draw from p
-    double before = use ? own[1] : own[0];            // inclusive sum over the lanes
+    auto scan = [&](double c) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o)
-            before += y;
-    }
+        for (int o = 1; o < 32; o <<= 1) {
+            const double y = __shfl_up_sync(0xffffffffu, c, o);
+            if (lane >= o)
+                c += y;
+        }
+        return c;
+    };
+    double before = scan(use ? own[1] : own[0]);
     const double target = (double)p.u[r1 - 1] * __shfl_sync(0xffffffffu, before, 31);
     before -= use ? own[1] : own[0];
     int owner = -1, last = -1;
     double until = 0.0; // the sum in front of the owner
+#pragma unroll
     for (int i = 0; i < WL; i++) {
         const int w = lane * WL + i;
         if (s_final[use][w] >= 0) {
@@ -410,46 +454,91 @@ __global__ void __cluster_dims__(PICK_CTAS, 1, 1) __launch_bounds__(PT)
     const int from = past ? 0 : __ffs(found) - 1;
     owner = past ? last : __shfl_sync(0xffffffffu, owner, from);
     until = __shfl_sync(0xffffffffu, until, from);
-    if (gw != owner)
+    if (owner / PW != rank)
         return;
-    int token = -1;
-    double pick = 0.0; // its probability
-    for (int b = t0; b < t1 && token < 0; b += PSTEP) {
-        if (!one)
-            weights(b);
+    // the owner's CTA walks the range, four consecutive tokens of a thread, their sums scanned
+    const int o0 = owner * per - skew, o1 = min(p.vocab, o0 + per);
+    for (int b = o0; b < o1 && !past; b += PT * 4) {
+        const int t = b + (int)threadIdx.x * 4;
+        float v[4], qt[4] = {};
+        load4(x, t, o1, v);
+        if (q)
+            load_q4(q, t, o1, wide, qt);
+        double pt[4], w[4], mine = 0.0;
 #pragma unroll
-        for (int k = 0; k < PPER; k++) {
-            const int t = b + lane + 32 * k;
-            const double pt = e[k] * invz, w = use ? pt : residual(t, pt, q_of(t));
-            double c = w;
+        for (int e = 0; e < 4; e++) {
+            pt[e] = weight(v[e]) * invz;
+            w[e] = use ? pt[e] : residual(t + e, pt[e], qt[e]);
+            mine += w[e];
+        }
+        const double c = scan(mine);
+        __syncthreads();
+        if (threadIdx.x == 0)
+            s_hit = INT_MAX;
+        if (lane == 31)
+            s_red[warp] = c;
+        __syncthreads();
+        const double ends = scan(lane < PW ? s_red[lane] : 0.0); // of the warps
+        double front = until + (c - mine) + (warp ? __shfl_sync(0xffffffffu, ends, warp - 1) : 0.0), at = 0.0;
+        until += __shfl_sync(0xffffffffu, ends, 31);
+        int hit = INT_MAX;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(0xffffffffu, c, o);
-                if (lane >= o)
-                    c += y;
+        for (int e = 0; e < 4; e++) {
+            front += w[e];
+            if (hit == INT_MAX && w[e] > 0.0 && front > target) {
+                hit = t + e;
+                at = pt[e];
             }
-            // behind the sum: the last token with weight
-            const unsigned hit = __ballot_sync(0xffffffffu, past ? t == s_final[use][owner] : w > 0.0 && until + c > target);
-            if (hit && token < 0) {
-                token = b + 32 * k + __ffs(hit) - 1;
-                pick = __shfl_sync(0xffffffffu, pt, __ffs(hit) - 1);
+        }
+        const int first = __reduce_min_sync(0xffffffffu, hit);
+        if (lane == 0 && first != INT_MAX)
+            atomicMin(&s_hit, first);
+        __syncthreads();
+        if (s_hit != INT_MAX) {
+            if (hit == s_hit) {
+                p.tokens[row] = hit;
+                if (p.probs)
+                    p.probs[row] = (float)at;
             }
-            until += __shfl_sync(0xffffffffu, c, 31);
+            return;
         }
     }
-    if (token < 0) { // the warp's own sum was rounded otherwise: its last token with weight
-        token = s_final[use][owner];
-        pick = exp(((double)clean(to_float(x[token])) - (double)r.m) * inv) * invz;
-    }
-    if (lane == 0) {
+    // no running sum exceeds the target: the last token with weight
+    const int token = s_final[use][owner];
+    if (threadIdx.x == 0) {
         p.tokens[row] = token;
         if (p.probs)
-            p.probs[row] = (float)pick;
+            p.probs[row] = (float)(exp(((double)clean(to_float(x[token])) - (double)r.m) * inv) * invz);
     }
 }
 
 // a row that starts off a 16-byte boundary reaches up to 7 tokens further
 int chunks(int vocab) { return (vocab + 7 + VCHUNK - 1) / VCHUNK; }
+
+template <class T, int CTAS>
+int pick(const VerifyParams &p, const RowPart *part, int n_chunks, cudaStream_t stream)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.n_seqs * CTAS);
+    cfg.blockDim = dim3(PT);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CTAS;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.n_rows > 0 ? 2 : 1;
+    LLMRS_CUDA_TRY(cudaLaunchKernelEx(&cfg, verify_pick_kernel<T, CTAS>, p, part, n_chunks));
+    return LLMRS_OK;
+}
+
+template <class T>
+cudaError_t prepare()
+{
+    return cudaFuncSetAttribute(verify_pick_kernel<T, 16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+}
 
 template <class T>
 int run(const VerifyParams &p, RowPart *part, cudaStream_t stream)
@@ -458,9 +547,12 @@ int run(const VerifyParams &p, RowPart *part, cudaStream_t stream)
     if (p.n_rows > 0)
         LLMRS_CUDA_TRY(launch(verify_rows_kernel<T>, dim3(n_chunks, p.n_rows), dim3(VT), 0, stream, false, p, part,
                               n_chunks));
-    LLMRS_CUDA_TRY(launch(verify_pick_kernel<T>, dim3(p.n_seqs * PICK_CTAS), dim3(PT), 0, stream, p.n_rows > 0, p,
-                          (const RowPart *)part, n_chunks));
-    return LLMRS_OK;
+    // the largest cluster with which all sequences' clusters fit at once, two CTAs an SM
+    if (p.n_seqs * 16 <= 296)
+        return pick<T, 16>(p, part, n_chunks, stream);
+    if (p.n_seqs * 8 <= 296)
+        return pick<T, 8>(p, part, n_chunks, stream);
+    return pick<T, 4>(p, part, n_chunks, stream);
 }
 
 } // namespace
@@ -468,6 +560,18 @@ int run(const VerifyParams &p, RowPart *part, cudaStream_t stream)
 size_t verify_workspace(int n_rows, int vocab)
 {
     return (size_t)n_rows * chunks(vocab) * sizeof(RowPart);
+}
+
+int verify_prepare(void)
+{
+    cudaError_t e = prepare<float>();
+    if (e == cudaSuccess)
+        e = prepare<__half>();
+    if (e == cudaSuccess)
+        e = prepare<__nv_bfloat16>();
+    if (e != cudaSuccess)
+        return fail(LLMRS_ECUDA, "verification kernel attributes: %s", cudaGetErrorString(e));
+    return LLMRS_OK;
 }
 
 int verify_launch(const VerifyParams &p, void *ws, cudaStream_t stream)

@@ -24,6 +24,8 @@ struct VerifyParams {
 };
 
 size_t verify_workspace(int n_rows, int vocab);
+// set kernel attributes on the current device (once per context, outside capture)
+int verify_prepare(void);
 int verify_launch(const VerifyParams &p, void *ws, cudaStream_t stream);
 
 } // namespace llmrs
