@@ -42,8 +42,9 @@ namespace llmrs {
 namespace {
 
 constexpr int FT = 32;        // tokens of a tile
-constexpr int FW = 8;         // warps of a CTA
-constexpr int F_MAX_CTAS = JOIN_SLOTS / FW;
+// warps of a CTA by column tiles: as many as the registers of a thread allow
+constexpr int few_warps(int nt) { return nt == 1 ? 12 : 8; }
+constexpr int F_MAX_CTAS = JOIN_SLOTS / few_warps(1);
 
 struct FewParams {
     CUtensorMap tk, tv; // code pools as rows of D bytes
@@ -55,24 +56,26 @@ struct FewParams {
 
 // what a warp needs to know of one tile
 struct __align__(16) Tile {
-    int row0, row1;       // pool rows of its 16-token halves (row1: only for pages of 16); -1: not there
-    int s, group, g, tile; // pair, and the tile's index in it
-    int n_tiles, len, r0, n; // of the sequence: tiles, cached tokens, first row, rows
+    int row0, row1;         // pool rows of its 16-token halves (row1: only for pages of 16); -1: not there
     float ks0, ks1, vs0, vs1;
-    int pad0, pad1;
+    int s, pair, tile;      // sequence, its KV head and group, and the tile's index in the pair
+    int len, r0, n;         // of the sequence: cached tokens, first row, rows
+    __device__ int n_tiles() const { return (int)(((long long)len + n + FT - 1) / FT); }
 };
-static_assert(sizeof(Tile) == 64, "four 16-byte words");
+static_assert(sizeof(Tile) == 48, "three 16-byte words");
 
-template <int D>
+template <int D, int NT>
 struct FewLay {
-    static constexpr int STAGES = D == 128 ? 3 : 6;
+    static constexpr int FW = few_warps(NT);
+    static constexpr int STAGES = (NT == 1 ? 2 : 3) * (128 / D);
     static constexpr int BOX = FT * D;            // bytes of K or V codes of a tile
     static constexpr int RING = STAGES * 2 * BOX; // per warp
-    static constexpr int TILES = 64;              // tile records per warp: two batches of 32
+    static constexpr int BATCH = 32;              // tile records made at a time
+    static constexpr int TILES = BATCH + 16;      // and held per warp
     static constexpr int tile_off = FW * RING;
     static constexpr int bar_off = tile_off + FW * TILES * (int)sizeof(Tile);
-    static constexpr int bytes = bar_off + FW * STAGES * 8 + 1024; // + alignment slack
-    static_assert(bytes <= 232448, "shared memory of one CTA");
+    static constexpr int bytes = bar_off + FW * STAGES * 16 + 1024; // + alignment slack
+    static_assert(bytes <= 232448 - 1024, "shared memory of one CTA, beside the static part");
 };
 
 __device__ __forceinline__ void tma_box(void *dst, const CUtensorMap *map, int row, uint64_t *bar, uint64_t policy)
@@ -118,9 +121,10 @@ __device__ __forceinline__ long long seq_tiles(const FewParams &p, int n, int le
 
 // T: type of the rows; SPLIT: two f16 pieces per value (f32 rows); NT: columns / 8
 template <class T, int D, bool SPLIT, int NT>
-__global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_constant__ FewParams p)
+__global__ void __launch_bounds__(few_warps(NT) * 32, 1) kv8_few_kernel(const __grid_constant__ FewParams p)
 {
-    using Lay = FewLay<D>;
+    using Lay = FewLay<D, NT>;
+    constexpr int FW = Lay::FW;
     constexpr int GV = group_vectors<SPLIT, NT>();
     constexpr int KS = D / 16;    // k steps of q.k
     constexpr int LD = D / 4;     // dims of q.k a lane holds: LD*t ..
@@ -136,9 +140,9 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
 
     uint8_t *ring = smem + warp * Lay::RING;
     Tile *rec = reinterpret_cast<Tile *>(smem + Lay::tile_off) + warp * Lay::TILES;
-    uint64_t *bar = reinterpret_cast<uint64_t *>(smem + Lay::bar_off) + warp * ST;
+    uint64_t *bar = reinterpret_cast<uint64_t *>(smem + Lay::bar_off) + warp * 2 * ST; // K, V of a stage
     if (lane == 0) {
-        for (int i = 0; i < ST; i++)
+        for (int i = 0; i < 2 * ST; i++)
             mbar_init(&bar[i], 1);
         fence_mbar_init();
     }
@@ -255,17 +259,16 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
         const long long first = __shfl_sync(0xffffffffu, incl - c, jj);
         Tile x;
         x.s = win_s + jj;
-        x.n_tiles = __shfl_sync(0xffffffffu, tiles, jj);
+        const int n_tiles = __shfl_sync(0xffffffffu, tiles, jj);
         x.len = __shfl_sync(0xffffffffu, len, jj);
         x.r0 = __shfl_sync(0xffffffffu, r0, jj);
         x.n = __shfl_sync(0xffffffffu, n, jj);
         const int ng = __shfl_sync(0xffffffffu, groups, jj);
         if (here) {
             const long long r = u - first;
-            const int pair = (int)(r / x.n_tiles);
-            x.tile = (int)(r - (long long)pair * x.n_tiles);
-            x.g = pair / ng; // the groups of a KV head follow one another and share its codes in the L2
-            x.group = pair - x.g * ng;
+            x.pair = (int)(r / n_tiles); // the groups of a KV head follow one another and share its codes in the L2
+            x.tile = (int)(r - (long long)x.pair * n_tiles);
+            const int g = x.pair / ng;
             const int t0 = x.tile * FT;
             auto piece = [&](int pos, int &row, float &ks, float &vs) {
                 row = -1;
@@ -275,7 +278,7 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
                 const int id = kv8_page(a.b, a.c, x.s, pos / page, a.err);
                 if (id < 0)
                     return;
-                const size_t at = (size_t)id * a.c.n_kv + x.g;
+                const size_t at = (size_t)id * a.c.n_kv + g;
                 row = (int)(at * page) + pos % page;
                 ks = a.c.ks[at];
                 vs = a.c.vs[at];
@@ -288,11 +291,10 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
                 x.ks1 = x.ks0;
                 x.vs1 = x.vs0;
             }
-            x.pad0 = x.pad1 = 0;
             const int4 *src = reinterpret_cast<const int4 *>(&x);
-            int4 *dst = reinterpret_cast<int4 *>(&rec[(made + lane) & (Lay::TILES - 1)]);
+            int4 *dst = reinterpret_cast<int4 *>(&rec[(made + lane) % Lay::TILES]);
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 3; i++)
                 dst[i] = src[i];
         }
         made += __popc(__ballot_sync(0xffffffffu, here));
@@ -301,28 +303,22 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
 
     const int mine = (int)(hi - lo);
     const uint64_t policy = policy_evict_first();
-    auto issue = [&](int i) { // lane 0: tile i into stage i % ST
-        const Tile &x = rec[i & (Lay::TILES - 1)];
-        uint8_t *dst = ring + (i % ST) * 2 * Lay::BOX;
-        uint64_t *b = &bar[i % ST];
+    auto issue = [&](int i, int v) { // lane 0: the K (v = 0) or V codes of tile i into stage i % ST
+        const Tile &x = rec[i % Lay::TILES];
+        uint8_t *dst = ring + ((i % ST) * 2 + v) * Lay::BOX;
+        uint64_t *b = &bar[(i % ST) * 2 + v];
+        const CUtensorMap *map = v ? &p.tv : &p.tk;
         const int row0 = x.row0, row1 = x.row1;
         if (page == 16) {
-            const uint32_t bytes = (row0 >= 0 ? Lay::BOX : 0) + (row1 >= 0 ? Lay::BOX : 0);
-            mbar_arrive_expect_tx(b, bytes);
-            if (row0 >= 0) {
-                tma_box(dst, &p.tk, row0, b, policy);
-                tma_box(dst + Lay::BOX, &p.tv, row0, b, policy);
-            }
-            if (row1 >= 0) {
-                tma_box(dst + Lay::BOX / 2, &p.tk, row1, b, policy);
-                tma_box(dst + Lay::BOX + Lay::BOX / 2, &p.tv, row1, b, policy);
-            }
+            mbar_arrive_expect_tx(b, ((row0 >= 0) + (row1 >= 0)) * (Lay::BOX / 2));
+            if (row0 >= 0)
+                tma_box(dst, map, row0, b, policy);
+            if (row1 >= 0)
+                tma_box(dst + Lay::BOX / 2, map, row1, b, policy);
         } else {
-            mbar_arrive_expect_tx(b, row0 >= 0 ? 2 * Lay::BOX : 0);
-            if (row0 >= 0) {
-                tma_box(dst, &p.tk, row0, b, policy);
-                tma_box(dst + Lay::BOX, &p.tv, row0, b, policy);
-            }
+            mbar_arrive_expect_tx(b, row0 >= 0 ? Lay::BOX : 0);
+            if (row0 >= 0)
+                tma_box(dst, map, row0, b, policy);
         }
     };
 
@@ -331,11 +327,15 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
     float acc[MT][NT][4];       // O^T: (dim row gl / gl+8, column 2t4 / 2t4+1)
     float m[NT][2], l[NT][2], fac[NT][2];
     int lim[NT][2];             // last position the column's row attends to
+    int pair_g = 0, pair_group = 0; // its KV head and group
     auto begin = [&](const Tile &x) {
+        const int groups = (x.n * rep + GV - 1) / GV;
+        pair_g = x.pair / groups;
+        pair_group = x.pair - pair_g * groups;
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-            const int v = x.group * GV + (SPLIT ? 4 * j + (gl & 3) : 8 * j + gl);
-            const int row = v / rep, head = x.g * rep + v % rep;
+            const int v = pair_group * GV + (SPLIT ? 4 * j + (gl & 3) : 8 * j + gl);
+            const int row = v / rep, head = pair_g * rep + v % rep;
             const bool live = row < x.n;
             float q[LD];
             float big = 0.0f;
@@ -405,7 +405,28 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
         }
     };
 
-    auto consume = [&](const Tile &x, const uint8_t *kb, const uint8_t *vb) {
+    int k_issued = 0, v_issued = 0; // tiles
+    bool ok = true;
+    auto arrived = [&](int i, int v) {
+        if (ok)
+            ok = kv8_wait(&bar[(i % ST) * 2 + v], (uint32_t)((i / ST) & 1), a.err);
+        ok = __all_sync(0xffffffffu, ok);
+        return ok;
+    };
+    auto refill = [&](int v, int &issued) { // the warp has read a stage
+        __syncwarp();
+        if (issued < mine) {
+            if (lane == 0) {
+                fence_proxy_async_smem(); // reads before the refill
+                issue(issued, v);
+            }
+            issued++;
+        }
+    };
+    auto consume = [&](const Tile &x, int at) {
+        const uint8_t *kb = ring + (at % ST) * 2 * Lay::BOX, *vb = kb + Lay::BOX;
+        if (!arrived(at, 0))
+            return;
         float s[2][NT][4];
 #pragma unroll
         for (int mt = 0; mt < 2; mt++) {
@@ -437,7 +458,7 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
                 }
             }
         }
-        // values of the tile's tokens 2t4, 2t4+1, 2t4+8, 2t4+9 (each half): the lane's LV dims
+        refill(0, k_issued);
         const float vs0 = x.vs0 * (1.0f / P_SCALE), vs1 = x.vs1 * (1.0f / P_SCALE);
         const bool half = page == 16;
         const int t0 = x.tile * FT;
@@ -499,8 +520,11 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
             for (int c = 0; c < 2; c++)
                 l[j][c] = l[j][c] * corr[j][c] + sum[c];
         }
+        if (!arrived(at, 1))
+            return;
         // O^T += V^T P: the tile's product in fresh accumulators, then one f32 step
-        constexpr int W = LV / 4; // 32-bit words of a token's LV codes
+        // a token's LV codes, tokens 2t4, 2t4+1, 2t4+8, 2t4+9 of each half
+        constexpr int W = LV / 4; // 32-bit words
         uint32_t vw[2][4][W];
 #pragma unroll
         for (int mt = 0; mt < 2; mt++)
@@ -516,6 +540,7 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
                     vw[mt][i][0] = w.x, vw[mt][i][1] = w.y;
                 }
             }
+        refill(1, v_issued);
 #pragma unroll
         for (int k = 0; k < W; k++) {
             float f[2][NT][4];
@@ -571,8 +596,8 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
         const int which = from_start ? 1 : 0;
         float *part = p.part + ((size_t)slot * 2 + which) * GV * (D + 2);
         if (from_start && !to_end && lane == 0) { // hi - 1 is tile x.tile; the range that holds the pair's last one
-            const long long end = hi - 1 + (x.n_tiles - 1 - x.tile);
-            p.head[slot] = make_int4(x.s, x.group, x.g, (int)(((end + 1) * active - 1) / total) - slot + 1);
+            const long long end = hi - 1 + (x.n_tiles() - 1 - x.tile);
+            p.head[slot] = make_int4(x.s, pair_group, pair_g, (int)(((end + 1) * active - 1) / total) - slot + 1);
         }
 #pragma unroll
         for (int j = 0; j < NT; j++) {
@@ -593,7 +618,7 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
                         o[2 * i + h] = y;
                     }
                 const int vi = SPLIT ? 4 * j + 2 * t4 + c : 8 * j + 2 * t4 + c; // vector within the group
-                const int v = x.group * GV + vi;
+                const int v = pair_group * GV + vi;
                 if ((SPLIT && t4 >= 2) || v >= x.n * rep)
                     continue;
                 if (done) {
@@ -602,7 +627,7 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
                     for (int i = 0; i < LV; i++)
                         o[i] *= inv;
                     T *out = reinterpret_cast<T *>(a.out) + (size_t)(x.r0 + v / rep) * a.ld_out +
-                             (size_t)(x.g * rep + v % rep) * D + LV * gl;
+                             (size_t)(pair_g * rep + v % rep) * D + LV * gl;
                     store_row<LV>(out, o);
                 } else {
                     float *dst = part + (size_t)vi * D + LV * gl;
@@ -616,50 +641,37 @@ __global__ void __launch_bounds__(FW * 32, 1) kv8_few_kernel(const __grid_consta
         }
     };
 
-    describe();
-    int issued = 0;
+    while (made < min(mine, ST))
+        describe();
+    k_issued = v_issued = min(mine, ST);
     if (lane == 0)
-        for (; issued < ST && issued < min(made, mine); issued++)
-            issue(issued);
-    issued = __shfl_sync(0xffffffffu, issued, 0);
-    bool ok = true, from_start = false;
+        for (int i = 0; i < k_issued; i++) {
+            issue(i, 0);
+            issue(i, 1);
+        }
+    bool from_start = false;
     int done = 0; // tiles consumed
-    for (int i = 0; i < mine; i++) {
-        // records ahead of the loads: a batch is made when the last one is half used
-        if (made < mine && made - i <= 32)
+    for (; done < mine; done++) {
+        // records ahead of the loads
+        while (made < mine && made - done <= Lay::TILES - Lay::BATCH)
             describe();
-        if (lane == 0)
-            for (; issued < min(made, mine) && issued < i + ST; issued++)
-                issue(issued);
-        const Tile x = rec[i & (Lay::TILES - 1)];
-        if (i == 0 || x.tile == 0) {
+        const Tile x = rec[done % Lay::TILES];
+        if (done == 0 || x.tile == 0) {
             from_start = x.tile == 0;
             begin(x);
         }
-        if (ok)
-            ok = kv8_wait(&bar[i % ST], (uint32_t)((i / ST) & 1), a.err);
-        ok = __all_sync(0xffffffffu, ok);
+        consume(x, done);
         if (!ok)
             break;
-        const uint8_t *kb = ring + (i % ST) * 2 * Lay::BOX;
-        consume(x, kb, kb + Lay::BOX);
-        done++;
-        __syncwarp();
-        if (lane == 0) {
-            fence_proxy_async_smem(); // this warp's reads of the stage precede its refill
-            if (issued == i + ST && issued < min(made, mine)) {
-                issue(issued);
-                issued++;
-            }
-        }
-        const bool to_end = x.tile == x.n_tiles - 1;
-        if (to_end || i == mine - 1)
+        const bool to_end = x.tile == x.n_tiles() - 1;
+        if (to_end || done == mine - 1)
             finish(x, from_start, to_end);
     }
     if (!ok && lane == 0) // copies in flight land before the shared memory goes
-        for (; done < issued; done++)
-            for (int it = 0; it < 100000 && !mbar_try_wait(&bar[done % ST], (uint32_t)((done / ST) & 1)); it++)
-                ;
+        for (int i = done; i < k_issued; i++)
+            for (int v = 0; v < 2 && (v == 0 || i < v_issued); v++)
+                for (int it = 0; it < 100000 && !mbar_try_wait(&bar[(i % ST) * 2 + v], (uint32_t)((i / ST) & 1)); it++)
+                    ;
 }
 
 // a code pool as rows of D bytes in swizzled boxes of `rows` rows
@@ -685,8 +697,9 @@ template <class T, int D, bool SPLIT, int NT>
 int run_few(const FewParams &p, int ctas, cudaStream_t stream)
 {
     constexpr int GV = group_vectors<SPLIT, NT>();
-    LLMRS_CUDA_TRY(launch(kv8_few_kernel<T, D, SPLIT, NT>, dim3(ctas), dim3(FW * 32), FewLay<D>::bytes, stream, false,
-                          p));
+    constexpr int FW = few_warps(NT);
+    LLMRS_CUDA_TRY(launch(kv8_few_kernel<T, D, SPLIT, NT>, dim3(ctas), dim3(FW * 32), FewLay<D, NT>::bytes, stream,
+                          false, p));
     LLMRS_CUDA_TRY(launch(kv8_join_kernel<T, D, GV>, dim3(2 * ctas), dim3(JT), 0, stream, true, p.a,
                           (const float *)p.part, (const int4 *)p.head, ctas * FW, 0));
     return LLMRS_OK;
@@ -697,9 +710,7 @@ int run_nt(const FewParams &p, int nt, int ctas, cudaStream_t stream)
 {
     if (nt == 1)
         return run_few<T, D, SPLIT, 1>(p, ctas, stream);
-    if (nt == 2)
-        return run_few<T, D, SPLIT, 2>(p, ctas, stream);
-    return run_few<T, D, SPLIT, 4>(p, ctas, stream);
+    return run_few<T, D, SPLIT, 2>(p, ctas, stream);
 }
 
 template <class T, bool SPLIT>
@@ -712,7 +723,7 @@ template <class T, bool SPLIT, int D, int NT>
 cudaError_t prepare_few()
 {
     return cudaFuncSetAttribute(kv8_few_kernel<T, D, SPLIT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                FewLay<D>::bytes);
+                                FewLay<D, NT>::bytes);
 }
 
 template <class T, bool SPLIT>
@@ -722,22 +733,19 @@ cudaError_t prepare_all()
     if (e == cudaSuccess)
         e = prepare_few<T, SPLIT, 128, 2>();
     if (e == cudaSuccess)
-        e = prepare_few<T, SPLIT, 128, 4>();
-    if (e == cudaSuccess)
         e = prepare_few<T, SPLIT, 64, 1>();
     if (e == cudaSuccess)
         e = prepare_few<T, SPLIT, 64, 2>();
-    if (e == cudaSuccess)
-        e = prepare_few<T, SPLIT, 64, 4>();
     return e;
 }
 
 // columns / 8 for the average sequence's vectors per KV head: a longer sequence
-// takes several groups.  A column more than needed costs its products and
-// registers, a group more reads the codes again (from the L2, mostly).
+// takes several groups, and each reads the codes again (from the L2, mostly).
+// 32 columns at a head of 128 do not fit the registers (f32 rows, 16 sequences
+// of 300 to 4000 tokens, 16 vectors each: 96 us against 68 for two groups).
 int few_nt(long long vectors, int per)
 {
-    return vectors <= per ? 1 : vectors <= 2 * per ? 2 : 4;
+    return vectors <= per ? 1 : 2;
 }
 
 long long mean_vectors(int rep, int n_rows, int n_seqs)
@@ -745,14 +753,18 @@ long long mean_vectors(int rep, int n_rows, int n_seqs)
     return n_seqs > 0 ? ((long long)n_rows + n_seqs - 1) / n_seqs * rep : 0;
 }
 
-// vectors per KV head from which on a sequence goes to the kernel for many rows
-constexpr int MANY = 64;
+// A sequence with more vectors per KV head than this goes to the kernel for many
+// rows: three groups here cost what its tile of 128 rows costs whatever it holds.
+// 16 sequences of 300 to 4000 tokens, heads of 128, f32 rows: 16 vectors 68 us
+// here, 88 there, 32 vectors 109 and 90; bf16 rows: 32 vectors 72 and 79, 48
+// vectors 93 and 82; heads of 64 cross at the same places.
+constexpr int many_from(int dtype) { return 3 * (dtype == LLMRS_BF16 ? 16 : 8); }
 
 // whether a sequence may have that many: with no more rows than sequences (a
 // decode step) every sequence is taken to have few, which is right for any
-bool some_many(int rep, int n_rows, int n_seqs)
+bool some_many(int rep, int n_rows, int n_seqs, int from)
 {
-    return rep <= MANY_MAX_REP && n_rows > n_seqs && (long long)n_rows * rep > MANY;
+    return rep <= MANY_MAX_REP && n_rows > n_seqs && (long long)n_rows * rep > from;
 }
 
 } // namespace
@@ -762,7 +774,7 @@ size_t kv8_attention_workspace(int rep, int head_dim, int n_rows, int n_seqs)
     // two pieces a warp, of the vectors of a group (16-bit rows: eight to a column tile)
     const int gv = 8 * few_nt(mean_vectors(rep, n_rows, n_seqs), 4);
     const size_t few = JOIN_SLOTS * (sizeof(int4) + 2 * (size_t)gv * (head_dim + 2) * sizeof(float));
-    return some_many(rep, n_rows, n_seqs) ? std::max(few, kv8_many_workspace(head_dim)) : few;
+    return some_many(rep, n_rows, n_seqs, many_from(LLMRS_F32)) ? std::max(few, kv8_many_workspace(head_dim)) : few;
 }
 
 int kv8_prepare(void)
@@ -780,16 +792,17 @@ int kv8_prepare(void)
 int kv8_attention(const Kv8Attn &a, void *ws, int sms, cudaStream_t stream)
 {
     const int rep = a.n_heads / a.c.n_kv;
-    const bool both = some_many(rep, a.b.n_rows, a.b.n_seqs);
+    const int from = many_from(a.dtype);
+    const bool both = some_many(rep, a.b.n_rows, a.b.n_seqs, from);
     if (both)
-        LLMRS_TRY(kv8_many(a, MANY, ws, sms, stream));
+        LLMRS_TRY(kv8_many(a, from, ws, sms, stream));
     FewParams p{};
     p.a = a;
     LLMRS_TRY(encode_codes(&p.tk, a.c.kq, a.c, std::min(a.c.page, FT)));
     LLMRS_TRY(encode_codes(&p.tv, a.c.vq, a.c, std::min(a.c.page, FT)));
     p.head = reinterpret_cast<int4 *>(ws);
     p.part = reinterpret_cast<float *>(p.head + JOIN_SLOTS);
-    p.many = both ? MANY : INT32_MAX;
+    p.many = both ? from : INT32_MAX;
     const int nt = few_nt(mean_vectors(rep, a.b.n_rows, a.b.n_seqs), a.dtype == LLMRS_BF16 ? 8 : 4);
     const int ctas = std::min(sms, F_MAX_CTAS);
     if (a.dtype == LLMRS_F32)

@@ -16,7 +16,7 @@ namespace {
 // 2^-28, and 22 bits as two pieces down to 2^-17
 constexpr float P_SCALE = 16384.0f;
 constexpr float P_SCALE_LOG2 = 14.0f;
-constexpr int JOIN_SLOTS = 1280; // most ranges of tiles that one launch cuts
+constexpr int JOIN_SLOTS = 1920; // most ranges of tiles that one launch cuts
 constexpr int JT = 256;          // threads of the joining kernel
 
 __device__ __forceinline__ float ex2(float x)
