@@ -50,7 +50,7 @@ struct FewParams {
     CUtensorMap tk, tv; // code pools as rows of D bytes
     Kv8Attn a;
     float *part;        // [warps][2][vectors][D + 2]
-    int4 *head;         // [warps]: a pair begun but not ended: (sequence, group, KV head, pieces)
+    JoinHead *head;     // [warps]
     int many;           // sequences with more vectors per KV head than this are another kernel's
 };
 
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(few_warps(NT) * 32, 1) kv8_few_kernel(const __
     const long long lo = slot < active ? total * slot / active : 0;
     const long long hi = slot < active ? total * (slot + 1) / active : 0;
     if (lane == 0)
-        p.head[slot] = make_int4(0, 0, 0, 0);
+        p.head[slot].pieces = 0;
     if (lo == hi)
         return;
     int win_s = s_seq[warp];
@@ -597,7 +597,13 @@ __global__ void __launch_bounds__(few_warps(NT) * 32, 1) kv8_few_kernel(const __
         float *part = p.part + ((size_t)slot * 2 + which) * GV * (D + 2);
         if (from_start && !to_end && lane == 0) { // hi - 1 is tile x.tile; the range that holds the pair's last one
             const long long end = hi - 1 + (x.n_tiles() - 1 - x.tile);
-            p.head[slot] = make_int4(x.s, pair_group, pair_g, (int)(((end + 1) * active - 1) / total) - slot + 1);
+            JoinHead h{};
+            h.pieces = (int)(((end + 1) * active - 1) / total) - slot + 1;
+            h.first = pair_group * GV;
+            h.vectors = min(GV, x.n * rep - h.first);
+            h.g = pair_g;
+            h.r0 = x.r0;
+            p.head[slot] = h;
         }
 #pragma unroll
         for (int j = 0; j < NT; j++) {
@@ -700,8 +706,8 @@ int run_few(const FewParams &p, int ctas, cudaStream_t stream)
     constexpr int FW = few_warps(NT);
     LLMRS_CUDA_TRY(launch(kv8_few_kernel<T, D, SPLIT, NT>, dim3(ctas), dim3(FW * 32), FewLay<D, NT>::bytes, stream,
                           false, p));
-    LLMRS_CUDA_TRY(launch(kv8_join_kernel<T, D, GV>, dim3(2 * ctas), dim3(JT), 0, stream, true, p.a,
-                          (const float *)p.part, (const int4 *)p.head, ctas * FW, 0));
+    LLMRS_CUDA_TRY(launch(kv8_join_kernel<T, D, GV>, dim3(4 * ctas), dim3(JT), 0, stream, true, p.a,
+                          (const float *)p.part, (const JoinHead *)p.head, ctas * FW));
     return LLMRS_OK;
 }
 
@@ -772,8 +778,10 @@ bool some_many(int rep, int n_rows, int n_seqs, int from)
 size_t kv8_attention_workspace(int rep, int head_dim, int n_rows, int n_seqs)
 {
     // two pieces a warp, of the vectors of a group (16-bit rows: eight to a column tile)
-    const int gv = 8 * few_nt(mean_vectors(rep, n_rows, n_seqs), 4);
-    const size_t few = JOIN_SLOTS * (sizeof(int4) + 2 * (size_t)gv * (head_dim + 2) * sizeof(float));
+    size_t few = 0;
+    for (int nt = 1; nt <= few_nt(mean_vectors(rep, n_rows, n_seqs), 4); nt++)
+        few = std::max(few, JOIN_SLOTS * sizeof(JoinHead) + F_MAX_CTAS * 2 * (size_t)few_warps(nt) * 8 * nt *
+                                                                (head_dim + 2) * sizeof(float));
     return some_many(rep, n_rows, n_seqs, many_from(LLMRS_F32)) ? std::max(few, kv8_many_workspace(head_dim)) : few;
 }
 
@@ -800,7 +808,7 @@ int kv8_attention(const Kv8Attn &a, void *ws, int sms, cudaStream_t stream)
     p.a = a;
     LLMRS_TRY(encode_codes(&p.tk, a.c.kq, a.c, std::min(a.c.page, FT)));
     LLMRS_TRY(encode_codes(&p.tv, a.c.vq, a.c, std::min(a.c.page, FT)));
-    p.head = reinterpret_cast<int4 *>(ws);
+    p.head = reinterpret_cast<JoinHead *>(ws);
     p.part = reinterpret_cast<float *>(p.head + JOIN_SLOTS);
     p.many = both ? from : INT32_MAX;
     const int nt = few_nt(mean_vectors(rep, a.b.n_rows, a.b.n_seqs), a.dtype == LLMRS_BF16 ? 8 : 4);

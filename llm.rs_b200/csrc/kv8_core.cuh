@@ -114,85 +114,114 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
     return d;
 }
 
+// A pair that a range begins and does not end.
+struct __align__(16) JoinHead {
+    int pieces;         // 0: no such pair
+    int first, vectors; // of its rows: the first (row, query head) of the KV head, and how many
+    int g, r0;          // KV head, first row of the sequence
+    int pad[3];
+};
+
 // Join the pieces of each pair that no range had to itself.  The tiles of all
 // pairs are cut into `slots` consecutive ranges; a range that begins a pair and
-// does not end it keeps its piece in its second slot and notes the pair and its
-// number of pieces in head; the ranges behind keep theirs in their first slots.
-// A piece: the unnormalised output [GV][D], then maxima [GV] (in powers of two)
-// and sums [GV].  Every block lists the pairs; a task is one vector of one
-// pair.  A warp takes a task, or, when there are no more tasks than blocks (one
-// long sequence: a hundred pieces and more), the whole block does.
-// rows: rows of a group of vectors, 0 when the groups cut the vectors anywhere.
+// does not end it keeps its piece in its second slot and notes the pair in
+// `head`; the ranges behind keep theirs in their first slots.  A piece: the
+// unnormalised output [GV][D], then maxima [GV] (in powers of two) and sums
+// [GV].  Every block lists the pairs; a task is one vector of one pair.  A warp
+// takes a task, or, when there are no more tasks than blocks (one long
+// sequence: a hundred pieces and more), the whole block does.  The kernel is a
+// chain of a few loads that depend on one another, so each step has all its
+// loads in flight at once.
 template <class T, int D, int GV>
-__global__ void __launch_bounds__(JT) kv8_join_kernel(Kv8Attn a, const float *part, const int4 *head, int slots, int rows)
+__global__ void __launch_bounds__(JT) kv8_join_kernel(Kv8Attn a, const float *part, const JoinHead *head, int slots)
 {
-    constexpr int W = JT / 32, DL = D / 32;
+    constexpr int W = JT / 32, DL = D / 32, PER = (JOIN_SLOTS + JT - 1) / JT;
+    constexpr int BATCH = 8; // pieces in flight
     __shared__ int s_owner[JOIN_SLOTS];
     __shared__ int s_n[W];
     __shared__ float s_m[W], s_l[W], s_o[W][D];
     griddep_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rep = a.n_heads / a.c.n_kv;
     const size_t stride = (size_t)GV * (D + 2);
-    int count = 0;
-    for (int w0 = 0; w0 < slots; w0 += JT) {
-        const int w = w0 + threadIdx.x;
-        const bool open = w < slots && head[w].w > 0;
-        const unsigned b = __ballot_sync(0xffffffffu, open);
-        __syncthreads();
-        if (lane == 0)
-            s_n[warp] = __popc(b);
-        __syncthreads();
-        int at = count;
+    int pieces[PER], mine = 0;
 #pragma unroll
-        for (int i = 0; i < W; i++) {
-            at += i < warp ? s_n[i] : 0;
-            count += s_n[i];
-        }
-        if (open)
-            s_owner[at + __popc(b & ((1u << lane) - 1))] = w;
+    for (int i = 0; i < PER; i++)
+        pieces[i] = i * JT + (int)threadIdx.x < slots ? head[i * JT + threadIdx.x].pieces : 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+        mine += pieces[i] > 0;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        upto += lane >= o ? y : 0;
     }
+    if (lane == 31)
+        s_n[warp] = upto;
+    __syncthreads();
+    int count = 0, at = upto - mine;
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+        at += i < warp ? s_n[i] : 0;
+        count += s_n[i];
+    }
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+        if (pieces[i] > 0)
+            s_owner[at++] = i * JT + threadIdx.x;
     __syncthreads();
     const bool wide = count * GV <= (int)gridDim.x;
     const int step = wide ? gridDim.x : gridDim.x * W;
     for (int task = wide ? blockIdx.x : blockIdx.x * W + warp; task < count * GV; task += step) {
         const int w = s_owner[task / GV], vi = task % GV;
-        const int4 h = head[w];
-        int r0, n, len;
-        kv8_seq(a.b, h.x, a.err, r0, n, len);
-        const int v = (rows ? h.y * rows * rep : h.y * GV) + vi;
-        if (v >= n * rep || (rows && vi >= rows * rep))
+        const JoinHead h = head[w];
+        if (vi >= h.vectors)
             continue; // the same for all of the task's warps
         auto piece = [&](int i) { return part + ((size_t)2 * (w + i) + (i ? 0 : 1)) * stride; };
-        float m = -INFINITY, l = 0.0f, o[DL];
+        const int p0 = wide ? h.pieces * warp / W : 0, p1 = wide ? h.pieces * (warp + 1) / W : h.pieces;
+        float m = -INFINITY, l = 0.0f, o[DL], x[BATCH][DL]; // lane i has dims DL * i ..
 #pragma unroll
         for (int k = 0; k < DL; k++)
             o[k] = 0.0f;
-        const int p0 = wide ? h.w * warp / W : 0, p1 = wide ? h.w * (warp + 1) / W : h.w;
         for (int i0 = p0; i0 < p1; i0 += 32) {
             const int here = min(32, p1 - i0);
             const float mi = lane < here ? piece(i0 + lane)[(size_t)GV * D + vi] : -INFINITY;
             const float li = lane < here ? piece(i0 + lane)[(size_t)GV * (D + 1) + vi] : 0.0f;
+            auto fetch = [&](int b) {
+#pragma unroll
+                for (int i = 0; i < BATCH; i++) {
+                    const float *src = piece(i0 + min(b + i, here - 1)) + (size_t)vi * D + lane * DL;
+                    if constexpr (DL == 4) {
+                        const float4 y = *reinterpret_cast<const float4 *>(src);
+                        x[i][0] = y.x, x[i][1] = y.y, x[i][2] = y.z, x[i][3] = y.w;
+                    } else {
+                        const float2 y = *reinterpret_cast<const float2 *>(src);
+                        x[i][0] = y.x, x[i][1] = y.y;
+                    }
+                }
+            };
+            fetch(0);
             const float mn = fmaxf(m, warp_max(mi)), ref = mn == -INFINITY ? 0.0f : mn;
-            const float c = ex2(m - ref), e = ex2(mi - ref);
+            const float c = ex2(m - ref), e = ex2(mi - ref); // 0 for the lanes behind the last piece
             l = l * c + warp_sum(li * e);
             m = mn;
 #pragma unroll
             for (int k = 0; k < DL; k++)
                 o[k] *= c;
-#pragma unroll 8
-            for (int i = 0; i < here; i++) {
-                const float ei = __shfl_sync(0xffffffffu, e, i);
-                const float *src = piece(i0 + i) + (size_t)vi * D + lane * DL;
-                if constexpr (DL == 4) {
-                    const float4 x = *reinterpret_cast<const float4 *>(src);
-                    o[0] += ei * x.x, o[1] += ei * x.y, o[2] += ei * x.z, o[3] += ei * x.w;
-                } else {
-                    const float2 x = *reinterpret_cast<const float2 *>(src);
-                    o[0] += ei * x.x, o[1] += ei * x.y;
+            for (int b = 0; b < here; b += BATCH) {
+                if (b)
+                    fetch(b);
+#pragma unroll
+                for (int i = 0; i < BATCH; i++) {
+                    const float ei = __shfl_sync(0xffffffffu, e, (b + i) & 31);
+#pragma unroll
+                    for (int k = 0; k < DL; k++)
+                        o[k] += ei * x[i][k];
                 }
             }
         }
-        T *out = reinterpret_cast<T *>(a.out) + (size_t)(r0 + v / rep) * a.ld_out + (size_t)(h.z * rep + v % rep) * D;
+        const int v = h.first + vi;
+        T *out = reinterpret_cast<T *>(a.out) + (size_t)(h.r0 + v / rep) * a.ld_out + (size_t)(h.g * rep + v % rep) * D;
         if (!wide) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll

@@ -52,7 +52,7 @@ static_assert(sizeof(ManyTile) == 160, "16-byte words");
 struct ManyParams {
     Kv8Attn a;
     float *part;
-    int4 *head;
+    JoinHead *head;
     int many; // sequences with at most this many vectors per KV head are another kernel's
 };
 
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
     const long long lo = slot < active ? total * slot / active : 0;
     const long long hi = slot < active ? total * (slot + 1) / active : 0;
     if (threadIdx.x == 0)
-        p.head[slot] = make_int4(0, 0, 0, 0);
+        p.head[slot].pieces = 0;
     if (lo == hi)
         return;
     long long base = 0;
@@ -533,8 +533,15 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
             if (x.last) {
                 const int row = x.mt * R + r / rep, head = x.g * rep + r % rep;
                 const bool done = x.from_start && x.to_end, live = r < R * rep && row < x.n;
-                if (!done && x.from_start && r == 0)
-                    p.head[slot] = make_int4(x.s, x.mt, x.g, x.pieces);
+                if (!done && x.from_start && r == 0) {
+                    JoinHead h{};
+                    h.pieces = x.pieces;
+                    h.first = x.mt * R * rep;
+                    h.vectors = min(R, x.n - x.mt * R) * rep;
+                    h.g = x.g;
+                    h.r0 = x.r0;
+                    p.head[slot] = h;
+                }
                 if (live) {
                     const float inv = !done ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
                     T *out = reinterpret_cast<T *>(a.out) + (size_t)(x.r0 + row) * a.ld_out + (size_t)head * D;
@@ -838,11 +845,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
 template <class T, int D, int QP, int PP>
 int run(const ManyParams &p, int ctas, cudaStream_t stream)
 {
-    const int rep = p.a.n_heads / p.a.c.n_kv;
     LLMRS_CUDA_TRY(launch(kv8_many_kernel<T, D, QP, PP>, dim3(ctas), dim3(MANY_THREADS), ManyLay<D, QP>::bytes, stream,
                           false, p));
-    LLMRS_CUDA_TRY(launch(kv8_join_kernel<T, D, MB>, dim3(2 * ctas), dim3(JT), 0, stream, true, p.a,
-                          (const float *)p.part, (const int4 *)p.head, ctas, MB / rep));
+    LLMRS_CUDA_TRY(launch(kv8_join_kernel<T, D, MB>, dim3(8 * ctas), dim3(JT), 0, stream, true, p.a,
+                          (const float *)p.part, (const JoinHead *)p.head, ctas));
     return LLMRS_OK;
 }
 
@@ -857,7 +863,7 @@ cudaError_t prepare()
 
 size_t kv8_many_workspace(int head_dim)
 {
-    return (size_t)MANY_CTAS * (sizeof(int4) + 2 * (size_t)MB * (head_dim + 2) * sizeof(float));
+    return (size_t)MANY_CTAS * (sizeof(JoinHead) + 2 * (size_t)MB * (head_dim + 2) * sizeof(float));
 }
 
 int kv8_many_prepare(void)
@@ -882,7 +888,7 @@ int kv8_many(const Kv8Attn &a, int many, void *ws, int sms, cudaStream_t stream)
 {
     ManyParams p{};
     p.a = a;
-    p.head = reinterpret_cast<int4 *>(ws);
+    p.head = reinterpret_cast<JoinHead *>(ws);
     p.part = reinterpret_cast<float *>(p.head + MANY_CTAS);
     p.many = many;
     const int ctas = sms < MANY_CTAS ? sms : MANY_CTAS;
