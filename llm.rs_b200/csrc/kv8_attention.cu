@@ -95,6 +95,15 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// the same from nothing
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
 {
     uint32_t y;
@@ -430,11 +439,6 @@ __global__ void __launch_bounds__(few_warps(NT) * 32, 1) kv8_few_kernel(const __
         float s[2][NT][4];
 #pragma unroll
         for (int mt = 0; mt < 2; mt++) {
-#pragma unroll
-            for (int j = 0; j < NT; j++)
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-                    s[mt][j][c] = 0.0f;
             // the lane's LD codes of tokens gl and gl + 8, in 16-byte units
 #pragma unroll
             for (int u = 0; u < LD / 16; u++) {
@@ -453,8 +457,12 @@ __global__ void __launch_bounds__(few_warps(NT) * 32, 1) kv8_few_kernel(const __
                     const uint32_t a0 = codes_f16(x0, 0x4140), a2 = codes_f16(x0, 0x4342);
                     const uint32_t a1 = codes_f16(x1, 0x4140), a3 = codes_f16(x1, 0x4342);
 #pragma unroll
-                    for (int j = 0; j < NT; j++)
-                        mma16816(s[mt][j], a0, a1, a2, a3, qf[j][4 * u + k][0], qf[j][4 * u + k][1]);
+                    for (int j = 0; j < NT; j++) {
+                        if (u == 0 && k == 0)
+                            mma16816_first(s[mt][j], a0, a1, a2, a3, qf[j][0][0], qf[j][0][1]);
+                        else
+                            mma16816(s[mt][j], a0, a1, a2, a3, qf[j][4 * u + k][0], qf[j][4 * u + k][1]);
+                    }
                 }
             }
         }
@@ -541,16 +549,31 @@ __global__ void __launch_bounds__(few_warps(NT) * 32, 1) kv8_few_kernel(const __
                 }
             }
         refill(1, v_issued);
+        // a new maximum scales what the sums hold (most tiles bring none to any column)
+        bool moved = false;
 #pragma unroll
-        for (int k = 0; k < W; k++) {
-            float f[2][NT][4];
+        for (int j = 0; j < NT; j++)
+            moved = moved || corr[j][0] != 1.0f || corr[j][1] != 1.0f;
+        if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int i = 0; i < MT; i++)
 #pragma unroll
                 for (int j = 0; j < NT; j++)
 #pragma unroll
                     for (int c = 0; c < 4; c++)
-                        f[i][j][c] = 0.0f;
+                        acc[i][j][c] *= corr[j][c & 1];
+        }
+        auto add = [&](float (&o)[4], const float (&f)[4], float by) { // o += f * by
+#pragma unroll
+            for (int c = 0; c < 4; c += 2) {
+                const float2 y = fma2(make_float2(f[c], f[c + 1]), make_float2(by, by), make_float2(o[c], o[c + 1]));
+                o[c] = y.x;
+                o[c + 1] = y.y;
+            }
+        };
+#pragma unroll
+        for (int k = 0; k < W; k++) {
+            float f[2][NT][4];
 #pragma unroll
             for (int mt = 0; mt < 2; mt++) {
                 // bytes (token, dim) -> per dim the token pairs (0, 1) and (2, 3)
@@ -564,29 +587,31 @@ __global__ void __launch_bounds__(few_warps(NT) * 32, 1) kv8_few_kernel(const __
                 const uint32_t b2 = codes_f16(y23, 0x4140), b3 = codes_f16(y23, 0x4342);
 #pragma unroll
                 for (int j = 0; j < NT; j++) {
-                    mma16816(f[0][j], a0, a1, a2, a3, pf[mt][j][0], pf[mt][j][1]);
-                    mma16816(f[1][j], b0, b1, b2, b3, pf[mt][j][0], pf[mt][j][1]);
+                    if (mt == 0) {
+                        mma16816_first(f[0][j], a0, a1, a2, a3, pf[0][j][0], pf[0][j][1]);
+                        mma16816_first(f[1][j], b0, b1, b2, b3, pf[0][j][0], pf[0][j][1]);
+                    } else {
+                        mma16816(f[0][j], a0, a1, a2, a3, pf[1][j][0], pf[1][j][1]);
+                        mma16816(f[1][j], b0, b1, b2, b3, pf[1][j][0], pf[1][j][1]);
+                    }
                 }
                 if (half && mt == 0) { // pages of 16: the two halves have scales of their own
 #pragma unroll
                     for (int i = 0; i < 2; i++)
 #pragma unroll
-                        for (int j = 0; j < NT; j++)
+                        for (int j = 0; j < NT; j++) {
+                            add(acc[2 * k + i][j], f[i][j], vs0);
 #pragma unroll
-                            for (int c = 0; c < 4; c++) {
-                                acc[2 * k + i][j][c] = acc[2 * k + i][j][c] * corr[j][c & 1] + f[i][j][c] * vs0;
+                            for (int c = 0; c < 4; c++)
                                 f[i][j][c] = 0.0f;
-                            }
+                        }
                 }
             }
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int j = 0; j < NT; j++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        acc[2 * k + i][j][c] = (half ? acc[2 * k + i][j][c] : acc[2 * k + i][j][c] * corr[j][c & 1]) +
-                                               f[i][j][c] * vs1;
+                    add(acc[2 * k + i][j], f[i][j], vs1);
         }
     };
 
