@@ -48,7 +48,7 @@ struct Kv8Attn {
     float scale;            // of q.k before the softmax
     uint32_t *err;
 };
-size_t kv8_attention_workspace(int rep, int head_dim, int n_rows, int n_seqs); // rep: query heads of a KV head
+size_t kv8_attention_workspace(int n_heads, int n_kv, int head_dim, int n_rows, int n_seqs);
 int kv8_attention(const Kv8Attn &a, void *ws, int sms, cudaStream_t stream);
 // set kernel attributes on the current device (once per context, outside capture)
 int kv8_prepare(void);

@@ -800,14 +800,15 @@ bool some_many(int rep, int n_rows, int n_seqs, int from)
 
 } // namespace
 
-size_t kv8_attention_workspace(int rep, int head_dim, int n_rows, int n_seqs)
+size_t kv8_attention_workspace(int n_heads, int n_kv, int head_dim, int n_rows, int n_seqs)
 {
+    const int rep = n_heads / n_kv;
     // two pieces a warp, of the vectors of a group (16-bit rows: eight to a column tile)
     size_t few = 0;
     for (int nt = 1; nt <= few_nt(mean_vectors(rep, n_rows, n_seqs), 4); nt++)
         few = std::max(few, JOIN_SLOTS * sizeof(JoinHead) + F_MAX_CTAS * 2 * (size_t)few_warps(nt) * 8 * nt *
                                                                 (head_dim + 2) * sizeof(float));
-    return some_many(rep, n_rows, n_seqs, many_from(LLMRS_F32)) ? std::max(few, kv8_many_workspace(head_dim)) : few;
+    return some_many(rep, n_rows, n_seqs, many_from(LLMRS_F32)) ? std::max(few, kv8_many_workspace(head_dim, n_heads, n_rows)) : few;
 }
 
 int kv8_prepare(void)

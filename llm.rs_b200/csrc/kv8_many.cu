@@ -10,16 +10,23 @@
 // the maximum and the value scales applied there: long sums do not pass
 // through the tensor core's accumulator.
 //
-// Warpgroups: 0 softmax (thread = row), 1 output (thread = row, D accumulators),
-// 2 codes to f16 in shared memory (keys K-major, values MN-major, both 128-byte
-// swizzled: the same image), 3: one warp issues the products, one looks up pages
-// and scales ahead, 4 rotates, scales and splits the next rows' Q.
+// Warpgroups: 0 and 4 softmax of every other tile (thread = row), 1 output
+// (thread = row, D accumulators), 2 and 5 key and value codes to f16 in shared
+// memory (keys K-major, values MN-major, both 128-byte swizzled: the same image),
+// 3: one warp issues the products, one looks up pages and scales ahead, one
+// fetches Q, which a kernel of its own has rotated, scaled and split.
+// The softmax keeps no state: it hands over a tile's maximum, sum and scale, and
+// the output warps, which go through the tiles in order, know the running ones.
 // S and O are double buffered (4 x 128 columns: all of TMEM), P lies over the S
 // it came from, Q is double buffered, K and V too where Q is one piece, so the
-// product of tile i + 1 runs while tile i is in the softmax.  The softmax reads
-// S from TMEM twice, 32 columns at a time in a rolled loop: unrolled over 128
-// registers (with Q's preparation in line) a third of all stalls were
-// instruction fetches.
+// product of tile i + 1 runs while tile i is in the softmax.
+//
+// What a tile costs is not a product's 1000 cycles but the longest of the roles'
+// chains, whose instructions take 4 to 5 cycles each: so each role that was the
+// longest got a second warpgroup or a kernel of its own, and each keeps its next
+// loads (TMEM columns, codes) in flight while it works.  Two prompts of 4000 rows,
+// bf16, 32 heads of 128 over 8: 740 us with one softmax, one widening and one Q
+// warpgroup.
 //
 // Work: the tiles of all (sequence, KV head, tile of rows) in one row, cut into
 // equal consecutive ranges, one per CTA; pieces of a softmax that a range cuts
@@ -33,9 +40,10 @@ namespace llmrs {
 namespace {
 
 constexpr int MB = 128;          // vectors, and tokens, of a tile
-constexpr int MANY_THREADS = 640;
+constexpr int MANY_THREADS = 768;
 constexpr int INFO = 8;          // tile descriptions in flight
 constexpr int RING = 4;          // softmax -> output hand-overs in flight
+constexpr int QT = 256;          // threads of the kernel that prepares Q
 
 struct ManyTile {
     int row[8];                  // pool rows of the tile's 16-token groups; -1: not there
@@ -45,12 +53,16 @@ struct ManyTile {
     int tile, s, g, mt;          // which
     int r0, n, len;              // of the sequence
     int from_start, to_end, pieces;
-    int pad[3];
+    int item;                    // number of the pair within this range
+    int pad[2];
 };
 static_assert(sizeof(ManyTile) == 160, "16-byte words");
 
 struct ManyParams {
+    CUtensorMap tq;   // prepared Q: [piece][row][head][D] f16, boxes of 64 dims of a tile's vectors
     Kv8Attn a;
+    __half *q16;      // the same memory
+    float *facs;      // [row][head] what the scores are multiplied by
     float *part;
     JoinHead *head;
     int many; // sequences with at most this many vectors per KV head are another kernel's
@@ -64,8 +76,7 @@ struct ManyLay {
     static constexpr int v_off = k_off + KVS * T;
     static constexpr int info_off = v_off + KVS * T;
     static constexpr int ring_off = info_off + INFO * (int)sizeof(ManyTile);
-    static constexpr int fac_off = ring_off + RING * 4 * MB * 4; // [2][MB] score factors of the rows
-    static constexpr int bar_off = fac_off + 2 * MB * 4;
+    static constexpr int bar_off = ring_off + RING * 3 * MB * 4;
     static constexpr int bytes = bar_off + 512 + 1024; // + alignment slack
     static_assert(bytes <= 232448 - 256, "shared memory of one CTA");
 };
@@ -100,12 +111,10 @@ __device__ __forceinline__ void tc_commit(uint64_t *bar)
 
 // Operand tile in 128-byte-swizzled atoms of 8 rows x 128 bytes, 1024 bytes
 // apart.  K-major: rows are M or N, 64 K values each (lead unused).  MN-major:
-// rows are K, 64 M or N values each, `lead` bytes to the next 64.
-__device__ __forceinline__ uint64_t sw128(uint32_t saddr, uint32_t lead)
-{
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
-           ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
-}
+// rows are K, 64 M or N values each, `lead` bytes to the next 64.  The low word
+// of its descriptor, whose unit is 16 bytes; the high word is always the same.
+__device__ __forceinline__ uint32_t sw128(uint32_t saddr, uint32_t lead) { return (saddr >> 4) | (lead >> 4) << 16; }
+constexpr uint32_t SW128_HI = (1024u >> 4) | 1u << (46 - 32) | 2u << (61 - 32);
 
 // kind::f16: f16 x f16 -> f32, M = 128; B K-major or MN-major
 __host__ __device__ constexpr uint32_t idesc_f16(int n, bool b_mn)
@@ -113,22 +122,40 @@ __host__ __device__ constexpr uint32_t idesc_f16(int n, bool b_mn)
     return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(MB >> 4) << 24);
 }
 
-// Whole warp, one elected lane issues: operands stay in uniform registers (under
-// a divergent branch every product paid for moving its descriptors there, 200
-// cycles each)
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, bool acc)
+// Four steps of 16 along K, 32 bytes apart in both operands.  Whole warp, one
+// elected lane issues, and the descriptors are sums of low words in one block:
+// in a divergent branch, or with a descriptor built per step, a step took 140
+// to 200 cycles to issue, and 64 to run.
+__device__ __forceinline__ void mma_ss4(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, bool acc)
 {
-    asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-                 "l"(ad), "l"(bd), "r"(idesc), "r"((int)acc)
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b32 x, y;\n\t.reg .b64 da, db;\n\t"
+                 "elect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+                 "mov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t"
+                 "add.u32 x, %1, 2;\n\tadd.u32 y, %2, 2;\n\tmov.b64 da, {x, %3};\n\tmov.b64 db, {y, %3};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, 1;\n\t"
+                 "add.u32 x, %1, 4;\n\tadd.u32 y, %2, 4;\n\tmov.b64 da, {x, %3};\n\tmov.b64 db, {y, %3};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, 1;\n\t"
+                 "add.u32 x, %1, 6;\n\tadd.u32 y, %2, 6;\n\tmov.b64 da, {x, %3};\n\tmov.b64 db, {y, %3};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, 1;\n\t}" ::"r"(d),
+                 "r"(a_lo), "r"(b_lo), "n"(SW128_HI), "r"(idesc), "r"((int)acc)
                  : "memory");
 }
 
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t at, uint64_t bd, uint32_t idesc, bool acc)
+// the same with A in TMEM, 16 columns a step, and B MN-major, 16 rows of 128 bytes a step
+__device__ __forceinline__ void mma_ts4(uint32_t d, uint32_t at, uint32_t b_lo, uint32_t idesc, bool acc)
 {
-    asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-                 "r"(at), "l"(bd), "r"(idesc), "r"((int)acc)
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b32 x, y;\n\t.reg .b64 db;\n\t"
+                 "elect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+                 "mov.b64 db, {%2, %3};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t"
+                 "add.u32 x, %1, 16;\n\tadd.u32 y, %2, 128;\n\tmov.b64 db, {y, %3};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, %4, 1;\n\t"
+                 "add.u32 x, %1, 32;\n\tadd.u32 y, %2, 256;\n\tmov.b64 db, {y, %3};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, %4, 1;\n\t"
+                 "add.u32 x, %1, 48;\n\tadd.u32 y, %2, 384;\n\tmov.b64 db, {y, %3};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, %4, 1;\n\t}" ::"r"(d),
+                 "r"(at), "r"(b_lo), "n"(SW128_HI), "r"(idesc), "r"((int)acc)
                  : "memory");
 }
 
@@ -171,11 +198,9 @@ __device__ __forceinline__ void tm_wait(uint32_t (&r)[16])
 {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : T8(r, 0), T8(r, 8) : : "memory");
 }
-__device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t (&r)[16])
+__device__ __forceinline__ void tm_st8(uint32_t addr, const uint32_t (&r)[8])
 {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
-                 "%13, %14, %15};" ::I8(r, 0),
-                 I8(r, 8), "r"(addr)
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::I8(r, 0), "r"(addr)
                  : "memory");
 }
 #undef R8
@@ -255,7 +280,6 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
     uint8_t *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     ManyTile *info = reinterpret_cast<ManyTile *>(smem + Lay::info_off);
     float *ring = reinterpret_cast<float *>(smem + Lay::ring_off); // [RING][change of max | scale of O | sum | max][MB]
-    float *facs = reinterpret_cast<float *>(smem + Lay::fac_off);
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + Lay::bar_off);
     __shared__ uint32_t s_tmem;
     __shared__ long long s_sum[MANY_THREADS / 32];
@@ -269,7 +293,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
     if (threadIdx.x == 0) {
         for (int i = 0; i < INFO; i++) {
             mbar_init(&bar[B_INFO_FULL + i], 1);
-            mbar_init(&bar[B_INFO_EMPTY + i], 13); // 12 warps and the issuing thread
+            mbar_init(&bar[B_INFO_EMPTY + i], 17); // 16 warps and the issuing thread
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&bar[B_K_FULL + i], 128);
@@ -280,8 +304,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
             mbar_init(&bar[B_P_FULL + i], 128);
             mbar_init(&bar[B_O_FULL + i], 1);
             mbar_init(&bar[B_O_EMPTY + i], 128);
-            mbar_init(&bar[B_Q_FULL + i], 128);
-            mbar_init(&bar[B_Q_EMPTY + i], 5); // the products and the softmax warps
+            mbar_init(&bar[B_Q_FULL + i], 1);
+            mbar_init(&bar[B_Q_EMPTY + i], 1);
         }
         fence_mbar_init();
         s_seq = 0;
@@ -350,43 +374,34 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
     tc_after();
     const uint32_t tmem = s_tmem;
     const int mine = (int)(hi - lo);
+    griddep_wait(); // Q is ready
     auto wait = [&](int b, int use) { // whole warp
         return __all_sync(0xffffffffu, kv8_wait(&bar[b], (uint32_t)(use & 1), a.err));
     };
     bool ok = true;
 
-    if (wg == 0) {
-        // ================================================= softmax: thread = row
-        regs_up<104>();
-        const int r = threadIdx.x;
-        const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-        float m = -INFINITY, l = 0.0f, fac = 0.0f;
-        int lim = -1, item = 0;
+    if (wg == 0 || wg == 4) {
+        // ================================================= softmax of every other tile: thread = row
+        static_assert(2 * 80 + 160 + 2 * 56 + 48 == 6 * 80, "the launch's registers, shared out");
+        const int r = threadIdx.x & 127, odd = wg >> 2;
+        const uint32_t sp = tmem + (uint32_t)odd * MB + ((uint32_t)((warp & 3) * 32) << 16);
+        float fac = 0.0f;
+        int lim = -1, item = -1;
         bool busy = false; // some row of this warp is there
-        for (int i = 0; i < mine && ok; i++) {
+        for (int i = odd; i < mine && ok; i += 2) {
             const ManyTile &x = info[i % INFO];
-            if (!(ok = wait(B_INFO_FULL + i % INFO, i / INFO)))
+            if (!(ok = wait(B_INFO_FULL + i % INFO, i / INFO) && wait(B_S_FULL + odd, i >> 1)))
                 break;
-            if (x.first) {
+            tc_after();
+            if (x.item != item) {
+                item = x.item;
                 const int row = x.mt * R + r / rep;
                 const bool live = r < R * rep && row < x.n;
                 lim = live ? x.len + row : -1;
                 busy = __any_sync(0xffffffffu, live);
-                m = -INFINITY;
-                l = 0.0f;
-                if (!(ok = wait(B_Q_FULL + (item & 1), item >> 1)))
-                    break;
-                fac = facs[(item & 1) * MB + r];
-                __syncwarp();
-                if (lane == 0)
-                    mbar_arrive(&bar[B_Q_EMPTY + (item & 1)]);
-                item++;
+                fac = live ? p.facs[(size_t)(x.r0 + row) * a.n_heads + x.g * rep + r % rep] : 0.0f;
             }
-            if (!(ok = wait(B_S_FULL + (i & 1), i >> 1)))
-                break;
-            tc_after();
-            const uint32_t sp = lanes + (uint32_t)(i & 1) * MB;
-            float corr = 1.0f, oscale = 0.0f;
+            float top = -INFINITY, ref2 = -INFINITY, sum = 0.0f;
             if (busy) {
                 const bool masked = x.masked;
                 if (masked) { // S becomes the scores themselves, the unseen ones at -inf
@@ -408,86 +423,87 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                     }
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
-                // 32 scores of the row as two groups of 16, and what they are multiplied by
-                auto scores = [&](int k, uint32_t(&s)[32], float(&kf)[2]) {
-                    tm_ld32(sp + 32 * k, s);
-                    kf[0] = masked ? 1.0f : fac * x.ks[2 * k];
-                    kf[1] = masked ? 1.0f : fac * x.ks[2 * k + 1];
-                    tm_wait(s);
+                const float f = masked ? 1.0f : fac;
+                // the row's largest score, and largest score with its value scale
+                auto most = [&](int g, const uint32_t *s) { // 16 scores of group g
+                    float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        t0 = fmaxf(fmaxf(t0, __uint_as_float(s[j])), __uint_as_float(s[j + 1]));
+                        t1 = fmaxf(fmaxf(t1, __uint_as_float(s[j + 2])), __uint_as_float(s[j + 3]));
+                    }
+                    t0 = fmaxf(t0, t1) * (masked ? 1.0f : f * x.ks[g]); // the factor is not negative
+                    top = fmaxf(top, t0);
+                    ref2 = fmaxf(ref2, t0 + x.lvs[g]);
                 };
-                float top = -INFINITY, ref2 = -INFINITY;
+                { // the next columns are on their way meanwhile
+                    uint32_t s0[16], s1[16];
+                    tm_ld16(sp, s0);
+                    tm_wait(s0);
 #pragma unroll 1
-                for (int k = 0; k < 4; k++) {
-                    uint32_t s[32];
-                    float kf[2];
-                    scores(k, s, kf);
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-                        for (int j = 0; j < 16; j += 4) {
-                            t0 = fmaxf(fmaxf(t0, __uint_as_float(s[16 * h + j])), __uint_as_float(s[16 * h + j + 1]));
-                            t1 = fmaxf(fmaxf(t1, __uint_as_float(s[16 * h + j + 2])), __uint_as_float(s[16 * h + j + 3]));
-                        }
-                        t0 = fmaxf(t0, t1) * kf[h]; // kf >= 0
-                        top = fmaxf(top, t0);
-                        ref2 = fmaxf(ref2, t0 + x.lvs[2 * k + h]);
+                    for (int g = 0; g < 8; g += 2) {
+                        tm_ld16(sp + 16 * g + 16, s1);
+                        most(g, s0);
+                        tm_wait(s1);
+                        tm_ld16(sp + min(16 * g + 32, 112), s0); // the last one is not used
+                        most(g + 1, s1);
+                        tm_wait(s0);
                     }
                 }
-                const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.0f : mn;
-                corr = ex2(m - ref);
-                m = mn;
                 // P = p * vs against the row's own largest p * vs of the tile: f16 keeps its bits
                 // whatever the scales of pages that the row hardly sees
+                const float ref = top == -INFINITY ? 0.0f : top;
                 const bool none = ref2 == -INFINITY; // no seen page has a scale above 0
                 ref2 = none ? 0.0f : ref2 - P_SCALE_LOG2;
-                oscale = none ? 0.0f : ex2(ref2 - ref);
-                float sum = 0.0f;
-#pragma unroll 1
-                for (int k = 0; k < 4; k++) {
-                    uint32_t s[32], ph[16], pl[16];
-                    float kf[2];
-                    scores(k, s, kf);
+                auto probabilities = [&](int g, const uint32_t *s) { // 16 of them, over the scores of group g
+                    const float lvs = x.lvs[g], kf = masked ? 1.0f : f * x.ks[g];
+                    // a scale of zero: f16 holds the probabilities as zero, the sum keeps them
+                    const bool zero = lvs == -INFINITY;
+                    const float add = zero ? -60.0f - ref : lvs - ref2;
+                    const float back = zero ? 0x1p60f : ex2(fminf(ref2 - lvs - ref, 120.0f));
+                    float2 g01 = make_float2(0.0f, 0.0f);
+                    uint32_t ph[8], pl[8];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const float lvs = x.lvs[2 * k + h];
-                        // a scale of zero: f16 holds the probabilities as zero, the sum keeps them
-                        const bool zero = lvs == -INFINITY;
-                        const float add = zero ? -60.0f - ref : lvs - ref2;
-                        const float back = zero ? 0x1p60f : ex2(fminf(ref2 - lvs - ref, 120.0f));
-                        float2 g01 = make_float2(0.0f, 0.0f);
-#pragma unroll
-                        for (int j = 0; j < 16; j += 2) {
-                            const float2 y = fma2(make_float2(__uint_as_float(s[16 * h + j]), __uint_as_float(s[16 * h + j + 1])),
-                                                  make_float2(kf[h], kf[h]), make_float2(add, add));
-                            const float e0 = ex2(y.x), e1 = ex2(y.y);
-                            g01 = add2(g01, make_float2(e0, e1));
-                            const uint32_t w = pack16(e0, e1);
-                            ph[8 * h + j / 2] = w;
-                            if constexpr (PP == 2) {
-                                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-                                pl[8 * h + j / 2] = pack16(e0 - f.x, e1 - f.y);
-                            }
+                    for (int j = 0; j < 16; j += 2) {
+                        const float2 y = fma2(make_float2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])),
+                                              make_float2(kf, kf), make_float2(add, add));
+                        const float e0 = ex2(y.x), e1 = ex2(y.y);
+                        g01 = add2(g01, make_float2(e0, e1));
+                        const uint32_t w = pack16(e0, e1);
+                        ph[j / 2] = w;
+                        if constexpr (PP == 2) {
+                            const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+                            pl[j / 2] = pack16(e0 - h.x, e1 - h.y);
                         }
-                        sum += (g01.x + g01.y) * back;
                     }
-                    // over the 32 columns just read: 16 of the first piece, 16 of the second
-                    tm_st16(sp + 32 * k, ph);
+                    sum += (g01.x + g01.y) * back;
+                    tm_st8(sp + 16 * g, ph);
                     if constexpr (PP == 2)
-                        tm_st16(sp + 32 * k + 16, pl);
+                        tm_st8(sp + 16 * g + 8, pl);
+                };
+                {
+                    uint32_t s0[16], s1[16];
+                    tm_ld16(sp, s0);
+                    tm_wait(s0);
+#pragma unroll 1
+                    for (int g = 0; g < 8; g += 2) {
+                        tm_ld16(sp + 16 * g + 16, s1);
+                        probabilities(g, s0);
+                        tm_wait(s1);
+                        tm_ld16(sp + min(16 * g + 32, 112), s0); // the last one is not used
+                        probabilities(g + 1, s1);
+                        tm_wait(s0);
+                    }
                 }
-                l = l * corr + sum;
+                ref2 = none ? -INFINITY : ref2;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             }
-            float *hand = ring + (i % RING) * 4 * MB;
-            hand[r] = corr;
-            hand[MB + r] = oscale;
-            if (x.last) {
-                hand[2 * MB + r] = l;
-                hand[3 * MB + r] = m;
-            }
+            float *hand = ring + (i % RING) * 3 * MB;
+            hand[r] = top;
+            hand[MB + r] = ref2;
+            hand[2 * MB + r] = sum;
             tc_before();
-            mbar_arrive(&bar[B_P_FULL + (i & 1)]);
+            mbar_arrive(&bar[B_P_FULL + odd]);
             __syncwarp();
             if (lane == 0)
                 mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
@@ -498,18 +514,22 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
         const int r = threadIdx.x - 128;
         const uint32_t lanes = tmem + 2 * MB + ((uint32_t)((warp & 3) * 32) << 16);
         float2 acc[D / 2];
+        float m = -INFINITY, l = 0.0f; // the softmax's running maximum and sum
         for (int i = 0; i < mine && ok; i++) {
             const ManyTile &x = info[i % INFO];
             if (!(ok = wait(B_INFO_FULL + i % INFO, i / INFO) && wait(B_O_FULL + (i & 1), i >> 1)))
                 break;
             tc_after();
-            const float *hand = ring + (i % RING) * 4 * MB;
-            const float corr = x.first ? 0.0f : hand[r], oscale = hand[MB + r];
-            float l = 0.0f, m = 0.0f;
-            if (x.last) {
-                l = hand[2 * MB + r];
-                m = hand[3 * MB + r];
+            const float *hand = ring + (i % RING) * 3 * MB;
+            const float top = hand[r], ref2 = hand[MB + r], sum = hand[2 * MB + r];
+            if (x.first) {
+                m = -INFINITY;
+                l = 0.0f;
             }
+            const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.0f : mn;
+            const float corr = ex2(m - ref), oscale = ex2(ref2 - ref); // 0 from -inf
+            l = l * corr + sum * ex2(top - ref);
+            m = mn;
             if (x.first) {
 #pragma unroll
                 for (int d = 0; d < D / 2; d++)
@@ -569,65 +589,61 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
             if (lane == 0)
                 mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
         }
-    } else if (wg == 2) {
-        // ================================================= codes to f16
+    } else if (wg == 2 || wg == 5) {
+        // ================================================= codes to f16: keys, values
+        regs_down<56>();
         // Eight lanes take eight 16-code units: for D = 128 half the units of two tokens,
         // crosswise, for D = 64 two tokens, so that the eight 16-byte stores of a pass fall
         // into eight bank groups.  Unit n of a thread: token tok + 32 * (n / PER), column
         // unit0 or unit1.
         constexpr int PER = D / 64;      // units of a token pair row that a thread takes
-        constexpr int N = 4 * PER;       // units a thread widens per half tile (K or V)
-        const int t = threadIdx.x - 256, j = t & 7, odd = j >> 2;
+        constexpr int N = 4 * PER;       // units a thread widens per tile
+        const bool v = wg == 5;
+        const int t = threadIdx.x & 127, j = t & 7, odd = j >> 2;
         const int tok = 2 * (t >> 3) + odd;
         const int unit0 = D == 128 ? 4 * odd + (j & 3) : j & 3, unit1 = unit0 ^ 4;
         const int sw = tok & 7;          // the same for every token of the thread
         auto place = [&](int unit) { return (unit >> 2) * (MB * 128) + tok * 128 + (((2 * (unit & 3)) ^ sw) << 4); };
         const int at0 = place(unit0), at1 = place(unit1);
-        uint4 cur[N], nxt[N];
-        auto load = [&](int h) { // half tile h: keys of tile h / 2, then its values
-            const ManyTile &x = info[(h >> 1) % INFO];
-            const int8_t *codes = (h & 1 ? a.c.vq : a.c.kq) + (tok & 15) * D;
+        uint4 codes[N];
+        const int8_t *pool = (v ? a.c.vq : a.c.kq) + (tok & 15) * D + unit0 * 16;
+        auto load = [&](int i) { // the thread's units of tile i
+            const int *rows = info[i % INFO].row + (tok >> 4);
 #pragma unroll
             for (int n = 0; n < 4; n++) {
-                const int row = x.row[(tok >> 4) + 2 * n];
-                const int8_t *src = codes + (size_t)row * D;
+                const int row = rows[2 * n];
+                const int8_t *src = pool + (size_t)row * D;
 #pragma unroll
                 for (int u = 0; u < PER; u++)
-                    nxt[n * PER + u] = row >= 0 ? __ldg(reinterpret_cast<const uint4 *>(src + (u ? unit1 : unit0) * 16))
-                                                : make_uint4(0, 0, 0, 0);
+                    codes[n * PER + u] = row >= 0 ? __ldg(reinterpret_cast<const uint4 *>(src + (u ? (unit1 - unit0) * 16 : 0)))
+                                                  : make_uint4(0, 0, 0, 0);
             }
+            __syncwarp();
+            if (lane == 0) // the rows are read
+                mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
         };
-        ok = wait(B_INFO_FULL, 0);
-        if (ok)
+        if ((ok = wait(B_INFO_FULL, 0)))
             load(0);
 #pragma unroll 1
-        for (int h = 0; h < 2 * mine && ok; h++) {
-            const int i = h >> 1, b = i % Lay::KVS, use = i / Lay::KVS, v = h & 1;
-#pragma unroll
-            for (int n = 0; n < N; n++)
-                cur[n] = nxt[n];
-            if (h + 1 < 2 * mine) {
-                if (v && !(ok = wait(B_INFO_FULL + (i + 1) % INFO, (i + 1) / INFO)))
-                    break;
-                load(h + 1);
-            }
+        for (int i = 0; i < mine && ok; i++) {
+            const int b = i % Lay::KVS, use = i / Lay::KVS;
             if (!(ok = use == 0 || wait((v ? B_V_EMPTY : B_K_EMPTY) + b, use - 1)))
                 break;
             uint8_t *dst = smem + (v ? Lay::v_off : Lay::k_off) + b * Lay::T;
 #pragma unroll
             for (int n = 0; n < N; n++) {
                 uint4 a0, a1;
-                widen(cur[n], a0, a1);
-                uint8_t *o = dst + (n % PER ? at1 : at0) + (n / PER) * 32 * 128;
-                *reinterpret_cast<uint4 *>(o) = a0;
-                *reinterpret_cast<uint4 *>(dst + ((n % PER ? at1 : at0) ^ 16) + (n / PER) * 32 * 128) = a1;
+                widen(codes[n], a0, a1);
+                const int at = (n % PER ? at1 : at0) + (n / PER) * 32 * 128;
+                *reinterpret_cast<uint4 *>(dst + at) = a0;
+                *reinterpret_cast<uint4 *>(dst + (at ^ 16)) = a1;
             }
             fence_proxy_async_smem();
             mbar_arrive(&bar[(v ? B_V_FULL : B_K_FULL) + b]);
-            if (v) {
-                __syncwarp();
-                if (lane == 0)
-                    mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
+            if (i + 1 < mine) {
+                if (!(ok = wait(B_INFO_FULL + (i + 1) % INFO, (i + 1) / INFO)))
+                    break;
+                load(i + 1);
             }
         }
     } else if (wg == 3) {
@@ -635,7 +651,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
         if (warp == 12) {
             // ============================================= the products
             constexpr uint32_t QK = idesc_f16(MB, false), PV = idesc_f16(D, true);
-            const uint32_t sq = smem_addr(smem), sk = smem_addr(smem + Lay::k_off), sv = smem_addr(smem + Lay::v_off);
+            const uint32_t sq = sw128(smem_addr(smem), 16), sk = sw128(smem_addr(smem + Lay::k_off), 16),
+                           sv = sw128(smem_addr(smem + Lay::v_off), MB * 128);
             int item = -1;
             auto qk = [&](int i, bool first, bool last) {
                 item += first;
@@ -645,14 +662,12 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                            (i < 2 || wait(B_O_FULL + (i & 1), (i >> 1) - 1))))
                     return;
                 tc_after();
-#pragma unroll 1
+#pragma unroll
                 for (int c = 0; c < QP; c++)
-#pragma unroll 4
-                    for (int k = 0; k < D / 16; k++) {
-                        const uint32_t o = (uint32_t)((k >> 2) * MB * 128 + (k & 3) * 32);
-                        mma_ss(tmem + (uint32_t)(i & 1) * MB, sw128(sq + ((item & 1) * QP + c) * Lay::T + o, 16),
-                               sw128(sk + b * Lay::T + o, 16), QK, c || k);
-                    }
+#pragma unroll
+                    for (int k = 0; k < D / 64; k++)
+                        mma_ss4(tmem + (uint32_t)(i & 1) * MB, sq + (((item & 1) * QP + c) * Lay::T + k * MB * 128) / 16,
+                                sk + (b * Lay::T + k * MB * 128) / 16, QK, c || k);
                 tc_commit(&bar[B_K_EMPTY + b]);
                 if (last)
                     tc_commit(&bar[B_Q_EMPTY + (item & 1)]);
@@ -664,13 +679,12 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                            (i < 2 || wait(B_O_EMPTY + (i & 1), (i >> 1) - 1))))
                     return;
                 tc_after();
-#pragma unroll 1
+#pragma unroll
                 for (int c = 0; c < PP; c++)
-#pragma unroll 4
-                    for (int k = 0; k < MB / 16; k++)
-                        mma_ts(tmem + 2 * MB + (uint32_t)(i & 1) * MB,
-                               tmem + (uint32_t)(i & 1) * MB + 32 * (k >> 1) + 16 * c + 8 * (k & 1),
-                               sw128(sv + b * Lay::T + k * 2048, MB * 128), PV, c || k);
+#pragma unroll
+                    for (int k = 0; k < 2; k++) // 64 tokens
+                        mma_ts4(tmem + 2 * MB + (uint32_t)(i & 1) * MB, tmem + (uint32_t)(i & 1) * MB + 64 * k + 8 * c,
+                                sv + (b * Lay::T + k * 64 * 128) / 16, PV, c || k);
                 tc_commit(&bar[B_V_EMPTY + b]);
                 tc_commit(&bar[B_O_FULL + (i & 1)]);
             };
@@ -693,145 +707,105 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
             ok = ok && wait(B_K_EMPTY + b, use) && wait(B_V_EMPTY + b, use) && wait(B_Q_EMPTY + (item & 1), item >> 1);
         } else if (warp == 13) {
             // ============================================= pages and scales, ahead
+            // Four tiles at a time, eight lanes each: a tile's page and then its scales are two
+            // trips to memory, 2000 cycles, and alone a tile would wait for both.
             Walk at;
-            int tile = at.start(p, s_seq, s_at, R);
+            int tile = at.start(p, s_seq, s_at, R), item = 0;
             bool from_start = tile == 0;
-            for (int i = 0; i < mine && ok; i++) {
-                const int pos = tile * MB + (lane & 7) * 16, need = at.len + min(at.n, (at.mt + 1) * R);
+            const int q = lane >> 3, group = lane & 7;
+            for (int i0 = 0; i0 < mine && ok; i0 += 4) {
+                Walk own = at; // of tile i0 + q
+                int own_tile = tile, own_item = item;
+                bool own_start = from_start;
+                for (int c = 0; c < 4 && i0 + c < mine; c++) {
+                    if (c == q) {
+                        own = at;
+                        own_tile = tile;
+                        own_item = item;
+                        own_start = from_start;
+                    }
+                    if (++tile == at.nt && i0 + c + 1 < mine) {
+                        tile = 0;
+                        item++;
+                        from_start = true;
+                        at.next(p, rep, R);
+                    }
+                }
+                const int pos = own_tile * MB + group * 16, need = own.len + min(own.n, (own.mt + 1) * R);
                 int row = -1;
                 float ks = 0.0f, vs = 0.0f;
-                if (pos < need) {
-                    const int id = kv8_page(a.b, a.c, at.s, pos / a.c.page, a.err);
+                if (pos < need && i0 + q < mine) {
+                    const int id = kv8_page(a.b, a.c, own.s, pos / a.c.page, a.err);
                     if (id >= 0) {
-                        const size_t o = (size_t)id * a.c.n_kv + at.g;
+                        const size_t o = (size_t)id * a.c.n_kv + own.g;
                         row = (int)(o * a.c.page) + pos % a.c.page;
                         ks = a.c.ks[o];
                         vs = a.c.vs[o];
                     }
                 }
                 const float lvs = log2f(vs);
-                const bool hole = __any_sync(0xffffffffu, row < 0);
-                if (i >= INFO && !(ok = wait(B_INFO_EMPTY + i % INFO, i / INFO - 1)))
+                const bool hole = (__ballot_sync(0xffffffffu, row < 0) >> (8 * q)) & 255u;
+                for (int c = 0; c < 4 && i0 + c < mine && ok; c++) {
+                    const int i = i0 + c;
+                    if (i >= INFO && !(ok = wait(B_INFO_EMPTY + i % INFO, i / INFO - 1)))
+                        break;
+                    ManyTile &x = info[i % INFO];
+                    if (q == c) {
+                        x.row[group] = row;
+                        x.ks[group] = ks;
+                        x.lvs[group] = lvs;
+                        if (group == 0) {
+                            x.first = i == 0 || own_tile == 0;
+                            x.to_end = own_tile == own.nt - 1;
+                            x.last = x.to_end || i == mine - 1;
+                            x.masked = hole || own_tile * MB + MB > own.len + own.mt * R + 1;
+                            x.tile = own_tile;
+                            x.s = own.s;
+                            x.g = own.g;
+                            x.mt = own.mt;
+                            x.r0 = own.r0;
+                            x.n = own.n;
+                            x.len = own.len;
+                            x.from_start = own_start;
+                            x.item = own_item;
+                            x.pieces = (int)(((lo + i + (own.nt - 1 - own_tile) + 1) * active - 1) / total) - slot + 1;
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive(&bar[B_INFO_FULL + i % INFO]);
+                }
+            }
+        } else if (warp == 14) {
+            // ============================================= Q of the next rows
+            Walk at;
+            int begun = at.start(p, s_seq, s_at, R), left = mine; // tiles of the pair in front of this range; tiles left
+            int item = 0;
+            for (; left > 0 && ok; item++) {
+                if (!(ok = item < 2 || wait(B_Q_EMPTY + (item & 1), (item >> 1) - 1)))
                     break;
-                ManyTile &x = info[i % INFO];
-                if (lane < 8) {
-                    x.row[lane] = row;
-                    x.ks[lane] = ks;
-                    x.lvs[lane] = lvs;
-                }
                 if (lane == 0) {
-                    x.first = i == 0 || tile == 0;
-                    x.to_end = tile == at.nt - 1;
-                    x.last = x.to_end || i == mine - 1;
-                    x.masked = hole || tile * MB + MB > at.len + at.mt * R + 1;
-                    x.tile = tile;
-                    x.s = at.s;
-                    x.g = at.g;
-                    x.mt = at.mt;
-                    x.r0 = at.r0;
-                    x.n = at.n;
-                    x.len = at.len;
-                    x.from_start = from_start;
-                    x.pieces = (int)(((lo + i + (at.nt - 1 - tile) + 1) * active - 1) / total) - slot + 1;
+                    uint64_t *full = &bar[B_Q_FULL + (item & 1)];
+                    mbar_arrive_expect_tx(full, QP * D * 2 * R * rep);
+                    for (int c = 0; c < QP; c++)
+                        for (int d = 0; d < D; d += 64)
+                            asm volatile(
+                                "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+                                " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+                                    smem_addr(smem + ((item & 1) * QP + c) * Lay::T + d * MB * 2)),
+                                "l"(&p.tq), "r"(d), "r"(at.g * rep), "r"(at.r0 + at.mt * R), "r"(c), "r"(smem_addr(full))
+                                : "memory");
                 }
                 __syncwarp();
-                if (lane == 0)
-                    mbar_arrive(&bar[B_INFO_FULL + i % INFO]);
-                if (++tile == at.nt && i + 1 < mine) {
-                    tile = 0;
-                    from_start = true;
+                left -= at.nt - begun;
+                begun = 0;
+                if (left > 0)
                     at.next(p, rep, R);
-                }
             }
-        }
-    } else {
-        // ================================================= Q of the next rows
-        regs_down<72>();
-        constexpr int L = D / 8; // lanes of a vector: four dims of each half
-        constexpr int H = D / 2;
-        const int t = threadIdx.x - 512, j = t % L;
-        Walk at;
-        int begun = at.start(p, s_seq, s_at, R), left = mine; // tiles of the pair in front of this range; tiles left
-        for (int item = 0; left > 0 && ok; item++) {
-            if (!(ok = item < 2 || wait(B_Q_EMPTY + (item & 1), (item >> 1) - 1)))
-                break;
-            uint8_t *dst = smem + (item & 1) * QP * Lay::T;
-            // The rows come in with asynchronous copies, all at once, each into the 128-byte
-            // lines that its own f16 pieces will take: f32 rows four, 16-bit rows two
-            constexpr int UNITS = D * (int)sizeof(T) / 16;
-            auto line = [&](int r, int unit) { // unit of row r: line unit / 8 of the row's lines, natural order
-                return dst + (unit >> 3) * (MB * 128) + r * 128 + (unit & 7) * 16;
-            };
-#pragma unroll 1
-            for (int r = t / L; r < MB; r += 128 / L) {
-                const int row = at.mt * R + r / rep, head = at.g * rep + r % rep;
-                if (r < R * rep && row < at.n) {
-                    const uint8_t *src = reinterpret_cast<const uint8_t *>(reinterpret_cast<const T *>(a.q) +
-                                                                           (size_t)(at.r0 + row) * a.ld_q + (size_t)head * D);
-#pragma unroll
-                    for (int u = j; u < UNITS; u += L)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(line(r, u))),
-                                     "l"(src + u * 16)
-                                     : "memory");
-                }
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            __syncwarp();
-#pragma unroll 1
-            for (int r = t / L; r < MB; r += 128 / L) {
-                const int row = at.mt * R + r / rep;
-                const bool live = r < R * rep && row < at.n;
-                float4 u = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = u;
-                if (live) {
-                    constexpr int B = (int)sizeof(T);
-                    u = kv8_load4(reinterpret_cast<const T *>(line(r, 4 * j * B / 16) + 4 * j * B % 16));
-                    v = kv8_load4(reinterpret_cast<const T *>(line(r, (H + 4 * j) * B / 16) + (H + 4 * j) * B % 16));
-                    if (a.r.cos) {
-                        const size_t o = (size_t)(at.len + row) * H + 4 * j;
-                        const float4 c = kv8_load4(a.r.cos + o), s = kv8_load4(a.r.sin + o), w = u;
-                        u.x = __fsub_rn(__fmul_rn(w.x, c.x), __fmul_rn(v.x, s.x));
-                        u.y = __fsub_rn(__fmul_rn(w.y, c.y), __fmul_rn(v.y, s.y));
-                        u.z = __fsub_rn(__fmul_rn(w.z, c.z), __fmul_rn(v.z, s.z));
-                        u.w = __fsub_rn(__fmul_rn(w.w, c.w), __fmul_rn(v.w, s.w));
-                        v.x = __fadd_rn(__fmul_rn(w.x, s.x), __fmul_rn(v.x, c.x));
-                        v.y = __fadd_rn(__fmul_rn(w.y, s.y), __fmul_rn(v.y, c.y));
-                        v.z = __fadd_rn(__fmul_rn(w.z, s.z), __fmul_rn(v.z, c.z));
-                        v.w = __fadd_rn(__fmul_rn(w.w, s.w), __fmul_rn(v.w, c.w));
-                    }
-                }
-                float big = fmaxf(fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(u.z), fabsf(u.w))),
-                                  fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-#pragma unroll
-                for (int o = 1; o < L; o <<= 1) // and every lane of the row has read its part
-                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-                int e = (int)((__float_as_uint(big) >> 23) & 255u) - 127;
-                e = max(-126, min(126, e)); // a power of two brings the largest value into [1, 2)
-                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                if (j == 0)
-                    facs[(item & 1) * MB + r] = __uint_as_float((uint32_t)(127 + e) << 23) * a.scale * 1.4426950408889634f;
-                __syncwarp();
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const float x[4] = {(h ? v.x : u.x) * down, (h ? v.y : u.y) * down, (h ? v.z : u.z) * down,
-                                        (h ? v.w : u.w) * down};
-                    const int unit = (h * H + 4 * j) / 8;
-                    uint8_t *b = dst + (unit / 8) * (MB * 128) + r * 128 + (((unit & 7) ^ (r & 7)) << 4) + (j & 1) * 8;
-                    const uint32_t w0 = pack16(x[0], x[1]), w1 = pack16(x[2], x[3]);
-                    *reinterpret_cast<uint2 *>(b) = make_uint2(w0, w1);
-                    if constexpr (QP == 2) {
-                        const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&w0));
-                        const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&w1));
-                        *reinterpret_cast<uint2 *>(b + Lay::T) =
-                            make_uint2(pack16(x[0] - f0.x, x[1] - f0.y), pack16(x[2] - f1.x, x[3] - f1.y));
-                    }
-                }
-            }
-            fence_proxy_async_smem();
-            mbar_arrive(&bar[B_Q_FULL + (item & 1)]);
-            left -= at.nt - begun;
-            begun = 0;
-            if (left > 0)
-                at.next(p, rep, R);
+            // copies in flight land before the shared memory goes
+            for (int i = max(0, item - 2); i < item; i++)
+                for (int it = 0; it < 100000 && !mbar_try_wait(&bar[B_Q_FULL + (i & 1)], (uint32_t)((i >> 1) & 1)); it++)
+                    ;
         }
     }
     if (!ok) // let products in flight end before their memory goes
@@ -839,14 +813,105 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
             __nanosleep(1000);
     __syncthreads();
     if (warp == 12)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s_tmem), "r"(512) : "memory");
+}
+
+// Q of the sequences with many rows, once: rotated by its position, brought to
+// [1, 2) by a power of two of each vector's own (f16 holds it whatever its
+// magnitude), in QP f16 pieces.  A CTA a row.  Bound by its bytes; inside the
+// attention kernel two or four warps took 5 to 25 us for a tile's vectors,
+// which the tiles of a prompt's first rows, with few tokens each, waited for.
+template <class T, int D, int QP>
+__global__ void __launch_bounds__(QT) kv8_q_kernel(const __grid_constant__ ManyParams p)
+{
+    constexpr int L = D / 8; // lanes of a vector: four dims of each half
+    constexpr int H = D / 2;
+    const Kv8Attn &a = p.a;
+    const int row = blockIdx.x, j = threadIdx.x % L;
+    int s = 0; // the row's sequence: how many end at or before it
+    for (int s0 = 0; s0 < a.b.n_seqs; s0 += QT)
+        s += __syncthreads_count(s0 + (int)threadIdx.x < a.b.n_seqs && a.b.row_start[s0 + threadIdx.x + 1] <= row);
+    if (s >= a.b.n_seqs)
+        return;
+    int r0, n, len;
+    kv8_seq(a.b, s, a.err, r0, n, len);
+    if (row < r0 || row >= r0 + n || (long long)n * (a.n_heads / a.c.n_kv) <= p.many)
+        return;
+    const T *q = reinterpret_cast<const T *>(a.q) + (size_t)row * a.ld_q;
+    float4 c = make_float4(1.0f, 1.0f, 1.0f, 1.0f), t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (a.r.cos) {
+        const size_t o = (size_t)(len + row - r0) * H + 4 * j;
+        c = kv8_load4(a.r.cos + o);
+        t = kv8_load4(a.r.sin + o);
+    }
+    for (int h0 = 0; h0 < a.n_heads; h0 += QT / L) { // whole warps: the shuffles are among all lanes
+        const int h = h0 + (int)threadIdx.x / L;
+        const bool live = h < a.n_heads;
+        float4 u = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = u;
+        if (live) {
+            u = kv8_load4(q + (size_t)h * D + 4 * j);
+            v = kv8_load4(q + (size_t)h * D + H + 4 * j);
+            if (a.r.cos) {
+                const float4 w = u;
+                u.x = __fsub_rn(__fmul_rn(w.x, c.x), __fmul_rn(v.x, t.x));
+                u.y = __fsub_rn(__fmul_rn(w.y, c.y), __fmul_rn(v.y, t.y));
+                u.z = __fsub_rn(__fmul_rn(w.z, c.z), __fmul_rn(v.z, t.z));
+                u.w = __fsub_rn(__fmul_rn(w.w, c.w), __fmul_rn(v.w, t.w));
+                v.x = __fadd_rn(__fmul_rn(w.x, t.x), __fmul_rn(v.x, c.x));
+                v.y = __fadd_rn(__fmul_rn(w.y, t.y), __fmul_rn(v.y, c.y));
+                v.z = __fadd_rn(__fmul_rn(w.z, t.z), __fmul_rn(v.z, c.z));
+                v.w = __fadd_rn(__fmul_rn(w.w, t.w), __fmul_rn(v.w, c.w));
+            }
+        }
+        float big = fmaxf(fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(u.z), fabsf(u.w))),
+                          fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+#pragma unroll
+        for (int o = 1; o < L; o <<= 1)
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+        int e = (int)((__float_as_uint(big) >> 23) & 255u) - 127;
+        e = max(-126, min(126, e));
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+        if (!live)
+            continue;
+        const size_t vec = (size_t)row * a.n_heads + h;
+        if (j == 0)
+            p.facs[vec] = __uint_as_float((uint32_t)(127 + e) << 23) * a.scale * 1.4426950408889634f;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const float x[4] = {(k ? v.x : u.x) * down, (k ? v.y : u.y) * down, (k ? v.z : u.z) * down,
+                                (k ? v.w : u.w) * down};
+            __half *o = p.q16 + vec * D + k * H + 4 * j;
+            const uint32_t w0 = pack16(x[0], x[1]), w1 = pack16(x[2], x[3]);
+            *reinterpret_cast<uint2 *>(o) = make_uint2(w0, w1);
+            if constexpr (QP == 2) {
+                const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&w0));
+                const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&w1));
+                *reinterpret_cast<uint2 *>(o + (size_t)a.b.n_rows * a.n_heads * D) =
+                    make_uint2(pack16(x[0] - f0.x, x[1] - f0.y), pack16(x[2] - f1.x, x[3] - f1.y));
+            }
+        }
+    }
 }
 
 template <class T, int D, int QP, int PP>
-int run(const ManyParams &p, int ctas, cudaStream_t stream)
+int run(ManyParams &p, int ctas, cudaStream_t stream)
 {
+    auto fn = tensor_map_encoder();
+    if (!fn)
+        return fail(LLMRS_ECUDA, "cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t heads = p.a.n_heads, rows = p.a.b.n_rows;
+    const cuuint32_t rep = p.a.n_heads / p.a.c.n_kv;
+    const cuuint64_t dims[4] = {D, heads, rows, QP};
+    const cuuint64_t strides[3] = {D * 2, heads * D * 2, rows * heads * D * 2};
+    const cuuint32_t box[4] = {64, rep, MB / rep, 1}, estr[4] = {1, 1, 1, 1};
+    const CUresult r = fn(&p.tq, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, p.q16, dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(LLMRS_ECUDA, "cuTensorMapEncodeTiled (prepared Q) failed (%d)", (int)r);
+    LLMRS_CUDA_TRY(launch(kv8_q_kernel<T, D, QP>, dim3(p.a.b.n_rows), dim3(QT), 0, stream, false, p));
     LLMRS_CUDA_TRY(launch(kv8_many_kernel<T, D, QP, PP>, dim3(ctas), dim3(MANY_THREADS), ManyLay<D, QP>::bytes, stream,
-                          false, p));
+                          true, p));
     LLMRS_CUDA_TRY(launch(kv8_join_kernel<T, D, MB>, dim3(8 * ctas), dim3(JT), 0, stream, true, p.a,
                           (const float *)p.part, (const JoinHead *)p.head, ctas));
     return LLMRS_OK;
@@ -861,9 +926,15 @@ cudaError_t prepare()
 
 } // namespace
 
-size_t kv8_many_workspace(int head_dim)
+static size_t pieces_bytes(int head_dim)
 {
-    return (size_t)MANY_CTAS * (sizeof(JoinHead) + 2 * (size_t)MB * (head_dim + 2) * sizeof(float));
+    const size_t bytes = (size_t)MANY_CTAS * (sizeof(JoinHead) + 2 * (size_t)MB * (head_dim + 2) * sizeof(float));
+    return (bytes + 255) & ~(size_t)255;
+}
+
+size_t kv8_many_workspace(int head_dim, int n_heads, int n_rows)
+{
+    return pieces_bytes(head_dim) + (size_t)n_rows * n_heads * (2 * head_dim * sizeof(__half) + sizeof(float));
 }
 
 int kv8_many_prepare(void)
@@ -890,6 +961,8 @@ int kv8_many(const Kv8Attn &a, int many, void *ws, int sms, cudaStream_t stream)
     p.a = a;
     p.head = reinterpret_cast<JoinHead *>(ws);
     p.part = reinterpret_cast<float *>(p.head + MANY_CTAS);
+    p.q16 = reinterpret_cast<__half *>(reinterpret_cast<uint8_t *>(ws) + pieces_bytes(a.c.D));
+    p.facs = reinterpret_cast<float *>(p.q16 + 2 * (size_t)a.b.n_rows * a.n_heads * a.c.D);
     p.many = many;
     const int ctas = sms < MANY_CTAS ? sms : MANY_CTAS;
     if (a.dtype == LLMRS_F32)

@@ -697,7 +697,7 @@ int llmrs_kv8_attention_workspace(const llmrs_kv8 *cache, const llmrs_kv8_batch 
     LLMRS_TRY(check_batch(cache, batch));
     LLMRS_CHECK_ARG(bytes && n_rows >= 0 && n_heads > 0 && n_heads % cache->n_kv_heads == 0,
                     "kv8_attention_workspace: bad arguments");
-    *bytes = llmrs::kv8_attention_workspace(n_heads / cache->n_kv_heads, cache->head_dim, n_rows, batch->n_seqs);
+    *bytes = llmrs::kv8_attention_workspace(n_heads, cache->n_kv_heads, cache->head_dim, n_rows, batch->n_seqs);
     return LLMRS_OK;
 }
 
@@ -722,7 +722,7 @@ int llmrs_kv8_attention(llmrs_ctx *ctx, const llmrs_kv8 *cache, const llmrs_kv8_
     OnDevice on(ctx->device);
     void *ws = nullptr;
     LLMRS_TRY(take_workspace(ctx, "kv8_attention", d_workspace, workspace_bytes,
-                             llmrs::kv8_attention_workspace(n_heads / cache->n_kv_heads, cache->head_dim, n_rows, batch->n_seqs), &ws));
+                             llmrs::kv8_attention_workspace(n_heads, cache->n_kv_heads, cache->head_dim, n_rows, batch->n_seqs), &ws));
     Kv8Attn a{};
     a.c = kv8_of(cache);
     a.b = batch_of(cache, batch, n_rows, d_rope_cos, n_pos);
