@@ -17,9 +17,10 @@
 // fetches Q, which a kernel of its own has rotated, scaled and split.
 // The softmax keeps no state: it hands over a tile's maximum, sum and scale, and
 // the output warps, which go through the tiles in order, know the running ones.
-// S and O are double buffered (4 x 128 columns: all of TMEM), P lies over the S
-// it came from, Q is double buffered, K and V too where Q is one piece, so the
-// product of tile i + 1 runs while tile i is in the softmax.
+// TMEM: three S, P over the S it came from, and O in the rest (once for heads of
+// 128, twice for 64): tiles i and i + 1 are in the softmax while the product of
+// tile i - 1 runs and the scores of tile i + 2 are made.  K and V are double
+// buffered, Q too but for two pieces of 128 dims.
 //
 // What a tile costs is not a product's 1000 cycles but the longest of the roles'
 // chains, whose instructions take 4 to 5 cycles each: so each role that was the
@@ -42,7 +43,8 @@ namespace {
 constexpr int MB = 128;          // vectors, and tokens, of a tile
 constexpr int MANY_THREADS = 768;
 constexpr int INFO = 8;          // tile descriptions in flight
-constexpr int RING = 4;          // softmax -> output hand-overs in flight
+constexpr int RING = 6;          // softmax -> output hand-overs in flight
+constexpr int NS = 3;            // buffers of S
 constexpr int QT = 256;          // threads of the kernel that prepares Q
 
 struct ManyTile {
@@ -70,9 +72,11 @@ struct ManyParams {
 
 template <int D, int QP>
 struct ManyLay {
-    static constexpr int KVS = QP == 1 ? 2 : 1; // buffers of K and of V
+    static constexpr int KVS = 2;                   // buffers of K and of V
+    static constexpr int QS = QP * D > 128 ? 1 : 2; // of Q
+    static constexpr int OS = (512 - NS * MB) / D;  // of O
     static constexpr int T = MB * D * 2;        // bytes of one piece of Q, of an f16 K or V tile
-    static constexpr int k_off = 2 * QP * T;    // Q: [2 buffers][QP pieces]
+    static constexpr int k_off = QS * QP * T;   // Q: [buffers][QP pieces]
     static constexpr int v_off = k_off + KVS * T;
     static constexpr int info_off = v_off + KVS * T;
     static constexpr int ring_off = info_off + INFO * (int)sizeof(ManyTile);
@@ -89,8 +93,9 @@ enum : int { // barriers
     B_V_FULL = B_K_EMPTY + 2,
     B_V_EMPTY = B_V_FULL + 2,
     B_S_FULL = B_V_EMPTY + 2,
-    B_P_FULL = B_S_FULL + 2,
-    B_O_FULL = B_P_FULL + 2,
+    B_P_FULL = B_S_FULL + NS,
+    B_P_EMPTY = B_P_FULL + NS,
+    B_O_FULL = B_P_EMPTY + NS,
     B_O_EMPTY = B_O_FULL + 2,
     B_Q_FULL = B_O_EMPTY + 2,
     B_Q_EMPTY = B_Q_FULL + 2,
@@ -300,12 +305,15 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
             mbar_init(&bar[B_K_EMPTY + i], 1);
             mbar_init(&bar[B_V_FULL + i], 128);
             mbar_init(&bar[B_V_EMPTY + i], 1);
-            mbar_init(&bar[B_S_FULL + i], 1);
-            mbar_init(&bar[B_P_FULL + i], 128);
             mbar_init(&bar[B_O_FULL + i], 1);
             mbar_init(&bar[B_O_EMPTY + i], 128);
             mbar_init(&bar[B_Q_FULL + i], 1);
             mbar_init(&bar[B_Q_EMPTY + i], 1);
+        }
+        for (int i = 0; i < NS; i++) {
+            mbar_init(&bar[B_S_FULL + i], 1);
+            mbar_init(&bar[B_P_FULL + i], 128);
+            mbar_init(&bar[B_P_EMPTY + i], 1);
         }
         fence_mbar_init();
         s_seq = 0;
@@ -384,15 +392,16 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
         // ================================================= softmax of every other tile: thread = row
         static_assert(2 * 80 + 160 + 2 * 56 + 48 == 6 * 80, "the launch's registers, shared out");
         const int r = threadIdx.x & 127, odd = wg >> 2;
-        const uint32_t sp = tmem + (uint32_t)odd * MB + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         float fac = 0.0f;
         int lim = -1, item = -1;
         bool busy = false; // some row of this warp is there
         for (int i = odd; i < mine && ok; i += 2) {
             const ManyTile &x = info[i % INFO];
-            if (!(ok = wait(B_INFO_FULL + i % INFO, i / INFO) && wait(B_S_FULL + odd, i >> 1)))
+            if (!(ok = wait(B_INFO_FULL + i % INFO, i / INFO) && wait(B_S_FULL + i % NS, i / NS)))
                 break;
             tc_after();
+            const uint32_t sp = lanes + (uint32_t)(i % NS) * MB;
             if (x.item != item) {
                 item = x.item;
                 const int row = x.mt * R + r / rep;
@@ -503,7 +512,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
             hand[MB + r] = ref2;
             hand[2 * MB + r] = sum;
             tc_before();
-            mbar_arrive(&bar[B_P_FULL + odd]);
+            mbar_arrive(&bar[B_P_FULL + i % NS]);
             __syncwarp();
             if (lane == 0)
                 mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
@@ -512,12 +521,12 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
         // ================================================= output: thread = row
         regs_up<160>();
         const int r = threadIdx.x - 128;
-        const uint32_t lanes = tmem + 2 * MB + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t lanes = tmem + NS * MB + ((uint32_t)((warp & 3) * 32) << 16);
         float2 acc[D / 2];
         float m = -INFINITY, l = 0.0f; // the softmax's running maximum and sum
         for (int i = 0; i < mine && ok; i++) {
             const ManyTile &x = info[i % INFO];
-            if (!(ok = wait(B_INFO_FULL + i % INFO, i / INFO) && wait(B_O_FULL + (i & 1), i >> 1)))
+            if (!(ok = wait(B_INFO_FULL + i % INFO, i / INFO) && wait(B_O_FULL + i % Lay::OS, i / Lay::OS)))
                 break;
             tc_after();
             const float *hand = ring + (i % RING) * 3 * MB;
@@ -539,11 +548,11 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
 #pragma unroll
             for (int k = 0; k < D / 16; k++) {
                 uint32_t o[16];
-                tm_ld16(lanes + (uint32_t)(i & 1) * MB + 16 * k, o);
+                tm_ld16(lanes + (uint32_t)(i % Lay::OS) * D + 16 * k, o);
                 tm_wait(o);
                 if (k == D / 16 - 1) {
                     tc_before();
-                    mbar_arrive(&bar[B_O_EMPTY + (i & 1)]);
+                    mbar_arrive(&bar[B_O_EMPTY + i % Lay::OS]);
                 }
 #pragma unroll
                 for (int d = 0; d < 8; d++)
@@ -657,39 +666,40 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
             auto qk = [&](int i, bool first, bool last) {
                 item += first;
                 const int b = i % Lay::KVS;
-                // S lies under the P of tile i - 2, which that tile's product has read
-                if (!(ok = (!first || wait(B_Q_FULL + (item & 1), item >> 1)) && wait(B_K_FULL + b, i / Lay::KVS) &&
-                           (i < 2 || wait(B_O_FULL + (i & 1), (i >> 1) - 1))))
+                // S lies under the P of tile i - NS, which that tile's product has read
+                if (!(ok = (!first || wait(B_Q_FULL + item % Lay::QS, item / Lay::QS)) && wait(B_K_FULL + b, i / Lay::KVS) &&
+                           (i < NS || wait(B_P_EMPTY + i % NS, i / NS - 1))))
                     return;
                 tc_after();
 #pragma unroll
                 for (int c = 0; c < QP; c++)
 #pragma unroll
                     for (int k = 0; k < D / 64; k++)
-                        mma_ss4(tmem + (uint32_t)(i & 1) * MB, sq + (((item & 1) * QP + c) * Lay::T + k * MB * 128) / 16,
+                        mma_ss4(tmem + (uint32_t)(i % NS) * MB, sq + ((item % Lay::QS * QP + c) * Lay::T + k * MB * 128) / 16,
                                 sk + (b * Lay::T + k * MB * 128) / 16, QK, c || k);
                 tc_commit(&bar[B_K_EMPTY + b]);
                 if (last)
-                    tc_commit(&bar[B_Q_EMPTY + (item & 1)]);
-                tc_commit(&bar[B_S_FULL + (i & 1)]);
+                    tc_commit(&bar[B_Q_EMPTY + item % Lay::QS]);
+                tc_commit(&bar[B_S_FULL + i % NS]);
             };
             auto pv = [&](int i) {
                 const int b = i % Lay::KVS;
-                if (!(ok = wait(B_P_FULL + (i & 1), i >> 1) && wait(B_V_FULL + b, i / Lay::KVS) &&
-                           (i < 2 || wait(B_O_EMPTY + (i & 1), (i >> 1) - 1))))
+                if (!(ok = wait(B_P_FULL + i % NS, i / NS) && wait(B_V_FULL + b, i / Lay::KVS) &&
+                           (i < Lay::OS || wait(B_O_EMPTY + i % Lay::OS, i / Lay::OS - 1))))
                     return;
                 tc_after();
 #pragma unroll
                 for (int c = 0; c < PP; c++)
 #pragma unroll
                     for (int k = 0; k < 2; k++) // 64 tokens
-                        mma_ts4(tmem + 2 * MB + (uint32_t)(i & 1) * MB, tmem + (uint32_t)(i & 1) * MB + 64 * k + 8 * c,
+                        mma_ts4(tmem + NS * MB + (uint32_t)(i % Lay::OS) * D, tmem + (uint32_t)(i % NS) * MB + 64 * k + 8 * c,
                                 sv + (b * Lay::T + k * 64 * 128) / 16, PV, c || k);
                 tc_commit(&bar[B_V_EMPTY + b]);
-                tc_commit(&bar[B_O_FULL + (i & 1)]);
+                tc_commit(&bar[B_P_EMPTY + i % NS]);
+                tc_commit(&bar[B_O_FULL + i % Lay::OS]);
             };
 #pragma unroll 1
-            for (int i = 0; i <= mine && ok; i++) { // the scores of tile i, then the output of tile i - 1
+            for (int i = 0; i < mine + 2 && ok; i++) { // the scores of tile i, then the output of tile i - 2
                 if (i < mine) {
                     if (!(ok = wait(B_INFO_FULL + i % INFO, i / INFO)))
                         break;
@@ -699,12 +709,13 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                         mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
                     qk(i, first, last);
                 }
-                if (ok && i)
-                    pv(i - 1);
+                if (ok && i > 1)
+                    pv(i - 2);
             }
             // every arrival lands before the barriers go
             const int b = (mine - 1) % Lay::KVS, use = (mine - 1) / Lay::KVS;
-            ok = ok && wait(B_K_EMPTY + b, use) && wait(B_V_EMPTY + b, use) && wait(B_Q_EMPTY + (item & 1), item >> 1);
+            ok = ok && wait(B_K_EMPTY + b, use) && wait(B_V_EMPTY + b, use) && wait(B_Q_EMPTY + item % Lay::QS, item / Lay::QS) &&
+                 wait(B_P_EMPTY + (mine - 1) % NS, (mine - 1) / NS);
         } else if (warp == 13) {
             // ============================================= pages and scales, ahead
             // Four tiles at a time, eight lanes each: a tile's page and then its scales are two
@@ -782,17 +793,17 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
             int begun = at.start(p, s_seq, s_at, R), left = mine; // tiles of the pair in front of this range; tiles left
             int item = 0;
             for (; left > 0 && ok; item++) {
-                if (!(ok = item < 2 || wait(B_Q_EMPTY + (item & 1), (item >> 1) - 1)))
+                if (!(ok = item < Lay::QS || wait(B_Q_EMPTY + item % Lay::QS, item / Lay::QS - 1)))
                     break;
                 if (lane == 0) {
-                    uint64_t *full = &bar[B_Q_FULL + (item & 1)];
+                    uint64_t *full = &bar[B_Q_FULL + item % Lay::QS];
                     mbar_arrive_expect_tx(full, QP * D * 2 * R * rep);
                     for (int c = 0; c < QP; c++)
                         for (int d = 0; d < D; d += 64)
                             asm volatile(
                                 "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
                                 " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-                                    smem_addr(smem + ((item & 1) * QP + c) * Lay::T + d * MB * 2)),
+                                    smem_addr(smem + (item % Lay::QS * QP + c) * Lay::T + d * MB * 2)),
                                 "l"(&p.tq), "r"(d), "r"(at.g * rep), "r"(at.r0 + at.mt * R), "r"(c), "r"(smem_addr(full))
                                 : "memory");
                 }
@@ -803,8 +814,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                     at.next(p, rep, R);
             }
             // copies in flight land before the shared memory goes
-            for (int i = max(0, item - 2); i < item; i++)
-                for (int it = 0; it < 100000 && !mbar_try_wait(&bar[B_Q_FULL + (i & 1)], (uint32_t)((i >> 1) & 1)); it++)
+            for (int i = max(0, item - Lay::QS); i < item; i++)
+                for (int it = 0; it < 100000 && !mbar_try_wait(&bar[B_Q_FULL + i % Lay::QS], (uint32_t)((i / Lay::QS) & 1)); it++)
                     ;
         }
     }
