@@ -217,6 +217,7 @@ __global__ void __launch_bounds__(few_warps(NT) * 32, 1) kv8_few_kernel(const __
         base += all;
     }
     __syncthreads();
+    griddep_wait(); // the kernels for many rows are done with the workspace
     const int slot = warp * gridDim.x + blockIdx.x;
     const long long lo = slot < active ? total * slot / active : 0;
     const long long hi = slot < active ? total * (slot + 1) / active : 0;
@@ -730,7 +731,7 @@ int run_few(const FewParams &p, int ctas, cudaStream_t stream)
     constexpr int GV = group_vectors<SPLIT, NT>();
     constexpr int FW = few_warps(NT);
     LLMRS_CUDA_TRY(launch(kv8_few_kernel<T, D, SPLIT, NT>, dim3(ctas), dim3(FW * 32), FewLay<D, NT>::bytes, stream,
-                          false, p));
+                          p.many != INT32_MAX, p));
     LLMRS_CUDA_TRY(launch(kv8_join_kernel<T, D, GV>, dim3(4 * ctas), dim3(JT), 0, stream, true, p.a,
                           (const float *)p.part, (const JoinHead *)p.head, ctas * FW));
     return LLMRS_OK;

