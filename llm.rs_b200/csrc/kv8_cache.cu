@@ -22,6 +22,7 @@ namespace llmrs {
 namespace {
 
 constexpr int AP_THREADS = 256;
+constexpr int FULL_WARPS = 4; // to a unit of full pages
 
 __device__ __forceinline__ float rot_lo(float lo, float hi, float c, float s)
 {
@@ -41,28 +42,43 @@ __device__ __forceinline__ float finite_or_zero(float x, bool &bad)
     return 0.0f;
 }
 
+// Four codes rint(x * inv).  1.5 * 2^23 added rounds to an integer, to even on a
+// tie like rint, and leaves it in the low byte.  New values need no clamp: |x| is
+// at most 127 s1 (1 + 2^-24) and inv rounds once more, so x * inv stays below
+// 127.0001.  Old codes may be -128 in a cache that another program filled.
+template <bool CLAMP>
 __device__ __forceinline__ uint32_t code4(float4 x, float inv)
 {
-    const float v[4] = {x.x, x.y, x.z, x.w};
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float r = fminf(fmaxf(rintf(__fmul_rn(v[i], inv)), -127.0f), 127.0f);
-        w |= ((uint32_t)(int)r & 0xffu) << (8 * i);
-    }
-    return w;
+    auto code = [&](float v) {
+        v = __fmul_rn(v, inv);
+        if constexpr (CLAMP)
+            v = fminf(fmaxf(v, -127.0f), 127.0f);
+        return __float_as_uint(__fadd_rn(v, 12582912.0f));
+    };
+    const uint32_t a = __byte_perm(code(x.x), code(x.y), 0x0040), c = __byte_perm(code(x.z), code(x.w), 0x0040);
+    return __byte_perm(a, c, 0x5410);
 }
 
-// One CTA per (touched page, KV head, K or V).  Bound by reading the rows.
-template <class T, int D>
+// WARPS warps per (touched page, KV head, K or V), the others of the CTA take
+// further heads of the page.  Up to HOLD rows of a thread are loaded at once and
+// stay in registers between the maximum and the codes; longer ones are read again,
+// from the L2.  Full pages are bound by reading the rows: 8192 rows of 8 heads of
+// 128, f32, pages of 32 take 26 us (84 MB: half of the memory's rate, whatever the
+// warps, rows held and CTAs per SM).  A row or two per page are a chain of loads
+// that depend on one another, so a warp to a unit keeps all of a decode step's
+// chains on the GPU at once: 191 rows 5 us, and 14 with a CTA to a unit.
+template <class T, int D, int WARPS>
 __global__ void __launch_bounds__(AP_THREADS) kv8_append_kernel(Kv8 c, Kv8Batch b, const T *k, const T *v,
                                                                 long long ld, Kv8Rope rope, uint32_t *err)
 {
     constexpr int TPR = D / 8;              // threads per row: dims 4j.. and D/2 + 4j..
-    constexpr int RPI = AP_THREADS / TPR;   // rows per round
+    constexpr int THREADS = 32 * WARPS;     // of a unit
+    constexpr int RPI = THREADS / TPR;      // rows per round
+    constexpr int HOLD = 2;
     __shared__ float s_max[AP_THREADS / 32];
-    const int page = c.page, g = blockIdx.y;
-    const bool is_v = blockIdx.z != 0;
+    const int page = c.page, unit = blockIdx.y * (AP_THREADS / THREADS) + (int)threadIdx.x / THREADS;
+    const int g = unit >> 1, tid = threadIdx.x % THREADS;
+    const bool is_v = unit & 1;
     long long within = 0;
     const int s = kv8_find_unit<AP_THREADS>(
         b.n_seqs, blockIdx.x,
@@ -72,7 +88,7 @@ __global__ void __launch_bounds__(AP_THREADS) kv8_append_kernel(Kv8 c, Kv8Batch 
             return n ? (len + n - 1) / page - len / page + 1 : 0;
         },
         within);
-    if (s < 0)
+    if (s < 0 || g >= c.n_kv)
         return;
     int r0, n, len;
     kv8_seq(b, s, err, r0, n, len);
@@ -87,9 +103,10 @@ __global__ void __launch_bounds__(AP_THREADS) kv8_append_kernel(Kv8 c, Kv8Batch 
     int8_t *codes = (is_v ? c.vq : c.kq) + at * page * D;
     float *scale = (is_v ? c.vs : c.ks) + at;
     const float s0 = held ? *scale : 0.0f;
-    const int j = threadIdx.x % TPR, rr = threadIdx.x / TPR;
+    const int j = tid % TPR, rr = tid / TPR, rows = t1 - t0;
     const bool turn = !is_v && rope.cos;
     bool bad = false;
+    bool clean = false; // some value is not finite, and goes as zero
     auto row = [&](int i, float4 &lo, float4 &hi) { // new row i: 4 values of each half, rotated
         const T *x = src + (size_t)i * ld;
         lo = kv8_load4(x + 4 * j);
@@ -104,44 +121,86 @@ __global__ void __launch_bounds__(AP_THREADS) kv8_append_kernel(Kv8 c, Kv8Batch 
             hi = make_float4(rot_hi(a.x, h.x, cs.x, sn.x), rot_hi(a.y, h.y, cs.y, sn.y),
                              rot_hi(a.z, h.z, cs.z, sn.z), rot_hi(a.w, h.w, cs.w, sn.w));
         }
-        lo = make_float4(finite_or_zero(lo.x, bad), finite_or_zero(lo.y, bad), finite_or_zero(lo.z, bad),
-                         finite_or_zero(lo.w, bad));
-        hi = make_float4(finite_or_zero(hi.x, bad), finite_or_zero(hi.y, bad), finite_or_zero(hi.z, bad),
-                         finite_or_zero(hi.w, bad));
+        if (clean) {
+            lo = make_float4(finite_or_zero(lo.x, bad), finite_or_zero(lo.y, bad), finite_or_zero(lo.z, bad),
+                             finite_or_zero(lo.w, bad));
+            hi = make_float4(finite_or_zero(hi.x, bad), finite_or_zero(hi.y, bad), finite_or_zero(hi.z, bad),
+                             finite_or_zero(hi.w, bad));
+        }
     };
-    float m = 0.0f;
-    for (int i = rr; i < t1 - t0; i += RPI) {
-        float4 lo, hi;
-        row(i, lo, hi);
-        m = fmaxf(m, fmaxf(fmaxf(fabsf(lo.x), fabsf(lo.y)), fmaxf(fabsf(lo.z), fabsf(lo.w))));
-        m = fmaxf(m, fmaxf(fmaxf(fabsf(hi.x), fabsf(hi.y)), fmaxf(fabsf(hi.z), fabsf(hi.w))));
-    }
-    m = warp_max(m);
-    if ((threadIdx.x & 31) == 0)
-        s_max[threadIdx.x >> 5] = m;
-    __syncthreads();
+    float4 lo[HOLD], hi[HOLD];
+    auto largest = [&]() { // of the unit's rows, infinite when a value is not finite
+        float m = 0.0f, nan = 0.0f; // a product with zero is zero but for those
+        auto see = [&](float x) {
+            m = fmaxf(m, fabsf(x));
+            nan = fmaf(x, 0.0f, nan);
+        };
+        for (int i0 = rr; i0 < rows; i0 += HOLD * RPI) {
 #pragma unroll
-    for (int w = 0; w < AP_THREADS / 32; w++)
-        m = fmaxf(m, s_max[w]);
+            for (int u = 0; u < HOLD; u++) {
+                lo[u] = hi[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (i0 + u * RPI < rows)
+                    row(i0 + u * RPI, lo[u], hi[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < HOLD; u++) {
+                see(lo[u].x), see(lo[u].y), see(lo[u].z), see(lo[u].w);
+                see(hi[u].x), see(hi[u].y), see(hi[u].z), see(hi[u].w);
+            }
+        }
+        m = warp_max(nan == 0.0f ? m : INFINITY);
+        if constexpr (WARPS > 1) {
+            const int first = (int)threadIdx.x / THREADS * WARPS;
+            auto sync = [&]() { // the unit's warps
+                asm volatile("bar.sync %0, %1;" ::"r"(1 + (int)threadIdx.x / THREADS), "n"(THREADS) : "memory");
+            };
+            sync(); // an earlier call's maxima are read
+            if ((threadIdx.x & 31) == 0)
+                s_max[threadIdx.x >> 5] = m;
+            sync();
+#pragma unroll
+            for (int w = 0; w < WARPS; w++)
+                m = fmaxf(m, s_max[first + w]);
+        }
+        return m;
+    };
+    float m = largest();
+    if (m == INFINITY) { // the same in the whole unit
+        clean = true;
+        m = largest();
+    }
     float s1 = fmaxf(s0, __fdiv_rn(m, 127.0f));
     if (s1 < FLT_MIN)
         s1 = 0.0f;
     const float inv = s1 > 0.0f ? __fdiv_rn(1.0f, s1) : 0.0f;
-    for (int i = rr; i < t1 - t0; i += RPI) {
-        float4 lo, hi;
-        row(i, lo, hi);
-        int8_t *dst = codes + (size_t)(held + i) * D;
-        *reinterpret_cast<uint32_t *>(dst + 4 * j) = code4(lo, inv);
-        *reinterpret_cast<uint32_t *>(dst + D / 2 + 4 * j) = code4(hi, inv);
+    const bool again = rows > HOLD * RPI; // more rows than the registers held
+    for (int i0 = rr; i0 < rows; i0 += HOLD * RPI) {
+#pragma unroll
+        for (int u = 0; u < HOLD; u++) {
+            const int i = i0 + u * RPI;
+            if (i >= rows)
+                continue;
+            if (again)
+                row(i, lo[u], hi[u]);
+            int8_t *dst = codes + (size_t)(held + i) * D;
+            *reinterpret_cast<uint32_t *>(dst + 4 * j) = code4<false>(lo[u], inv);
+            *reinterpret_cast<uint32_t *>(dst + D / 2 + 4 * j) = code4<false>(hi[u], inv);
+        }
     }
     if (s1 > s0 && held) {
         const float ratio = __fdiv_rn(s0, s1);
-        for (int w = threadIdx.x; w < held * D / 4; w += AP_THREADS) {
-            const char4 o = reinterpret_cast<const char4 *>(codes)[w];
-            reinterpret_cast<uint32_t *>(codes)[w] = code4(make_float4(o.x, o.y, o.z, o.w), ratio);
+        for (int w = tid; w < held * D / 16; w += THREADS) {
+            int4 x = reinterpret_cast<const int4 *>(codes)[w];
+            char4 o[4];
+            memcpy(o, &x, 16);
+            uint32_t y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                y[e] = code4<true>(make_float4(o[e].x, o[e].y, o[e].z, o[e].w), ratio);
+            reinterpret_cast<uint4 *>(codes)[w] = make_uint4(y[0], y[1], y[2], y[3]);
         }
     }
-    if (threadIdx.x == 0)
+    if (tid == 0)
         *scale = s1;
     if (bad)
         atomicCAS(err, 0u, (uint32_t)DEV_ERR_NONFINITE);
@@ -179,14 +238,28 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, const int *pages, 
     }
 }
 
+template <class T, int D>
+cudaError_t append_d(const Kv8 &c, const Kv8Batch &b, const T *k, const T *v, long long ld, const Kv8Rope &r,
+                     uint32_t *err, unsigned pages, cudaStream_t stream)
+{
+    auto run = [&](auto kernel, int warps) {
+        const int per = AP_THREADS / 32 / warps; // units of a CTA
+        return launch(kernel, dim3(pages, (2 * c.n_kv + per - 1) / per), dim3(AP_THREADS), 0, stream, false, c, b, k, v, ld,
+                      r, err);
+    };
+    if (b.n_rows <= 2 * b.n_seqs) // a decode step: a row or two per page
+        return run(kv8_append_kernel<T, D, 1>, 1);
+    return run(kv8_append_kernel<T, D, FULL_WARPS>, FULL_WARPS);
+}
+
 template <class T>
 cudaError_t append_t(const Kv8 &c, const Kv8Batch &b, const void *k, const void *v, long long ld, const Kv8Rope &r,
-                     uint32_t *err, dim3 grid, cudaStream_t stream)
+                     uint32_t *err, unsigned pages, cudaStream_t stream)
 {
     const T *kt = reinterpret_cast<const T *>(k), *vt = reinterpret_cast<const T *>(v);
     if (c.D == 128)
-        return launch(kv8_append_kernel<T, 128>, grid, dim3(AP_THREADS), 0, stream, false, c, b, kt, vt, ld, r, err);
-    return launch(kv8_append_kernel<T, 64>, grid, dim3(AP_THREADS), 0, stream, false, c, b, kt, vt, ld, r, err);
+        return append_d<T, 128>(c, b, kt, vt, ld, r, err, pages, stream);
+    return append_d<T, 64>(c, b, kt, vt, ld, r, err, pages, stream);
 }
 
 } // namespace
@@ -196,7 +269,7 @@ int kv8_append(const Kv8 &c, const Kv8Batch &b, const void *k, const void *v, in
 {
     // n rows of one sequence touch at most n pages, and at most n/page + 2
     const long long units = std::min((long long)b.n_rows, (long long)b.n_rows / c.page + 2LL * b.n_seqs);
-    const dim3 grid((unsigned)units, (unsigned)c.n_kv, 2);
+    const unsigned grid = (unsigned)units;
     if (dtype == LLMRS_F32)
         LLMRS_CUDA_TRY(append_t<float>(c, b, k, v, ld, r, err, grid, stream));
     else if (dtype == LLMRS_BF16)
