@@ -50,7 +50,8 @@ constexpr int QT = 256;          // threads of the kernel that prepares Q
 struct ManyTile {
     int row[8];                  // pool rows of the tile's 16-token groups; -1: not there
     float ks[8];                 // key scales
-    float lvs[8];                // log2 of the value scales (-inf: zero)
+    float vs[8];                 // value scales
+    float lvs[8];                // log2 of them, rounded up (-inf: zero)
     int first, last, masked;     // of the pair within this range; some row does not see all tokens
     int tile, s, g, mt;          // which
     int r0, n, len;              // of the sequence
@@ -58,7 +59,7 @@ struct ManyTile {
     int item;                    // number of the pair within this range
     int pad[2];
 };
-static_assert(sizeof(ManyTile) == 160, "16-byte words");
+static_assert(sizeof(ManyTile) == 192, "16-byte words");
 
 struct ManyParams {
     CUtensorMap tq;   // prepared Q: [piece][row][head][D] f16, boxes of 64 dims of a tile's vectors
@@ -211,6 +212,9 @@ __device__ __forceinline__ void tm_st8(uint32_t addr, const uint32_t (&r)[8])
 #undef R8
 #undef T8
 #undef I8
+
+// 2^n, -126 <= n <= 126
+__device__ __forceinline__ float exp2i(int n) { return __int_as_float((n + 127) << 23); }
 
 template <int N>
 __device__ __forceinline__ void regs_up()
@@ -410,7 +414,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                 busy = __any_sync(0xffffffffu, live);
                 fac = live ? p.facs[(size_t)(x.r0 + row) * a.n_heads + x.g * rep + r % rep] : 0.0f;
             }
-            float top = -INFINITY, ref2 = -INFINITY, sum = 0.0f;
+            float top = -INFINITY, sum = 0.0f;
+            int shift = 0; // P is p * vs * 2^shift
             if (busy) {
                 const bool masked = x.masked;
                 if (masked) { // S becomes the scores themselves, the unseen ones at -inf
@@ -433,7 +438,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
                 const float f = masked ? 1.0f : fac;
-                // the row's largest score, and largest score with its value scale
+                // the row's largest score, and a bound of the largest with its value scale
+                float ref2 = -INFINITY;
                 auto most = [&](int g, const uint32_t *s) { // 16 scores of group g
                     float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
@@ -459,33 +465,35 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                         tm_wait(s0);
                     }
                 }
-                // P = p * vs against the row's own largest p * vs of the tile: f16 keeps its bits
-                // whatever the scales of pages that the row hardly sees
+                // P = p * vs, shifted so that the row's largest lies at 2^14: f16 keeps its bits
+                // whatever the scales of pages that the row hardly sees.  p and vs are f32
+                // factors, not one power of two, so P and the sum share p's rounding.
                 const float ref = top == -INFINITY ? 0.0f : top;
-                const bool none = ref2 == -INFINITY; // no seen page has a scale above 0
-                ref2 = none ? 0.0f : ref2 - P_SCALE_LOG2;
+                if (ref2 > -INFINITY) // some seen page has a scale above 0
+                    shift = (int)fminf(fmaxf(P_SCALE_LOG2 - ceilf(ref2 - ref), -126.0f), 126.0f);
                 auto probabilities = [&](int g, const uint32_t *s) { // 16 of them, over the scores of group g
-                    const float lvs = x.lvs[g], kf = masked ? 1.0f : f * x.ks[g];
-                    // a scale of zero: f16 holds the probabilities as zero, the sum keeps them
-                    const bool zero = lvs == -INFINITY;
-                    const float add = zero ? -60.0f - ref : lvs - ref2;
-                    const float back = zero ? 0x1p60f : ex2(fminf(ref2 - lvs - ref, 120.0f));
+                    // where vs * 2^shift alone would overflow (its scores are far below the row's
+                    // largest), 2^up goes to p
+                    const float up = fmaxf(x.lvs[g] + (float)(shift - 60), 0.0f);
+                    const float kf = masked ? 1.0f : f * x.ks[g], add = up - ref;
+                    const float by = x.vs[g] * exp2i(shift - (int)up);
                     float2 g01 = make_float2(0.0f, 0.0f);
                     uint32_t ph[8], pl[8];
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
                         const float2 y = fma2(make_float2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])),
                                               make_float2(kf, kf), make_float2(add, add));
-                        const float e0 = ex2(y.x), e1 = ex2(y.y);
-                        g01 = add2(g01, make_float2(e0, e1));
-                        const uint32_t w = pack16(e0, e1);
+                        const float2 e = make_float2(ex2(y.x), ex2(y.y));
+                        g01 = add2(g01, e);
+                        const float2 o = mul2(e, make_float2(by, by));
+                        const uint32_t w = pack16(o.x, o.y);
                         ph[j / 2] = w;
                         if constexpr (PP == 2) {
                             const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-                            pl[j / 2] = pack16(e0 - h.x, e1 - h.y);
+                            pl[j / 2] = pack16(o.x - h.x, o.y - h.y);
                         }
                     }
-                    sum += (g01.x + g01.y) * back;
+                    sum += up > 0.0f ? (g01.x + g01.y) * ex2(-up) : g01.x + g01.y;
                     tm_st8(sp + 16 * g, ph);
                     if constexpr (PP == 2)
                         tm_st8(sp + 16 * g + 8, pl);
@@ -504,12 +512,11 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                         tm_wait(s0);
                     }
                 }
-                ref2 = none ? -INFINITY : ref2;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             }
             float *hand = ring + (i % RING) * 3 * MB;
             hand[r] = top;
-            hand[MB + r] = ref2;
+            hand[MB + r] = exp2i(-shift);
             hand[2 * MB + r] = sum;
             tc_before();
             mbar_arrive(&bar[B_P_FULL + i % NS]);
@@ -530,14 +537,14 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                 break;
             tc_after();
             const float *hand = ring + (i % RING) * 3 * MB;
-            const float top = hand[r], ref2 = hand[MB + r], sum = hand[2 * MB + r];
+            const float top = hand[r], back = hand[MB + r], sum = hand[2 * MB + r];
             if (x.first) {
                 m = -INFINITY;
                 l = 0.0f;
             }
             const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.0f : mn;
-            const float corr = ex2(m - ref), oscale = ex2(ref2 - ref); // 0 from -inf
-            l = l * corr + sum * ex2(top - ref);
+            const float corr = ex2(m - ref), tile = ex2(top - ref), oscale = tile * back; // 0 from -inf
+            l = l * corr + sum * tile;
             m = mn;
             if (x.first) {
 #pragma unroll
@@ -672,11 +679,11 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                     return;
                 tc_after();
 #pragma unroll
-                for (int c = 0; c < QP; c++)
+                for (int c = QP - 1; c >= 0; c--) // the small pieces first: the accumulator cuts off at every step
 #pragma unroll
                     for (int k = 0; k < D / 64; k++)
                         mma_ss4(tmem + (uint32_t)(i % NS) * MB, sq + ((item % Lay::QS * QP + c) * Lay::T + k * MB * 128) / 16,
-                                sk + (b * Lay::T + k * MB * 128) / 16, QK, c || k);
+                                sk + (b * Lay::T + k * MB * 128) / 16, QK, c < QP - 1 || k);
                 tc_commit(&bar[B_K_EMPTY + b]);
                 if (last)
                     tc_commit(&bar[B_Q_EMPTY + item % Lay::QS]);
@@ -689,11 +696,11 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                     return;
                 tc_after();
 #pragma unroll
-                for (int c = 0; c < PP; c++)
+                for (int c = PP - 1; c >= 0; c--)
 #pragma unroll
                     for (int k = 0; k < 2; k++) // 64 tokens
                         mma_ts4(tmem + NS * MB + (uint32_t)(i % Lay::OS) * D, tmem + (uint32_t)(i % NS) * MB + 64 * k + 8 * c,
-                                sv + (b * Lay::T + k * 64 * 128) / 16, PV, c || k);
+                                sv + (b * Lay::T + k * 64 * 128) / 16, PV, c < PP - 1 || k);
                 tc_commit(&bar[B_V_EMPTY + b]);
                 tc_commit(&bar[B_P_EMPTY + i % NS]);
                 tc_commit(&bar[B_O_FULL + i % Lay::OS]);
@@ -754,7 +761,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                         vs = a.c.vs[o];
                     }
                 }
-                const float lvs = log2f(vs);
+                const float lvs = ceilf(log2f(vs));
                 const bool hole = (__ballot_sync(0xffffffffu, row < 0) >> (8 * q)) & 255u;
                 for (int c = 0; c < 4 && i0 + c < mine && ok; c++) {
                     const int i = i0 + c;
@@ -764,6 +771,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                     if (q == c) {
                         x.row[group] = row;
                         x.ks[group] = ks;
+                        x.vs[group] = vs;
                         x.lvs[group] = lvs;
                         if (group == 0) {
                             x.first = i == 0 || own_tile == 0;
