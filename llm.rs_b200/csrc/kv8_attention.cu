@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(few_warps(NT) * 32, 1) kv8_few_kernel(const __
         __syncwarp();
     };
 
-    const int mine = (int)(hi - lo);
+    int mine = (int)(hi - lo);
     const uint64_t policy = policy_evict_first();
     auto issue = [&](int i, int v) { // lane 0: the K (v = 0) or V codes of tile i into stage i % ST
         const Tile &x = rec[i % Lay::TILES];
@@ -673,8 +673,15 @@ __global__ void __launch_bounds__(few_warps(NT) * 32, 1) kv8_few_kernel(const __
         }
     };
 
-    while (made < min(mine, ST))
-        describe();
+    auto describe_to = [&](int least) { // records of the range's first `least` tiles, at the least
+        while (made < min(mine, least)) {
+            const int before = made;
+            describe();
+            if (made == before) // only if the batch's numbers changed under way
+                mine = made;
+        }
+    };
+    describe_to(ST);
     k_issued = v_issued = min(mine, ST);
     if (lane == 0)
         for (int i = 0; i < k_issued; i++) {
@@ -685,8 +692,7 @@ __global__ void __launch_bounds__(few_warps(NT) * 32, 1) kv8_few_kernel(const __
     int done = 0; // tiles consumed
     for (; done < mine; done++) {
         // records ahead of the loads
-        while (made < mine && made - done <= Lay::TILES - Lay::BATCH)
-            describe();
+        describe_to(done + Lay::TILES - Lay::BATCH + 1);
         const Tile x = rec[done % Lay::TILES];
         if (done == 0 || x.tile == 0) {
             from_start = x.tile == 0;

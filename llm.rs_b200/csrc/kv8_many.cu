@@ -265,7 +265,7 @@ struct Walk {
                 do {
                     s++;
                     kv8_seq(p.a.b, s, p.a.err, r0, n, len);
-                } while ((long long)n * rep <= p.many);
+                } while ((long long)n * rep <= p.many && s + 1 < p.a.b.n_seqs);
             }
         }
         nt = token_tiles(len, n, R, mt);
