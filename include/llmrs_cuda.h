@@ -251,10 +251,12 @@ int llmrs_kv8_read(llmrs_ctx *ctx, const llmrs_kv8 *cache, const int *d_pages, i
  * ld_q / ld_out elements apart, on 16-byte boundaries; query head h reads KV
  * head h / (n_heads/n_kv_heads), any whole ratio.  q is rotated on the way (NULL
  * tables: it is not).  scale multiplies q.k (0: 1/sqrt(head_dim)).  f32 rows are
- * computed to f32 accuracy, 16-bit rows to that of their type.  A row for which
+ * computed to f32 accuracy (against the row's largest values, where the value scales
+ * of pages lie further apart than 2^15), 16-bit rows to that of their type.  A row for which
  * no page can be read gets zeros.  d_workspace: llmrs_kv8_attention_workspace
  * bytes (which depend on the sizes only), 16-byte aligned, contents irrelevant; NULL: the
- * context's scratch (not while capturing). */
+ * context's scratch (not while capturing, and not by calls that may run at the same
+ * time on several streams). */
 int llmrs_kv8_attention_workspace(const llmrs_kv8 *cache, const llmrs_kv8_batch *batch, int n_heads, int n_rows,
                                   size_t *bytes);
 int llmrs_kv8_attention(llmrs_ctx *ctx, const llmrs_kv8 *cache, const llmrs_kv8_batch *batch, const void *d_q,

@@ -43,18 +43,12 @@ __device__ __forceinline__ float finite_or_zero(float x, bool &bad)
 }
 
 // Four codes rint(x * inv).  1.5 * 2^23 added rounds to an integer, to even on a
-// tie like rint, and leaves it in the low byte.  New values need no clamp: |x| is
-// at most 127 s1 (1 + 2^-24) and inv rounds once more, so x * inv stays below
-// 127.0001.  Old codes may be -128 in a cache that another program filled.
-template <bool CLAMP>
+// tie like rint, and leaves it in the low byte.  No clamp: a new |x| is at most
+// 127 s1 (1 + 2^-24) and inv rounds once more, so x * inv stays below 127.0001;
+// an old code is multiplied by less than one.
 __device__ __forceinline__ uint32_t code4(float4 x, float inv)
 {
-    auto code = [&](float v) {
-        v = __fmul_rn(v, inv);
-        if constexpr (CLAMP)
-            v = fminf(fmaxf(v, -127.0f), 127.0f);
-        return __float_as_uint(__fadd_rn(v, 12582912.0f));
-    };
+    auto code = [&](float v) { return __float_as_uint(__fadd_rn(__fmul_rn(v, inv), 12582912.0f)); };
     const uint32_t a = __byte_perm(code(x.x), code(x.y), 0x0040), c = __byte_perm(code(x.z), code(x.w), 0x0040);
     return __byte_perm(a, c, 0x5410);
 }
@@ -183,8 +177,8 @@ __global__ void __launch_bounds__(AP_THREADS) kv8_append_kernel(Kv8 c, Kv8Batch 
             if (again)
                 row(i, lo[u], hi[u]);
             int8_t *dst = codes + (size_t)(held + i) * D;
-            *reinterpret_cast<uint32_t *>(dst + 4 * j) = code4<false>(lo[u], inv);
-            *reinterpret_cast<uint32_t *>(dst + D / 2 + 4 * j) = code4<false>(hi[u], inv);
+            *reinterpret_cast<uint32_t *>(dst + 4 * j) = code4(lo[u], inv);
+            *reinterpret_cast<uint32_t *>(dst + D / 2 + 4 * j) = code4(hi[u], inv);
         }
     }
     if (s1 > s0 && held) {
@@ -196,7 +190,7 @@ __global__ void __launch_bounds__(AP_THREADS) kv8_append_kernel(Kv8 c, Kv8Batch 
             uint32_t y[4];
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                y[e] = code4<true>(make_float4(o[e].x, o[e].y, o[e].z, o[e].w), ratio);
+                y[e] = code4(make_float4(o[e].x, o[e].y, o[e].z, o[e].w), ratio);
             reinterpret_cast<uint4 *>(codes)[w] = make_uint4(y[0], y[1], y[2], y[3]);
         }
     }
