@@ -5,7 +5,8 @@
 //   S = Q K^T (128 x 128, K = D), P = exp2(S * ks - max) * vs, O = P V,
 // f16 operands, f32 accumulators in TMEM.  The codes are exact in f16.  f32
 // rows: Q and P are two f16 pieces each (22 bits and more), so the products
-// run twice; f16 rows: Q in two pieces, P in one; bf16 rows: one each.  Every
+// run twice; f16 rows too (with P in one piece they are 1.4 times as far off as
+// the rounding of the result); bf16 rows: one each.  Every
 // tile's O is a fresh product that registers add up in f32, with the change of
 // the maximum and the value scales applied there: long sums do not pass
 // through the tensor core's accumulator.
@@ -962,9 +963,9 @@ int kv8_many_prepare(void)
     if (e == cudaSuccess)
         e = prepare<float, 64, 2, 2>();
     if (e == cudaSuccess)
-        e = prepare<__half, 128, 2, 1>();
+        e = prepare<__half, 128, 2, 2>();
     if (e == cudaSuccess)
-        e = prepare<__half, 64, 2, 1>();
+        e = prepare<__half, 64, 2, 2>();
     if (e == cudaSuccess)
         e = prepare<__nv_bfloat16, 128, 1, 1>();
     if (e == cudaSuccess)
@@ -987,7 +988,7 @@ int kv8_many(const Kv8Attn &a, int many, void *ws, int sms, cudaStream_t stream)
     if (a.dtype == LLMRS_F32)
         return a.c.D == 128 ? run<float, 128, 2, 2>(p, ctas, stream) : run<float, 64, 2, 2>(p, ctas, stream);
     if (a.dtype == LLMRS_F16)
-        return a.c.D == 128 ? run<__half, 128, 2, 1>(p, ctas, stream) : run<__half, 64, 2, 1>(p, ctas, stream);
+        return a.c.D == 128 ? run<__half, 128, 2, 2>(p, ctas, stream) : run<__half, 64, 2, 2>(p, ctas, stream);
     return a.c.D == 128 ? run<__nv_bfloat16, 128, 1, 1>(p, ctas, stream)
                         : run<__nv_bfloat16, 64, 1, 1>(p, ctas, stream);
 }
