@@ -23,12 +23,14 @@
 // tile i - 1 runs and the scores of tile i + 2 are made.  K and V are double
 // buffered, Q too but for two pieces of 128 dims.
 //
-// What a tile costs is not a product's 1000 cycles but the longest of the roles'
-// chains, whose instructions take 4 to 5 cycles each: so each role that was the
-// longest got a second warpgroup or a kernel of its own, and each keeps its next
-// loads (TMEM columns, codes) in flight while it works.  Two prompts of 4000 rows,
-// bf16, 32 heads of 128 over 8: 740 us with one softmax, one widening and one Q
-// warpgroup.
+// What a tile costs is not its products' 1000 cycles but the roles' chains, whose
+// instructions take 4 to 5 cycles each: so each role that was the longest got a
+// second warpgroup or a kernel of its own, and each keeps its next loads (TMEM
+// columns, codes) in flight while it works.  Two prompts of 3500 to 4096 rows,
+// bf16, 32 heads of 128 over 8: 495 us (494 TFLOP/s; 740 us with one softmax, one
+// widening and one Q warpgroup), chunks of 3 prompts of 1000 rows behind 0 to 3000
+// tokens, f32: 272 us.  Left: a tile takes 3400 to 3900 cycles, and no role is at
+// work for more than 3200 of them.
 //
 // Work: the tiles of all (sequence, KV head, tile of rows) in one row, cut into
 // equal consecutive ranges, one per CTA; pieces of a softmax that a range cuts
