@@ -27,10 +27,11 @@
 // instructions take 4 to 5 cycles each: so each role that was the longest got a
 // second warpgroup or a kernel of its own, and each keeps its next loads (TMEM
 // columns, codes) in flight while it works.  Two prompts of 3500 to 4096 rows,
-// bf16, 32 heads of 128 over 8: 495 us (494 TFLOP/s; 740 us with one softmax, one
+// bf16, 32 heads of 128 over 8: 493 us (496 TFLOP/s; 740 us with one softmax, one
 // widening and one Q warpgroup), chunks of 3 prompts of 1000 rows behind 0 to 3000
-// tokens, f32: 272 us.  Left: a tile takes 3400 to 3900 cycles, and no role is at
-// work for more than 3200 of them.
+// tokens, f32: 265 us.  Left: 3400 to 3900 cycles a tile, spread over all roles:
+// without any softmax it would be 394 us, without widening 454, without the
+// output's sums 471.
 //
 // Work: the tiles of all (sequence, KV head, tile of rows) in one row, cut into
 // equal consecutive ranges, one per CTA; pieces of a softmax that a range cuts
@@ -218,6 +219,17 @@ __device__ __forceinline__ void tm_st8(uint32_t addr, const uint32_t (&r)[8])
 
 // 2^n, -126 <= n <= 126
 __device__ __forceinline__ float exp2i(int n) { return __int_as_float((n + 127) << 23); }
+
+// whether a barrier's phase is over, without waiting
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok)
+                 : "r"(smem_addr(bar)), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
 
 template <int N>
 __device__ __forceinline__ void regs_up()
@@ -673,13 +685,13 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
             const uint32_t sq = sw128(smem_addr(smem), 16), sk = sw128(smem_addr(smem + Lay::k_off), 16),
                            sv = sw128(smem_addr(smem + Lay::v_off), MB * 128);
             int item = -1;
+            auto test = [&](int b, int use) { return __all_sync(0xffffffffu, mbar_test(&bar[b], (uint32_t)(use & 1))); };
             auto qk = [&](int i, bool first, bool last) {
-                item += first;
                 const int b = i % Lay::KVS;
                 // S lies under the P of tile i - NS, which that tile's product has read
-                if (!(ok = (!first || wait(B_Q_FULL + item % Lay::QS, item / Lay::QS)) && wait(B_K_FULL + b, i / Lay::KVS) &&
-                           (i < NS || wait(B_P_EMPTY + i % NS, i / NS - 1))))
-                    return;
+                if (!((!first || test(B_Q_FULL + item % Lay::QS, item / Lay::QS)) && test(B_K_FULL + b, i / Lay::KVS) &&
+                      (i < NS || test(B_P_EMPTY + i % NS, i / NS - 1))))
+                    return false;
                 tc_after();
 #pragma unroll
                 for (int c = QP - 1; c >= 0; c--) // the small pieces first: the accumulator cuts off at every step
@@ -691,12 +703,13 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                 if (last)
                     tc_commit(&bar[B_Q_EMPTY + item % Lay::QS]);
                 tc_commit(&bar[B_S_FULL + i % NS]);
+                return true;
             };
             auto pv = [&](int i) {
                 const int b = i % Lay::KVS;
-                if (!(ok = wait(B_P_FULL + i % NS, i / NS) && wait(B_V_FULL + b, i / Lay::KVS) &&
-                           (i < Lay::OS || wait(B_O_EMPTY + i % Lay::OS, i / Lay::OS - 1))))
-                    return;
+                if (!(test(B_P_FULL + i % NS, i / NS) && test(B_V_FULL + b, i / Lay::KVS) &&
+                      (i < Lay::OS || test(B_O_EMPTY + i % Lay::OS, i / Lay::OS - 1))))
+                    return false;
                 tc_after();
 #pragma unroll
                 for (int c = PP - 1; c >= 0; c--)
@@ -707,20 +720,42 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                 tc_commit(&bar[B_V_EMPTY + b]);
                 tc_commit(&bar[B_P_EMPTY + i % NS]);
                 tc_commit(&bar[B_O_FULL + i % Lay::OS]);
+                return true;
             };
+            // whichever is ready: the scores of tile iq, the output of tile ip
+            int iq = 0, ip = 0;
+            bool known = false, first = false, last = false;
+            uint32_t left = 1u << 22; // polls without either
 #pragma unroll 1
-            for (int i = 0; i < mine + 2 && ok; i++) { // the scores of tile i, then the output of tile i - 2
-                if (i < mine) {
-                    if (!(ok = wait(B_INFO_FULL + i % INFO, i / INFO)))
-                        break;
-                    const bool first = __shfl_sync(0xffffffffu, info[i % INFO].first, 0);
-                    const bool last = __shfl_sync(0xffffffffu, info[i % INFO].last, 0);
-                    if (lane == 0)
-                        mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
-                    qk(i, first, last);
+            while (ip < mine && ok) {
+                bool did = false;
+                if (iq < mine) {
+                    if (!known && test(B_INFO_FULL + iq % INFO, iq / INFO)) {
+                        first = __shfl_sync(0xffffffffu, info[iq % INFO].first, 0);
+                        last = __shfl_sync(0xffffffffu, info[iq % INFO].last, 0);
+                        if (lane == 0)
+                            mbar_arrive(&bar[B_INFO_EMPTY + iq % INFO]);
+                        item += first;
+                        known = true;
+                    }
+                    if (known && qk(iq, first, last)) {
+                        iq++;
+                        known = false;
+                        did = true;
+                    }
                 }
-                if (ok && i > 1)
-                    pv(i - 2);
+                if (ip < iq && pv(ip)) {
+                    ip++;
+                    did = true;
+                }
+                if (did)
+                    left = 1u << 22;
+                else if (--left == 0) {
+                    atomicCAS(a.err, 0u, (uint32_t)DEV_ERR_MBAR_TIMEOUT);
+                    ok = false;
+                } else {
+                    __nanosleep(20);
+                }
             }
             // every arrival lands before the barriers go
             const int b = (mine - 1) % Lay::KVS, use = (mine - 1) / Lay::KVS;
