@@ -41,10 +41,6 @@ __device__ __forceinline__ uint32_t pack16(float a, float b)
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-
 // N (a multiple of 16/sizeof(T) ... 16) consecutive floats to a row of T
 template <int N>
 __device__ __forceinline__ void store_row(float *p, const float (&x)[N])

@@ -6,10 +6,9 @@
 // f16 operands, f32 accumulators in TMEM.  The codes are exact in f16.  f32
 // rows: Q and P are two f16 pieces each (22 bits and more), so the products
 // run twice; f16 rows too (with P in one piece they are 1.4 times as far off as
-// the rounding of the result); bf16 rows: one each.  Every
-// tile's O is a fresh product that registers add up in f32, with the change of
-// the maximum and the value scales applied there: long sums do not pass
-// through the tensor core's accumulator.
+// the rounding of the result); bf16 rows: one each.  Every tile's O is a fresh
+// product that registers add up in f32, with the change of the maximum applied
+// there: long sums do not pass through the tensor core's accumulator.
 //
 // Warpgroups: 0 and 4 softmax of every other tile (thread = row), 1 output
 // (thread = row, D accumulators), 2 and 5 key and value codes to f16 in shared
@@ -47,7 +46,9 @@ namespace {
 constexpr int MB = 128;          // vectors, and tokens, of a tile
 constexpr int MANY_THREADS = 768;
 constexpr int INFO = 8;          // tile descriptions in flight
-constexpr int RING = 6;          // softmax -> output hand-overs in flight
+// softmax -> output hand-overs in flight: the scores of tile i wait for the product of
+// tile i - NS, and that for the output to have taken one or two tiles before it
+constexpr int RING = 6;
 constexpr int NS = 3;            // buffers of S
 constexpr int QT = 256;          // threads of the kernel that prepares Q
 
@@ -303,7 +304,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
     extern __shared__ __align__(128) uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     ManyTile *info = reinterpret_cast<ManyTile *>(smem + Lay::info_off);
-    float *ring = reinterpret_cast<float *>(smem + Lay::ring_off); // [RING][change of max | scale of O | sum | max][MB]
+    float *ring = reinterpret_cast<float *>(smem + Lay::ring_off); // [RING][maximum | scale of O | sum][MB]
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + Lay::bar_off);
     __shared__ uint32_t s_tmem;
     __shared__ long long s_sum[MANY_THREADS / 32];
