@@ -266,10 +266,12 @@ int llmrs_kv8_attention(llmrs_ctx *ctx, const llmrs_kv8 *cache, const llmrs_kv8_
 
 /* Verify drafted tokens.  Sequence s has rows [d_row_start[s], d_row_start[s+1])
  * of target logits: one for each of its drafts and one behind them (one row:
- * plain sampling; no rows: nothing but d_accepted[s] = 0).  d_draft_tokens holds
- * the drafts of all sequences packed (one fewer than the rows of each sequence
- * that has rows), d_draft_probs [drafts][ld_probs] the f32 distributions they
- * were drawn from (NULL: each draft was certain, e.g. found by lookup).  With
+ * plain sampling; no rows: nothing but d_accepted[s] = 0).  d_draft_tokens [n_drafts]
+ * holds the drafts of all sequences packed (one fewer than the rows of each sequence
+ * that has rows), d_draft_probs [n_drafts][ld_probs] the f32 distributions they
+ * were drawn from (NULL: each draft was certain, e.g. found by lookup).  Both may be
+ * longer than the row starts say; a sequence whose drafts would lie behind their end
+ * counts as one whose rows do not fit.  With
  * p = softmax(logits / temperature), draft i is accepted while
  *   u[row i] * q_i(d_i) < p_i(d_i),
  * and the next token is drawn with u[last row] from max(p - q, 0) of the first
@@ -282,6 +284,14 @@ int llmrs_kv8_attention(llmrs_ctx *ctx, const llmrs_kv8 *cache, const llmrs_kv8_
  * then the next token, then -1; d_accepted[n_seqs]; d_token_probs[rows] (may be
  * NULL) p of each token given out, 0 behind them. */
 int llmrs_verify_draft_workspace(int n_rows, int vocab, size_t *bytes);
+int llmrs_verify_draft_counted(llmrs_ctx *ctx, const void *d_logits, long long ld_logits, int dtype, int vocab,
+                               int n_rows, int n_seqs, const int *d_row_start, const int *d_draft_tokens,
+                               const float *d_draft_probs, long long ld_probs, int n_drafts, const float *d_uniforms,
+                               const float *d_temperature, int *d_tokens, int *d_accepted, float *d_token_probs,
+                               void *d_workspace, size_t workspace_bytes);
+/* The same for buffers of n_rows - 1 drafts and distributions at the least: as many as
+ * any row starts that fit n_rows can ask for (NULL d_draft_tokens: none; refused for more
+ * rows than sequences). */
 int llmrs_verify_draft(llmrs_ctx *ctx, const void *d_logits, long long ld_logits, int dtype, int vocab, int n_rows,
                        int n_seqs, const int *d_row_start, const int *d_draft_tokens, const float *d_draft_probs,
                        long long ld_probs, const float *d_uniforms, const float *d_temperature, int *d_tokens,

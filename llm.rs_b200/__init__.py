@@ -44,7 +44,7 @@ EXPORTS = [
     "llmrs_attention_decode", "llmrs_attention_decode_noalloc", "llmrs_attention_prefill",
     "llmrs_sample", "llmrs_model_sample", "llmrs_model_trace_decode",
     "llmrs_kv8_append", "llmrs_kv8_read", "llmrs_kv8_attention", "llmrs_kv8_attention_workspace",
-    "llmrs_verify_draft", "llmrs_verify_draft_workspace",
+    "llmrs_verify_draft", "llmrs_verify_draft_counted", "llmrs_verify_draft_workspace",
     "llmrs_model_tp_region", "llmrs_model_tp_connect", "llmrs_ipc_get_handle", "llmrs_ipc_open_handle",
     "llmrs_ipc_close_handle", "llmrs_model_set_peer_timeout", "llmrs_model_tp_epoch", "llmrs_model_tp_resync",
 ]
@@ -163,6 +163,7 @@ def lib():
         "llmrs_kv8_attention": (ci, [vp, vp, vp, vp, cl, vp, cl, ci, ci, ci, vp, vp, ci, cf, vp, sz]),
         "llmrs_verify_draft_workspace": (ci, [ci, ci, ctypes.POINTER(sz)]),
         "llmrs_verify_draft": (ci, [vp, vp, cl, ci, ci, ci, ci, vp, vp, vp, cl, vp, vp, vp, vp, vp, vp, sz]),
+        "llmrs_verify_draft_counted": (ci, [vp, vp, cl, ci, ci, ci, ci, vp, vp, vp, cl, ci, vp, vp, vp, vp, vp, vp, sz]),
         "llmrs_model_tp_region": (ci, [vp, pp, ctypes.POINTER(sz)]),
         "llmrs_model_tp_connect": (ci, [vp, pp]),
         "llmrs_ipc_get_handle": (ci, [vp, vp]),
@@ -576,7 +577,7 @@ class CudaBackend:
 
     def verify_draft(self, logits, row_start, draft_tokens, draft_probs, uniforms, tokens, accepted, token_probs=None,
                      temperature=None, workspace=None):
-        """Verify drafted tokens (llmrs_verify_draft): logits [n, vocab]; row_start int32
+        """Verify drafted tokens (llmrs_verify_draft_counted): logits [n, vocab]; row_start int32
         [seqs+1]; draft_tokens int32 and draft_probs f32 [drafts, vocab] (or None: certain
         drafts), packed; uniforms f32 [n].  Writes tokens int32 [n], accepted int32
         [seqs] and token_probs f32 [n]."""
@@ -595,10 +596,10 @@ class CudaBackend:
             raise ValueError("verify_draft: token_probs must be [%d]" % n)
         if temperature is not None and tuple(temperature.shape) != (n_seqs,):
             raise ValueError("verify_draft: temperature must be [%d]" % n_seqs)
-        some = draft_tokens is not None and draft_tokens.shape[0] > 0
-        check(lib().llmrs_verify_draft(
+        n_drafts = 0 if draft_tokens is None else draft_tokens.shape[0]
+        check(lib().llmrs_verify_draft_counted(
             self.ctx.h, lp, ld, lt, vocab, n, n_seqs, _array(row_start, _INT32, "row_start"),
-            _array(draft_tokens, _INT32, "draft_tokens") if some else None, qp, qld,
+            _array(draft_tokens, _INT32, "draft_tokens") if n_drafts else None, qp, qld, n_drafts,
             _array(uniforms, _F32, "uniforms"),
             None if temperature is None else _array(temperature, _F32, "temperature"),
             _array(tokens, _INT32, "tokens"), _array(accepted, _INT32, "accepted"),

@@ -750,14 +750,28 @@ int llmrs_verify_draft(llmrs_ctx *ctx, const void *d_logits, long long ld_logits
                        long long ld_probs, const float *d_uniforms, const float *d_temperature, int *d_tokens,
                        int *d_accepted, float *d_token_probs, void *d_workspace, size_t workspace_bytes)
 {
+    const int n_drafts = d_draft_tokens && n_rows > 0 ? n_rows - 1 : 0;
+    LLMRS_CHECK_ARG(n_rows <= n_seqs || d_draft_tokens, "verify_draft: no drafted tokens for %d rows of %d sequences",
+                    n_rows, n_seqs);
+    return llmrs_verify_draft_counted(ctx, d_logits, ld_logits, dtype, vocab, n_rows, n_seqs, d_row_start, d_draft_tokens,
+                                      d_draft_probs, ld_probs, n_drafts, d_uniforms, d_temperature, d_tokens, d_accepted,
+                                      d_token_probs, d_workspace, workspace_bytes);
+}
+
+int llmrs_verify_draft_counted(llmrs_ctx *ctx, const void *d_logits, long long ld_logits, int dtype, int vocab,
+                               int n_rows, int n_seqs, const int *d_row_start, const int *d_draft_tokens,
+                               const float *d_draft_probs, long long ld_probs, int n_drafts, const float *d_uniforms,
+                               const float *d_temperature, int *d_tokens, int *d_accepted, float *d_token_probs,
+                               void *d_workspace, size_t workspace_bytes)
+{
     LLMRS_CHECK_ARG(known_dtype(dtype), "verify_draft: dtype %d unknown", dtype);
     LLMRS_CHECK_ARG(vocab > 0 && n_rows >= 0 && n_rows <= 65535 && n_seqs >= 0 && n_seqs <= 65535,
                     "verify_draft: vocab %d, n_rows %d, n_seqs %d (at most 65535 rows)", vocab, n_rows, n_seqs);
     LLMRS_CHECK_ARG(n_seqs == 0 || (d_row_start && d_accepted), "verify_draft: NULL argument");
     LLMRS_CHECK_ARG(n_seqs == 0 || n_rows == 0 || (d_logits && d_uniforms && d_tokens),
                     "verify_draft: NULL argument");
-    LLMRS_CHECK_ARG(n_rows <= n_seqs || d_draft_tokens, "verify_draft: no drafted tokens for %d rows of %d sequences",
-                    n_rows, n_seqs);
+    LLMRS_CHECK_ARG(n_drafts >= 0 && (n_drafts == 0 || d_draft_tokens), "verify_draft: n_drafts %d, d_draft_tokens %p",
+                    n_drafts, (const void *)d_draft_tokens);
     LLMRS_CHECK_ARG(ld_logits >= vocab && (!d_draft_probs || ld_probs >= vocab),
                     "verify_draft: row strides %lld, %lld shorter than the vocabulary", ld_logits, ld_probs);
     LLMRS_CHECK_ARG(ctx, "verify_draft: ctx is NULL");
@@ -773,6 +787,7 @@ int llmrs_verify_draft(llmrs_ctx *ctx, const void *d_logits, long long ld_logits
     p.vocab = vocab;
     p.n_rows = n_rows;
     p.n_seqs = n_seqs;
+    p.n_drafts = n_drafts;
     p.row_start = d_row_start;
     p.draft = d_draft_tokens;
     p.q = d_draft_probs;

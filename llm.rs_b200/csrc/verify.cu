@@ -288,14 +288,14 @@ __global__ void __launch_bounds__(PT, 2) verify_pick_kernel(VerifyParams p, cons
         in_front += __syncthreads_count(rows > 0);
         rising = !__syncthreads_or(rows < 0) && rising;
     }
-    if (!rising) {
+    const int k = n - 1, d0 = r0 - p.row_start[0] - in_front; // drafts and their first place
+    if (!rising || (k > 0 && d0 + k > p.n_drafts)) { // or more drafts than there are
         if (rank == 0 && threadIdx.x == 0) {
             p.accepted[seq] = 0;
             atomicCAS(p.err, 0u, (uint32_t)DEV_ERR_BAD_BATCH);
         }
         return;
     }
-    const int k = n - 1, d0 = r0 - p.row_start[0] - in_front; // drafts and their first place
     const float T_ = p.temperature ? p.temperature[seq] : 1.0f;
     const bool greedy = !(T_ > 0.0f);
     const double inv = greedy ? 1.0 : 1.0 / (double)T_;

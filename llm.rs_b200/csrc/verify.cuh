@@ -11,9 +11,10 @@ struct VerifyParams {
     const void *logits;       // [n_rows][ld]
     long long ld;
     int dtype, vocab, n_rows, n_seqs;
+    int n_drafts;             // entries of draft, rows of q
     const int *row_start;     // [n_seqs + 1]
-    const int *draft;         // [drafts], packed: one fewer than the rows of each sequence
-    const float *q;           // [drafts][ldq] the drafting model's probabilities; nullptr: each draft was certain
+    const int *draft;         // [n_drafts], packed: one fewer than the rows of each sequence
+    const float *q;           // [n_drafts][ldq] the drafting model's probabilities; nullptr: each draft was certain
     long long ldq;
     const float *u;           // [n_rows] uniform draws
     const float *temperature; // [n_seqs] or nullptr (1)

@@ -169,6 +169,12 @@ extern "C" {
                               d_uniforms: *const f32, d_temperature: *const f32, d_tokens: *mut c_int,
                               d_accepted: *mut c_int, d_token_probs: *mut f32, d_workspace: *mut c_void,
                               workspace_bytes: usize) -> c_int;
+    pub fn llmrs_verify_draft_counted(ctx: *mut llmrs_ctx, d_logits: *const c_void, ld_logits: c_longlong, dtype: c_int,
+                                      vocab: c_int, n_rows: c_int, n_seqs: c_int, d_row_start: *const c_int,
+                                      d_draft_tokens: *const c_int, d_draft_probs: *const f32, ld_probs: c_longlong,
+                                      n_drafts: c_int, d_uniforms: *const f32, d_temperature: *const f32,
+                                      d_tokens: *mut c_int, d_accepted: *mut c_int, d_token_probs: *mut f32,
+                                      d_workspace: *mut c_void, workspace_bytes: usize) -> c_int;
 
     // ---- model: device-resident weights + KV cache, fused token loop ----
     pub fn llmrs_model_create(ctx: *mut llmrs_ctx, cfg: *const llmrs_config, out: *mut *mut llmrs_model) -> c_int;

@@ -1,0 +1,62 @@
+"""Verification of drafted tokens where its inputs are at their ends: fewer drafts than the
+row starts ask for, none at all."""
+import numpy as np
+import pytest
+
+import serving_oracle as S
+from test_gpu_verify import check, make, run
+
+pytestmark = pytest.mark.gpu
+
+
+def _reported(llmrs, ctx, word):
+    with pytest.raises(llmrs.LlmrsError) as e:
+        ctx.sync()
+    assert e.value.code == llmrs.EDEVICE and "word %d" % word in str(e.value)
+    ctx.sync()  # reported once
+
+
+@pytest.mark.parametrize("probs", [True, False])
+@pytest.mark.parametrize("row_start,have,short", [
+    ([0, 10, 10, 10, 10, 10], 5, [0]),     # nine drafts in one sequence, room for one of each of five
+    ([0, 3, 3, 6, 10], 3, [2, 3]),         # the first two sequences' drafts are there
+    ([0, 0, 0, 0, 3], 0, [3]),             # none at all
+    ([0, 4, 5, 6], 2, [0])])               # what is behind a short sequence without drafts is drawn
+def test_verify_drafts_that_are_not_there(llmrs, ctx, be, row_start, have, short, probs):
+    c = make(50, 700, [k - 1 for k in np.diff(row_start)], probs=probs)
+    assert c["row_start"].tolist() == row_start
+    c["draft"] = c["draft"][:have].copy()
+    if probs:
+        c["q"] = c["q"][:have].copy()
+        if have == 0:
+            c["q"] = None
+    tokens, accepted, out = run(llmrs, ctx, be, c)
+    _reported(llmrs, ctx, 5)
+    for s, (a, b) in enumerate(zip(row_start, row_start[1:])):
+        if s in short:
+            assert accepted[s] == 0 and np.all(tokens[a:b] == 777) and np.all(out[a:b] == 777)
+    # the others as if the short ones had no rows
+    whole = make(50, 700, [k - 1 for k in np.diff(row_start)], probs=probs)
+    want, count, p, margin = S.verify(whole["logits"], whole["row_start"], whole["draft"], whole["q"], whole["u"], whole["heats"])
+    for s, (a, b) in enumerate(zip(row_start, row_start[1:])):
+        if s not in short:
+            assert margin[s].min() > 1e-4  # no draw of this input lies on a border
+            assert accepted[s] == count[s] and np.array_equal(tokens[a:b], want[a:b])
+            assert np.all(np.abs(out[a:b] - p[a:b]) <= 2.0 ** -18 * p[a:b])
+
+
+def test_verify_plain_sampling_with_rows_behind_the_last_sequence(llmrs, ctx, be):
+    """More rows than sequences and no drafts: the spare rows belong to nobody."""
+    c = make(51, 900, [0, 0, -1, 0])
+    for name, value in (("raw", np.nan), ("logits", np.nan), ("u", 0.5)):
+        c[name] = np.concatenate([c[name], np.full((4,) + c[name].shape[1:], value, np.float32)])
+    c["q"] = None
+    assert check(llmrs, ctx, be, c) == 4
+    ctx.sync()
+    T = llmrs.DeviceTensor.from_numpy
+    tokens, accepted = T(ctx, np.full(7, 777, np.int32)), T(ctx, np.full(4, 777, np.int32))
+    be.verify_draft(T(ctx, c["raw"]), T(ctx, c["row_start"]), None, None, T(ctx, c["u"]), tokens, accepted)
+    ctx.sync()
+    want = S.verify(c["logits"], c["row_start"], c["draft"], None, c["u"], None)[0]
+    assert np.array_equal(tokens.numpy()[:3], want[:3]) and np.all(tokens.numpy()[3:] == 777)
+    assert np.all(accepted.numpy() == 0)
