@@ -282,7 +282,8 @@ int llmrs_kv8_attention(llmrs_ctx *ctx, const llmrs_kv8 *cache, const llmrs_kv8_
  * without any yields token -1 and accepts nothing.  A draft outside the vocabulary is
  * rejected and reported by llmrs_sync.  Out: d_tokens[rows] the accepted drafts,
  * then the next token, then -1; d_accepted[n_seqs]; d_token_probs[rows] (may be
- * NULL) p of each token given out, 0 behind them. */
+ * NULL) p of each token given out, 0 behind them.  At most 65535 rows and sequences,
+ * and 2^30 tokens. */
 int llmrs_verify_draft_workspace(int n_rows, int vocab, size_t *bytes);
 int llmrs_verify_draft_counted(llmrs_ctx *ctx, const void *d_logits, long long ld_logits, int dtype, int vocab,
                                int n_rows, int n_seqs, const int *d_row_start, const int *d_draft_tokens,

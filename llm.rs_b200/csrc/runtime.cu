@@ -740,7 +740,8 @@ int llmrs_kv8_attention(llmrs_ctx *ctx, const llmrs_kv8 *cache, const llmrs_kv8_
 
 int llmrs_verify_draft_workspace(int n_rows, int vocab, size_t *bytes)
 {
-    LLMRS_CHECK_ARG(bytes && n_rows >= 0 && vocab > 0, "verify_draft_workspace: bad arguments");
+    LLMRS_CHECK_ARG(bytes && n_rows >= 0 && vocab > 0 && vocab <= VERIFY_MAX_VOCAB,
+                    "verify_draft_workspace: bad arguments");
     *bytes = verify_workspace(n_rows, vocab);
     return LLMRS_OK;
 }
@@ -765,8 +766,10 @@ int llmrs_verify_draft_counted(llmrs_ctx *ctx, const void *d_logits, long long l
                                void *d_workspace, size_t workspace_bytes)
 {
     LLMRS_CHECK_ARG(known_dtype(dtype), "verify_draft: dtype %d unknown", dtype);
-    LLMRS_CHECK_ARG(vocab > 0 && n_rows >= 0 && n_rows <= 65535 && n_seqs >= 0 && n_seqs <= 65535,
-                    "verify_draft: vocab %d, n_rows %d, n_seqs %d (at most 65535 rows)", vocab, n_rows, n_seqs);
+    LLMRS_CHECK_ARG(vocab > 0 && vocab <= VERIFY_MAX_VOCAB && n_rows >= 0 && n_rows <= 65535 && n_seqs >= 0 &&
+                        n_seqs <= 65535,
+                    "verify_draft: vocab %d, n_rows %d, n_seqs %d (at most 2^30 tokens, 65535 rows)", vocab, n_rows,
+                    n_seqs);
     LLMRS_CHECK_ARG(n_seqs == 0 || (d_row_start && d_accepted), "verify_draft: NULL argument");
     LLMRS_CHECK_ARG(n_seqs == 0 || n_rows == 0 || (d_logits && d_uniforms && d_tokens),
                     "verify_draft: NULL argument");

@@ -24,6 +24,9 @@ struct VerifyParams {
     uint32_t *err;
 };
 
+// tokens are counted in 32 bits, in steps that reach some thousands past the last one
+constexpr int VERIFY_MAX_VOCAB = 1 << 30;
+
 size_t verify_workspace(int n_rows, int vocab);
 // set kernel attributes on the current device (once per context, outside capture)
 int verify_prepare(void);

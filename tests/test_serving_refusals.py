@@ -1,8 +1,6 @@
 """What the serving operators' entries refuse before any GPU work (on the CPU)."""
 import ctypes
 
-import pytest
-
 
 def _refused(llmrs, rc, words):
     assert rc == llmrs.EINVAL
@@ -27,3 +25,13 @@ def test_counted_drafts_are_checked(llmrs):
     _refused(llmrs, _verify(llmrs, E, ldq=99), "strides")
     _refused(llmrs, _verify(llmrs, "llmrs_verify_draft", draft=None), "no drafted tokens")
     _refused(llmrs, _verify(llmrs, "llmrs_verify_draft", draft=None, n=1), "ctx is NULL")
+
+
+def test_vocabularies_past_32_bit_steps_are_refused(llmrs):
+    n = ctypes.c_size_t(0)
+    for vocab in ((1 << 30) + 1, (1 << 31) - 8192, (1 << 31) - 1):
+        for entry in ("llmrs_verify_draft", "llmrs_verify_draft_counted"):
+            _refused(llmrs, _verify(llmrs, entry, vocab=vocab, ld=1 << 31, ldq=1 << 31), "vocab")
+        _refused(llmrs, llmrs.lib().llmrs_verify_draft_workspace(5, vocab, ctypes.byref(n)), "bad arguments")
+    assert llmrs.lib().llmrs_verify_draft_workspace(5, 1 << 30, ctypes.byref(n)) == llmrs.OK
+    assert n.value >= 5 * (1 << 30) // 8192 * 16
