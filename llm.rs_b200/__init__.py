@@ -325,20 +325,33 @@ def _address(x):
     return x.ptr.value if isinstance(x, DeviceTensor) else x.data_ptr()
 
 
-def _array(x, kinds, what):
-    """Address of a contiguous array of one of the element types `kinds`."""
+def _device(x):
+    """Index of the GPU that holds a DeviceTensor or a torch tensor; -1: host memory."""
+    return x.ctx.device if isinstance(x, DeviceTensor) else x.get_device()
+
+
+def _elsewhere(x, what, device):
+    return ValueError("%s: on %s, not on GPU %d" % (what, "the host" if _device(x) < 0 else "GPU %d" % _device(x), device))
+
+
+def _array(x, kinds, what, device):
+    """Address of a contiguous array of one of the element types `kinds` on GPU `device`."""
     if x.dtype not in kinds:
         _learn_torch(x.dtype, kinds, what)
     if isinstance(x, DeviceTensor):
+        if x.ctx.device != device:
+            raise _elsewhere(x, what, device)
         return x.ptr.value
+    if x.get_device() != device:
+        raise _elsewhere(x, what, device)
     if not x.is_contiguous():
         raise ValueError("%s must be contiguous" % what)
     return x.data_ptr()
 
 
-def _rows(x, width, what):
-    """(address, dtype code, rows, row stride) of rows of `width` elements: [n, width]
-    or [n, heads, D], the elements of a row next to each other."""
+def _rows(x, width, what, device):
+    """(address, dtype code, rows, row stride) of rows of `width` elements on GPU `device`:
+    [n, width] or [n, heads, D], the elements of a row next to each other."""
     kind = _DTYPES.get(x.dtype)
     if kind is None:
         kind = _learn_torch(x.dtype, _DTYPES, what)
@@ -347,7 +360,11 @@ def _rows(x, width, what):
     if size != width:
         raise ValueError("%s: rows of %d elements, not %d" % (what, size, width))
     if isinstance(x, DeviceTensor):
+        if x.ctx.device != device:
+            raise _elsewhere(x, what, device)
         return x.ptr.value, kind, n, width
+    if x.get_device() != device:
+        raise _elsewhere(x, what, device)
     strides, inner = x.stride(), 1
     if len(shape) == 2 and strides[1] == 1:
         return x.data_ptr(), kind, n, strides[0] if n > 1 else width
@@ -375,9 +392,10 @@ class Kv8Cache:
                          (self.v_scales, scales)):
             if tuple(x.shape) != shape:
                 raise ValueError("Kv8Cache: pool of shape %s, not %s" % (tuple(x.shape), shape))
-        self.struct = Kv8Struct(_array(self.k_codes, _INT8, "k_codes"), _array(self.v_codes, _INT8, "v_codes"),
-                                _array(self.k_scales, _F32, "k_scales"), _array(self.v_scales, _F32, "v_scales"),
-                                n_pages, page_size, n_kv_heads, head_dim)
+        dev = ctx.device
+        self.struct = Kv8Struct(_array(self.k_codes, _INT8, "k_codes", dev), _array(self.v_codes, _INT8, "v_codes", dev),
+                                _array(self.k_scales, _F32, "k_scales", dev),
+                                _array(self.v_scales, _F32, "v_scales", dev), n_pages, page_size, n_kv_heads, head_dim)
         self._ref = ctypes.addressof(self.struct)
 
 
@@ -392,20 +410,24 @@ class SeqBatch:
             raise ValueError("SeqBatch: row_start %s, lens %s, page_table %s" % (
                 tuple(row_start.shape), tuple(lens.shape), tuple(page_table.shape)))
         self.row_start, self.lens, self.page_table, self.n_seqs = row_start, lens, page_table, n
-        self.struct = Kv8BatchStruct(n, _array(row_start, _INT32, "row_start"), _array(lens, _INT32, "lens"),
-                                     _array(page_table, _INT32, "page_table"), page_table.shape[1])
+        self.device = dev = _device(row_start)
+        if dev < 0:
+            raise ValueError("SeqBatch: row_start is on the host")
+        self.struct = Kv8BatchStruct(n, _array(row_start, _INT32, "row_start", dev), _array(lens, _INT32, "lens", dev),
+                                     _array(page_table, _INT32, "page_table", dev), page_table.shape[1])
         self._ref = ctypes.addressof(self.struct)
 
 
-def _rope(cos, sin, head_dim):
+def _rope(cos, sin, head_dim, device):
     """(cos address, sin address, rows) of the rotation tables, or none."""
     if cos is None and sin is None:
         return None, None, 0
     if cos is None or sin is None:
         raise ValueError("rope tables: both or neither")
-    if tuple(cos.shape) != tuple(sin.shape) or len(cos.shape) != 2 or cos.shape[1] != head_dim // 2:
-        raise ValueError("rope tables: shapes %s, %s" % (tuple(cos.shape), tuple(sin.shape)))
-    return _array(cos, _F32, "rope_cos"), _array(sin, _F32, "rope_sin"), cos.shape[0]
+    shape = cos.shape
+    if shape != sin.shape or len(shape) != 2 or shape[1] != head_dim // 2:
+        raise ValueError("rope tables: shapes %s, %s" % (tuple(shape), tuple(sin.shape)))
+    return _array(cos, _F32, "rope_cos", device), _array(sin, _F32, "rope_sin", device), shape[0]
 
 
 class CudaBackend:
@@ -520,15 +542,30 @@ class CudaBackend:
         return tok.value
 
     # ---- paged 8-bit KV cache and drafts: the rows and outputs may be DeviceTensors
-    # or torch tensors, on any GPU memory of the context's device
+    # or torch tensors, in GPU memory of the context's device
+    def _kv8_device(self, cache, batch):
+        dev = self.ctx.device
+        if cache.ctx.device != dev or (batch is not None and batch.device != dev):
+            raise ValueError("kv8: a cache or batch of another GPU than the context's, %d" % dev)
+        return dev
+
+    def _workspace(self, x):
+        """(address, bytes) of a workspace, or none."""
+        if x is None:
+            return None, 0
+        if _device(x) != self.ctx.device:
+            raise _elsewhere(x, "workspace", self.ctx.device)
+        return _address(x), x.nbytes
+
     def kv8_append(self, cache, batch, k, v, rope_cos=None, rope_sin=None):
         """Append the batch's new rows (k, v: [n, n_kv_heads*head_dim], strided rows allowed)."""
         _, kv, _, d = cache.shape
-        kp, kt, kn, kld = _rows(k, kv * d, "k")
-        vp, vt, vn, vld = _rows(v, kv * d, "v")
+        dev = self._kv8_device(cache, batch)
+        kp, kt, kn, kld = _rows(k, kv * d, "k", dev)
+        vp, vt, vn, vld = _rows(v, kv * d, "v", dev)
         if kt != vt or kn != vn or (kld != vld and kn > 1):
             raise ValueError("kv8_append: k and v must agree in dtype, rows and row stride")
-        cp, sp, n_pos = _rope(rope_cos, rope_sin, d)
+        cp, sp, n_pos = _rope(rope_cos, rope_sin, d, dev)
         check(lib().llmrs_kv8_append(self.ctx.h, cache._ref, batch._ref, kp, vp, kt, kld, kn, cp, sp, n_pos))
 
     def kv8_read(self, cache, pages, k_out, v_out):
@@ -537,8 +574,9 @@ class CudaBackend:
         shape = (n,) + cache.shape[1:]
         if tuple(k_out.shape) != shape or tuple(v_out.shape) != shape or k_out.dtype != v_out.dtype:
             raise ValueError("kv8_read: outputs must be two arrays of shape %s" % (shape,))
-        kp, vp = _array(k_out, _DTYPES, "k_out"), _array(v_out, _DTYPES, "v_out")
-        check(lib().llmrs_kv8_read(self.ctx.h, cache._ref, _array(pages, _INT32, "pages"), n, kp, vp,
+        dev = self._kv8_device(cache, None)
+        kp, vp = _array(k_out, _DTYPES, "k_out", dev), _array(v_out, _DTYPES, "v_out", dev)
+        check(lib().llmrs_kv8_read(self.ctx.h, cache._ref, _array(pages, _INT32, "pages", dev), n, kp, vp,
                                    _DTYPES[k_out.dtype]))
 
     def kv8_attention_workspace(self, cache, batch, n_heads, n_rows):
@@ -550,23 +588,21 @@ class CudaBackend:
     def kv8_attention(self, cache, batch, q, out=None, rope_cos=None, rope_sin=None, scale=None, workspace=None):
         """Causal attention of the batch's rows q [n, n_heads*head_dim] over the cache,
         after kv8_append of the same batch; writes and returns `out`."""
-        d = cache.shape[3]
+        d, dev = cache.shape[3], self._kv8_device(cache, batch)
         width = q.shape[1] if len(q.shape) == 2 else int(np.prod(q.shape[1:]))
         n_heads = width // d
         if n_heads * d != width:
             raise ValueError("kv8_attention: q rows of %d elements are no heads of %d" % (width, d))
         if out is None:
             out = DeviceTensor(self.ctx, tuple(q.shape), {F32: np.float32, F16: np.float16, BF16: np.uint16}[
-                _rows(q, width, "q")[1]])
-        qp, qt, qn, qld = _rows(q, width, "q")
-        op, ot, on, old = _rows(out, width, "out")
+                _rows(q, width, "q", dev)[1]])
+        qp, qt, qn, qld = _rows(q, width, "q", dev)
+        op, ot, on, old = _rows(out, width, "out", dev)
         if qt != ot or qn != on:
             raise ValueError("kv8_attention: q and out must agree in dtype and rows")
-        cp, sp, n_pos = _rope(rope_cos, rope_sin, d)
+        cp, sp, n_pos = _rope(rope_cos, rope_sin, d, dev)
         check(lib().llmrs_kv8_attention(self.ctx.h, cache._ref, batch._ref, qp, qld, op, old, qt, qn, n_heads, cp, sp,
-                                        n_pos, 0.0 if scale is None else float(scale),
-                                        None if workspace is None else _address(workspace),
-                                        0 if workspace is None else workspace.nbytes))
+                                        n_pos, 0.0 if scale is None else float(scale), *self._workspace(workspace)))
         return out
 
     def verify_draft_workspace(self, n_rows, vocab):
@@ -581,11 +617,11 @@ class CudaBackend:
         [seqs+1]; draft_tokens int32 and draft_probs f32 [drafts, vocab] (or None: certain
         drafts), packed; uniforms f32 [n].  Writes tokens int32 [n], accepted int32
         [seqs] and token_probs f32 [n]."""
-        vocab, n_seqs = logits.shape[1], row_start.shape[0] - 1
-        lp, lt, n, ld = _rows(logits, vocab, "logits")
+        vocab, n_seqs, dev = logits.shape[1], row_start.shape[0] - 1, self.ctx.device
+        lp, lt, n, ld = _rows(logits, vocab, "logits", dev)
         qp, qld = None, 0
         if draft_probs is not None and draft_probs.shape[0]:
-            qp, qt, qn, qld = _rows(draft_probs, vocab, "draft_probs")
+            qp, qt, qn, qld = _rows(draft_probs, vocab, "draft_probs", dev)
             if qt != F32:
                 raise TypeError("draft_probs: dtype %s" % draft_probs.dtype)
             if qn != draft_tokens.shape[0]:
@@ -598,13 +634,13 @@ class CudaBackend:
             raise ValueError("verify_draft: temperature must be [%d]" % n_seqs)
         n_drafts = 0 if draft_tokens is None else draft_tokens.shape[0]
         check(lib().llmrs_verify_draft_counted(
-            self.ctx.h, lp, ld, lt, vocab, n, n_seqs, _array(row_start, _INT32, "row_start"),
-            _array(draft_tokens, _INT32, "draft_tokens") if n_drafts else None, qp, qld, n_drafts,
-            _array(uniforms, _F32, "uniforms"),
-            None if temperature is None else _array(temperature, _F32, "temperature"),
-            _array(tokens, _INT32, "tokens"), _array(accepted, _INT32, "accepted"),
-            None if token_probs is None else _array(token_probs, _F32, "token_probs"),
-            None if workspace is None else _address(workspace), 0 if workspace is None else workspace.nbytes))
+            self.ctx.h, lp, ld, lt, vocab, n, n_seqs, _array(row_start, _INT32, "row_start", dev),
+            _array(draft_tokens, _INT32, "draft_tokens", dev) if n_drafts else None, qp, qld, n_drafts,
+            _array(uniforms, _F32, "uniforms", dev),
+            None if temperature is None else _array(temperature, _F32, "temperature", dev),
+            _array(tokens, _INT32, "tokens", dev), _array(accepted, _INT32, "accepted", dev),
+            None if token_probs is None else _array(token_probs, _F32, "token_probs", dev),
+            *self._workspace(workspace)))
 
     # CpuBackend::quantize_row_q8_0 and Tensor::quantize_q4 (bit-exact)
     def quantize_row_q8_0(self, x):
