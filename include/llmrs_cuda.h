@@ -74,6 +74,13 @@ int llmrs_ctx_create(int device, llmrs_ctx **out);
 int llmrs_ctx_destroy(llmrs_ctx *ctx);
 /* optional: run on a caller-owned cudaStream_t (NULL restores the context's own stream) */
 int llmrs_ctx_set_stream(llmrs_ctx *ctx, void *cuda_stream);
+/* order the context's stream with another one of its device (NULL: the legacy default
+ * stream): what the context is given from now on runs behind what `cuda_stream` has been
+ * given so far, and the other way round.  While `cuda_stream` is captured into a graph the
+ * first takes the context's calls into that graph, and the second has to follow before
+ * the capture ends; a captured context cannot wait for a stream that is not (LLMRS_EINVAL) */
+int llmrs_ctx_wait_stream(llmrs_ctx *ctx, void *cuda_stream);
+int llmrs_stream_wait_ctx(llmrs_ctx *ctx, void *cuda_stream);
 int llmrs_malloc(llmrs_ctx *ctx, size_t bytes, void **d_ptr);
 int llmrs_free(llmrs_ctx *ctx, void *d_ptr);
 /* host<->device copies (Tensor::to_device, src/core/tensor.rs:218-291) */
@@ -196,7 +203,8 @@ int llmrs_quantize_q4(llmrs_ctx *ctx, const float *d_w, size_t n, uint8_t *d_qs,
  * Keys and values are int8 codes with one f32 scale for each (page, KV head);
  * a cached value is code * scale (scales are not negative).  The caller owns
  * every buffer.  All calls run
- * on the context's stream on the context's device; none of them synchronises,
+ * on the context's stream on the context's device (buffers that another stream fills or
+ * reads: llmrs_ctx_wait_stream, llmrs_stream_wait_ctx); none of them synchronises,
  * and with a workspace of the caller's none allocates, so they can be captured
  * into CUDA graphs (graphs that may run at the same time need a workspace
  * each).  Arrays named d_* are read when the work runs, not when the call is

@@ -31,7 +31,7 @@ WFMT_Q4_0, WFMT_Q8_0 = 0, 1
 # every symbol include/llmrs_cuda.h declares (checked by tests/test_synth_and_capi.py)
 EXPORTS = [
     "llmrs_last_error", "llmrs_version", "llmrs_device_count", "llmrs_ctx_create", "llmrs_ctx_destroy",
-    "llmrs_ctx_set_stream", "llmrs_malloc", "llmrs_free", "llmrs_h2d", "llmrs_d2h", "llmrs_d2d",
+    "llmrs_ctx_set_stream", "llmrs_ctx_wait_stream", "llmrs_stream_wait_ctx", "llmrs_malloc", "llmrs_free", "llmrs_h2d", "llmrs_d2h", "llmrs_d2d",
     "llmrs_memset", "llmrs_sync", "llmrs_backend_name", "llmrs_ctx_device",
     "llmrs_matmul_transposed_q4", "llmrs_matmul_transposed_q8", "llmrs_matmul_transposed_f32",
     "llmrs_matmul", "llmrs_matmul_slice", "llmrs_add_assign", "llmrs_silu_mul", "llmrs_rope_inplace",
@@ -110,6 +110,8 @@ def lib():
         "llmrs_ctx_create": (ci, [ci, pp]),
         "llmrs_ctx_destroy": (ci, [vp]),
         "llmrs_ctx_set_stream": (ci, [vp, vp]),
+        "llmrs_ctx_wait_stream": (ci, [vp, vp]),
+        "llmrs_stream_wait_ctx": (ci, [vp, vp]),
         "llmrs_ctx_device": (ci, [vp, ip]),
         "llmrs_malloc": (ci, [vp, sz, pp]),
         "llmrs_free": (ci, [vp, vp]),
@@ -215,6 +217,7 @@ class Context:
         check(lib().llmrs_ctx_create(device, ctypes.byref(h)))
         self.h = h
         self.device = device
+        self.raw_stream = None  # the stream as torch numbers it (0: the default one); None: the context's own
         self._children = weakref.WeakSet()  # models / tensors that must go first
 
     def _adopt(self, obj):
@@ -241,6 +244,7 @@ class Context:
         `stream.cuda_stream`; 0, the default stream, by its name
         cudaStreamLegacy); None goes back to the context's own stream."""
         check(lib().llmrs_ctx_set_stream(self.h, 1 if cuda_stream == 0 else cuda_stream))
+        self.raw_stream = 0 if cuda_stream == 1 else cuda_stream
 
 
 class DeviceTensor:
@@ -325,6 +329,26 @@ def _address(x):
     return x.ptr.value if isinstance(x, DeviceTensor) else x.data_ptr()
 
 
+_raw_stream = None
+
+
+def _torch_stream(device):
+    """Torch's current stream on a GPU, as a number (0: the default stream)."""
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        _raw_stream = torch._C._cuda_getCurrentRawStream
+    return _raw_stream(device)
+
+
+def _foreign(*arrays):
+    """Whether some of the arrays are torch's."""
+    for x in arrays:
+        if x is not None and not isinstance(x, DeviceTensor):
+            return True
+    return False
+
+
 def _device(x):
     """Index of the GPU that holds a DeviceTensor or a torch tensor; -1: host memory."""
     return x.ctx.device if isinstance(x, DeviceTensor) else x.get_device()
@@ -396,6 +420,7 @@ class Kv8Cache:
         self.struct = Kv8Struct(_array(self.k_codes, _INT8, "k_codes", dev), _array(self.v_codes, _INT8, "v_codes", dev),
                                 _array(self.k_scales, _F32, "k_scales", dev),
                                 _array(self.v_scales, _F32, "v_scales", dev), n_pages, page_size, n_kv_heads, head_dim)
+        self.torch = _foreign(self.k_codes, self.v_codes, self.k_scales, self.v_scales)
         self._ref = ctypes.addressof(self.struct)
 
 
@@ -415,6 +440,7 @@ class SeqBatch:
             raise ValueError("SeqBatch: row_start is on the host")
         self.struct = Kv8BatchStruct(n, _array(row_start, _INT32, "row_start", dev), _array(lens, _INT32, "lens", dev),
                                      _array(page_table, _INT32, "page_table", dev), page_table.shape[1])
+        self.torch = _foreign(row_start, lens, page_table)
         self._ref = ctypes.addressof(self.struct)
 
 
@@ -542,7 +568,23 @@ class CudaBackend:
         return tok.value
 
     # ---- paged 8-bit KV cache and drafts: the rows and outputs may be DeviceTensors
-    # or torch tensors, in GPU memory of the context's device
+    # or torch tensors, in GPU memory of the context's device.  A call with torch tensors
+    # runs behind what torch's current stream has been given, and that stream's later work
+    # behind the call, whichever stream the context is on (on torch's own: no cost).
+    def _launch(self, foreign, fn, *args):
+        """A C entry; foreign: some of its arrays are torch's."""
+        ctx = self.ctx
+        if foreign:
+            other = _torch_stream(ctx.device)
+            if other != ctx.raw_stream:
+                check(lib().llmrs_ctx_wait_stream(ctx.h, other))
+                try:
+                    check(fn(ctx.h, *args))
+                finally:
+                    check(lib().llmrs_stream_wait_ctx(ctx.h, other))
+                return
+        check(fn(ctx.h, *args))
+
     def _kv8_device(self, cache, batch):
         dev = self.ctx.device
         if cache.ctx.device != dev or (batch is not None and batch.device != dev):
@@ -566,7 +608,8 @@ class CudaBackend:
         if kt != vt or kn != vn or (kld != vld and kn > 1):
             raise ValueError("kv8_append: k and v must agree in dtype, rows and row stride")
         cp, sp, n_pos = _rope(rope_cos, rope_sin, d, dev)
-        check(lib().llmrs_kv8_append(self.ctx.h, cache._ref, batch._ref, kp, vp, kt, kld, kn, cp, sp, n_pos))
+        self._launch(batch.torch or cache.torch or _foreign(k, v, rope_cos, rope_sin), lib().llmrs_kv8_append,
+                     cache._ref, batch._ref, kp, vp, kt, kld, kn, cp, sp, n_pos)
 
     def kv8_read(self, cache, pages, k_out, v_out):
         """The values of `pages` (int32 [n]) into k_out, v_out [n, n_kv_heads, page_size, head_dim]."""
@@ -576,8 +619,8 @@ class CudaBackend:
             raise ValueError("kv8_read: outputs must be two arrays of shape %s" % (shape,))
         dev = self._kv8_device(cache, None)
         kp, vp = _array(k_out, _DTYPES, "k_out", dev), _array(v_out, _DTYPES, "v_out", dev)
-        check(lib().llmrs_kv8_read(self.ctx.h, cache._ref, _array(pages, _INT32, "pages", dev), n, kp, vp,
-                                   _DTYPES[k_out.dtype]))
+        self._launch(cache.torch or _foreign(pages, k_out, v_out), lib().llmrs_kv8_read, cache._ref,
+                     _array(pages, _INT32, "pages", dev), n, kp, vp, _DTYPES[k_out.dtype])
 
     def kv8_attention_workspace(self, cache, batch, n_heads, n_rows):
         """A workspace for kv8_attention of this many heads and rows (one call at a time)."""
@@ -601,8 +644,9 @@ class CudaBackend:
         if qt != ot or qn != on:
             raise ValueError("kv8_attention: q and out must agree in dtype and rows")
         cp, sp, n_pos = _rope(rope_cos, rope_sin, d, dev)
-        check(lib().llmrs_kv8_attention(self.ctx.h, cache._ref, batch._ref, qp, qld, op, old, qt, qn, n_heads, cp, sp,
-                                        n_pos, 0.0 if scale is None else float(scale), *self._workspace(workspace)))
+        self._launch(batch.torch or cache.torch or _foreign(q, out, rope_cos, rope_sin, workspace),
+                     lib().llmrs_kv8_attention, cache._ref, batch._ref, qp, qld, op, old, qt, qn, n_heads, cp, sp,
+                     n_pos, 0.0 if scale is None else float(scale), *self._workspace(workspace))
         return out
 
     def verify_draft_workspace(self, n_rows, vocab):
@@ -633,14 +677,16 @@ class CudaBackend:
         if temperature is not None and tuple(temperature.shape) != (n_seqs,):
             raise ValueError("verify_draft: temperature must be [%d]" % n_seqs)
         n_drafts = 0 if draft_tokens is None else draft_tokens.shape[0]
-        check(lib().llmrs_verify_draft_counted(
-            self.ctx.h, lp, ld, lt, vocab, n, n_seqs, _array(row_start, _INT32, "row_start", dev),
+        self._launch(
+            _foreign(logits, row_start, draft_tokens, draft_probs, uniforms, tokens, accepted, token_probs, temperature,
+                     workspace),
+            lib().llmrs_verify_draft_counted, lp, ld, lt, vocab, n, n_seqs, _array(row_start, _INT32, "row_start", dev),
             _array(draft_tokens, _INT32, "draft_tokens", dev) if n_drafts else None, qp, qld, n_drafts,
             _array(uniforms, _F32, "uniforms", dev),
             None if temperature is None else _array(temperature, _F32, "temperature", dev),
             _array(tokens, _INT32, "tokens", dev), _array(accepted, _INT32, "accepted", dev),
             None if token_probs is None else _array(token_probs, _F32, "token_probs", dev),
-            *self._workspace(workspace)))
+            *self._workspace(workspace))
 
     # CpuBackend::quantize_row_q8_0 and Tensor::quantize_q4 (bit-exact)
     def quantize_row_q8_0(self, x):

@@ -271,6 +271,70 @@ int llmrs_ctx_set_stream(llmrs_ctx *ctx, void *s)
     return LLMRS_OK;
 }
 
+namespace {
+
+// make the context's device current for the launches of one call
+struct OnDevice {
+    int before = -1, device;
+    explicit OnDevice(int d) : device(d)
+    {
+        if (cudaGetDevice(&before) != cudaSuccess)
+            before = -1;
+        if (before != device)
+            cudaSetDevice(device);
+    }
+    ~OnDevice()
+    {
+        if (before >= 0 && before != device)
+            cudaSetDevice(before);
+    }
+};
+
+} // namespace
+
+// whether work given to a stream becomes part of a graph; asked of the legacy default
+// stream while another one is captured, CUDA answers with an error
+static bool capturing(cudaStream_t s)
+{
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(s, &st) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return false;
+    }
+    return st != cudaStreamCaptureStatusNone;
+}
+
+// what `later` is given from now on runs behind what `first` has been given so far
+static int stream_order(llmrs_ctx *ctx, cudaStream_t first, cudaStream_t later)
+{
+    if (first == later)
+        return LLMRS_OK;
+    OnDevice on(ctx->device);
+    LLMRS_CHECK_ARG(!capturing(later) || capturing(first),
+                    "a stream under capture cannot wait for one that is not captured");
+    cudaEvent_t e;
+    LLMRS_CUDA_TRY(cudaEventCreateWithFlags(&e, cudaEventDisableTiming));
+    cudaError_t rc = cudaEventRecord(e, first);
+    if (rc == cudaSuccess)
+        rc = cudaStreamWaitEvent(later, e, 0);
+    (void)cudaEventDestroy(e);
+    if (rc != cudaSuccess)
+        return fail(LLMRS_ECUDA, "ordering two streams: %s", cudaGetErrorString(rc));
+    return LLMRS_OK;
+}
+
+int llmrs_ctx_wait_stream(llmrs_ctx *ctx, void *s)
+{
+    LLMRS_CHECK_ARG(ctx, "ctx is NULL");
+    return stream_order(ctx, reinterpret_cast<cudaStream_t>(s), ctx->stream);
+}
+
+int llmrs_stream_wait_ctx(llmrs_ctx *ctx, void *s)
+{
+    LLMRS_CHECK_ARG(ctx, "ctx is NULL");
+    return stream_order(ctx, ctx->stream, reinterpret_cast<cudaStream_t>(s));
+}
+
 int llmrs_ctx_device(llmrs_ctx *ctx, int *device)
 {
     LLMRS_CHECK_ARG(ctx && device, "NULL argument");
@@ -563,23 +627,6 @@ int llmrs_quantize_q4(llmrs_ctx *ctx, const float *d_w, size_t n, uint8_t *d_qs,
 
 // ---------------------------------------------------------------- paged 8-bit KV cache, drafts
 namespace {
-
-// make the context's device current for the launches of one call
-struct OnDevice {
-    int before = -1, device;
-    explicit OnDevice(int d) : device(d)
-    {
-        if (cudaGetDevice(&before) != cudaSuccess)
-            before = -1;
-        if (before != device)
-            cudaSetDevice(device);
-    }
-    ~OnDevice()
-    {
-        if (before >= 0 && before != device)
-            cudaSetDevice(before);
-    }
-};
 
 bool known_dtype(int t) { return t == LLMRS_F32 || t == LLMRS_BF16 || t == LLMRS_F16; }
 bool aligned16(const void *p) { return !((uintptr_t)p & 15); }

@@ -94,6 +94,8 @@ extern "C" {
     pub fn llmrs_ctx_create(device: c_int, out: *mut *mut llmrs_ctx) -> c_int;
     pub fn llmrs_ctx_destroy(ctx: *mut llmrs_ctx) -> c_int;
     pub fn llmrs_ctx_set_stream(ctx: *mut llmrs_ctx, cuda_stream: *mut c_void) -> c_int;
+    pub fn llmrs_ctx_wait_stream(ctx: *mut llmrs_ctx, cuda_stream: *mut c_void) -> c_int;
+    pub fn llmrs_stream_wait_ctx(ctx: *mut llmrs_ctx, cuda_stream: *mut c_void) -> c_int;
     pub fn llmrs_malloc(ctx: *mut llmrs_ctx, bytes: usize, d_ptr: *mut *mut c_void) -> c_int;
     pub fn llmrs_free(ctx: *mut llmrs_ctx, d_ptr: *mut c_void) -> c_int;
     pub fn llmrs_h2d(ctx: *mut llmrs_ctx, d_dst: *mut c_void, h_src: *const c_void, bytes: usize) -> c_int;

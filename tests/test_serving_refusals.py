@@ -1,4 +1,5 @@
-"""What the serving operators' entries refuse before any GPU work (on the CPU)."""
+"""What the serving operators refuse before any GPU work, and how their wrappers order streams
+(on the CPU)."""
 import ctypes
 
 import numpy as np
@@ -129,3 +130,51 @@ def test_caches_and_batches_of_the_host_and_of_other_gpus_are_refused(llmrs):
         be.kv8_append(there, llmrs.SeqBatch(I(3), I(2), I(2, 4)), rows, rows)
     with pytest.raises(ValueError, match="another GPU"):
         be.kv8_attention(here, llmrs.SeqBatch(I(3, device=1), I(2, device=1), I(2, 4, device=1)), rows, rows)
+
+
+# ------------------------------------------------------------------ streams
+class _Entries:
+    """Stands for the C library: notes the calls."""
+
+    def __init__(self, fails):
+        self.said, self.fails = [], fails
+
+    def llmrs_ctx_wait_stream(self, h, s):
+        self.said.append(("ctx behind", s))
+        return 0
+
+    def llmrs_stream_wait_ctx(self, h, s):
+        self.said.append(("stream behind", s))
+        return 0
+
+    def llmrs_last_error(self):
+        return b"as told"
+
+    def entry(self, h, *args):
+        self.said.append(("call", args))
+        return 1 if self.fails else 0
+
+
+@pytest.mark.parametrize("fails", [False, True])
+@pytest.mark.parametrize("foreign", [False, True])
+@pytest.mark.parametrize("own,torchs", [(None, 0), (0, 0), (7, 7), (0, 7), (7, 0)])
+def test_calls_are_ordered_with_torch_s_stream(llmrs, monkeypatch, own, torchs, foreign, fails):
+    L = _Entries(fails)
+    monkeypatch.setattr(llmrs, "lib", lambda: L)
+    monkeypatch.setattr(llmrs, "_raw_stream", lambda device: torchs)
+    be = llmrs.CudaBackend(_Gpu(0))
+    be.ctx.raw_stream = own
+    if fails:
+        with pytest.raises(llmrs.LlmrsError):
+            be._launch(foreign, L.entry, 1, 2)
+    else:
+        be._launch(foreign, L.entry, 1, 2)
+    call = [("call", (1, 2))]
+    if foreign and own != torchs:  # torch's stream waits even behind a call that failed
+        call = [("ctx behind", torchs)] + call + [("stream behind", torchs)]
+    assert L.said == call
+
+
+def test_stream_entries_are_checked(llmrs):
+    _refused(llmrs, llmrs.lib().llmrs_ctx_wait_stream(None, None), "ctx is NULL")
+    _refused(llmrs, llmrs.lib().llmrs_stream_wait_ctx(None, None), "ctx is NULL")
