@@ -324,11 +324,6 @@ def _learn_torch(dtype, kinds, what):
     return kinds[dtype]
 
 
-def _address(x):
-    """Device address of a DeviceTensor, or of a torch tensor (anything with data_ptr())."""
-    return x.ptr.value if isinstance(x, DeviceTensor) else x.data_ptr()
-
-
 _raw_stream = None
 
 
@@ -407,7 +402,7 @@ class Kv8Cache:
     def __init__(self, ctx, n_pages, page_size, n_kv_heads, head_dim, k_codes=None, v_codes=None, k_scales=None,
                  v_scales=None):
         codes, scales = (n_pages, n_kv_heads, page_size, head_dim), (n_pages, n_kv_heads)
-        self.ctx, self.shape = ctx, codes
+        self.ctx, self.shape, self.device = ctx, codes, ctx.device
         self.k_codes = DeviceTensor(ctx, codes, np.int8) if k_codes is None else k_codes
         self.v_codes = DeviceTensor(ctx, codes, np.int8) if v_codes is None else v_codes
         self.k_scales = DeviceTensor(ctx, scales) if k_scales is None else k_scales
@@ -587,7 +582,7 @@ class CudaBackend:
 
     def _kv8_device(self, cache, batch):
         dev = self.ctx.device
-        if cache.ctx.device != dev or (batch is not None and batch.device != dev):
+        if cache.device != dev or (batch is not None and batch.device != dev):
             raise ValueError("kv8: a cache or batch of another GPU than the context's, %d" % dev)
         return dev
 
@@ -597,7 +592,7 @@ class CudaBackend:
             return None, 0
         if _device(x) != self.ctx.device:
             raise _elsewhere(x, "workspace", self.ctx.device)
-        return _address(x), x.nbytes
+        return (x.ptr.value if isinstance(x, DeviceTensor) else x.data_ptr()), x.nbytes
 
     def kv8_append(self, cache, batch, k, v, rope_cos=None, rope_sin=None):
         """Append the batch's new rows (k, v: [n, n_kv_heads*head_dim], strided rows allowed)."""
@@ -615,7 +610,7 @@ class CudaBackend:
         """The values of `pages` (int32 [n]) into k_out, v_out [n, n_kv_heads, page_size, head_dim]."""
         n = pages.shape[0]
         shape = (n,) + cache.shape[1:]
-        if tuple(k_out.shape) != shape or tuple(v_out.shape) != shape or k_out.dtype != v_out.dtype:
+        if k_out.shape != shape or v_out.shape != shape or k_out.dtype != v_out.dtype:
             raise ValueError("kv8_read: outputs must be two arrays of shape %s" % (shape,))
         dev = self._kv8_device(cache, None)
         kp, vp = _array(k_out, _DTYPES, "k_out", dev), _array(v_out, _DTYPES, "v_out", dev)
@@ -670,11 +665,11 @@ class CudaBackend:
                 raise TypeError("draft_probs: dtype %s" % draft_probs.dtype)
             if qn != draft_tokens.shape[0]:
                 raise ValueError("verify_draft: %d drafted tokens, %d distributions" % (draft_tokens.shape[0], qn))
-        if tuple(uniforms.shape) != (n,) or tuple(tokens.shape) != (n,) or tuple(accepted.shape) != (n_seqs,):
+        if uniforms.shape != (n,) or tokens.shape != (n,) or accepted.shape != (n_seqs,):
             raise ValueError("verify_draft: uniforms and tokens must be [%d], accepted [%d]" % (n, n_seqs))
-        if token_probs is not None and tuple(token_probs.shape) != (n,):
+        if token_probs is not None and token_probs.shape != (n,):
             raise ValueError("verify_draft: token_probs must be [%d]" % n)
-        if temperature is not None and tuple(temperature.shape) != (n_seqs,):
+        if temperature is not None and temperature.shape != (n_seqs,):
             raise ValueError("verify_draft: temperature must be [%d]" % n_seqs)
         n_drafts = 0 if draft_tokens is None else draft_tokens.shape[0]
         self._launch(
