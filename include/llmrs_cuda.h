@@ -210,8 +210,9 @@ int llmrs_quantize_q4(llmrs_ctx *ctx, const float *d_w, size_t n, uint8_t *d_qs,
  * each).  Arrays named d_* are read when the work runs, not when the call is
  * made.  Numbers in them that lead outside the buffers are skipped and reported
  * by the next llmrs_sync (LLMRS_EDEVICE): a sequence whose rows or length do
- * not fit counts as having no rows, tokens of a page id outside the pool are
- * left out.
+ * not fit counts as having no rows, whatever stands in front of it or behind (rows
+ * that two sequences claim have unspecified results), tokens of a page id outside the
+ * pool are left out.
  * ====================================================================== */
 typedef struct {
     int8_t *d_k_codes, *d_v_codes; /* [n_pages][n_kv_heads][page_size][head_dim], 16-byte aligned */

@@ -35,6 +35,8 @@
 // Work: the tiles of all (sequence, KV head, tile of rows) in one row, cut into
 // equal consecutive ranges, one per CTA; pieces of a softmax that a range cuts
 // are joined by a second kernel (kv8_core.cuh).
+#include <limits.h>
+
 #include "gemv.cuh"
 #include "kv8_core.cuh"
 #include "kv8_many.cuh"
@@ -886,14 +888,25 @@ __global__ void __launch_bounds__(QT) kv8_q_kernel(const __grid_constant__ ManyP
     constexpr int H = D / 2;
     const Kv8Attn &a = p.a;
     const int row = blockIdx.x, j = threadIdx.x % L;
-    int s = 0; // the row's sequence: how many end at or before it
-    for (int s0 = 0; s0 < a.b.n_seqs; s0 += QT)
-        s += __syncthreads_count(s0 + (int)threadIdx.x < a.b.n_seqs && a.b.row_start[s0 + threadIdx.x + 1] <= row);
-    if (s >= a.b.n_seqs)
-        return;
+    // the row's sequence: the first with many rows, this one among them, whose numbers fit (as
+    // kv8_many_kernel judges them, each by its own: the row starts of a bad batch can fall)
+    __shared__ int s_owner;
+    if (threadIdx.x == 0)
+        s_owner = INT_MAX;
+    __syncthreads();
     int r0, n, len;
+    for (int s = threadIdx.x; s < a.b.n_seqs; s += QT)
+        if (a.b.row_start[s] <= row && row < a.b.row_start[s + 1]) {
+            kv8_seq(a.b, s, a.err, r0, n, len);
+            if ((long long)n * (a.n_heads / a.c.n_kv) > p.many)
+                atomicMin(&s_owner, s);
+        }
+    __syncthreads();
+    const int s = s_owner;
+    if (s == INT_MAX)
+        return;
     kv8_seq(a.b, s, a.err, r0, n, len);
-    if (row < r0 || row >= r0 + n || (long long)n * (a.n_heads / a.c.n_kv) <= p.many)
+    if (row < r0 || row >= r0 + n) // only if the batch's numbers changed under way
         return;
     const T *q = reinterpret_cast<const T *>(a.q) + (size_t)row * a.ld_q;
     float4 c = make_float4(1.0f, 1.0f, 1.0f, 1.0f), t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
