@@ -280,7 +280,8 @@ int llmrs_kv8_attention(llmrs_ctx *ctx, const llmrs_kv8 *cache, const llmrs_kv8_
  * that has rows), d_draft_probs [n_drafts][ld_probs] the f32 distributions they
  * were drawn from (NULL: each draft was certain, e.g. found by lookup).  Both may be
  * longer than the row starts say; a sequence whose drafts would lie behind their end
- * counts as one whose rows do not fit.  With
+ * counts as one whose rows do not fit, and so does each behind row starts that fall
+ * (where its drafts lie is not known): d_accepted[s] = 0, reported by llmrs_sync.  With
  * p = softmax(logits / temperature), draft i is accepted while
  *   u[row i] * q_i(d_i) < p_i(d_i),
  * and the next token is drawn with u[last row] from max(p - q, 0) of the first

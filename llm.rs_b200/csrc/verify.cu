@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(VT) verify_rows_kernel(VerifyParams p, RowPart
     __shared__ float s_m[VT / 32];
     __shared__ int s_at[VT / 32];
     __shared__ double s_s[VT / 32];
+    __shared__ int s_seq;
     constexpr int E = 16 / (int)sizeof(T); // logits of a 16-byte load
     const int row = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const T *x = reinterpret_cast<const T *>(p.logits) + (size_t)row * p.ld;
@@ -137,13 +138,20 @@ __global__ void __launch_bounds__(VT) verify_rows_kernel(VerifyParams p, RowPart
                 l[i * E + e] = t + e >= 0 && t + e < p.vocab ? to_float(x[t + e]) : -INFINITY;
         }
     }
-    // the row's sequence, for its temperature: how many sequences end at or before the row
-    int seq = 0;
-    for (int s0 = 0; p.temperature && s0 < p.n_seqs; s0 += VT) {
-        const int s = s0 + (int)threadIdx.x;
-        seq += __syncthreads_count(s < p.n_seqs && p.row_start[s + 1] <= row);
+    // the row's sequence, for its temperature: the first that holds it (row starts that fall
+    // end the batch for verify_pick, and in front of them no other sequence does)
+    float T_ = 1.0f;
+    if (p.temperature) {
+        if (threadIdx.x == 0)
+            s_seq = INT_MAX;
+        __syncthreads();
+        for (int s = threadIdx.x; s < p.n_seqs; s += VT)
+            if (p.row_start[s] <= row && row < p.row_start[s + 1])
+                atomicMin(&s_seq, s);
+        __syncthreads();
+        if (s_seq != INT_MAX)
+            T_ = p.temperature[s_seq];
     }
-    const float T_ = p.temperature && seq < p.n_seqs ? p.temperature[seq] : 1.0f;
     const float inv = T_ > 0.0f ? 1.4426950408889634f / T_ : 0.0f;
     float m = -INFINITY;
     int at = INT_MAX;

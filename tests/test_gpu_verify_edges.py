@@ -1,10 +1,10 @@
 """Verification of drafted tokens where its inputs are at their ends: fewer drafts than the
-row starts ask for, none at all."""
+row starts ask for, none at all, row starts that fall."""
 import numpy as np
 import pytest
 
 import serving_oracle as S
-from test_gpu_verify import check, make, run
+from test_gpu_verify import P_OFF, check, make, run
 
 pytestmark = pytest.mark.gpu
 
@@ -42,7 +42,7 @@ def test_verify_drafts_that_are_not_there(llmrs, ctx, be, row_start, have, short
         if s not in short:
             assert margin[s].min() > 1e-4  # no draw of this input lies on a border
             assert accepted[s] == count[s] and np.array_equal(tokens[a:b], want[a:b])
-            assert np.all(np.abs(out[a:b] - p[a:b]) <= 2.0 ** -18 * p[a:b])
+            assert np.all(np.abs(out[a:b] - p[a:b]) <= P_OFF * p[a:b])
 
 
 def test_verify_plain_sampling_with_rows_behind_the_last_sequence(llmrs, ctx, be):
@@ -60,3 +60,18 @@ def test_verify_plain_sampling_with_rows_behind_the_last_sequence(llmrs, ctx, be
     want = S.verify(c["logits"], c["row_start"], c["draft"], None, c["u"], None)[0]
     assert np.array_equal(tokens.numpy()[:3], want[:3]) and np.all(tokens.numpy()[3:] == 777)
     assert np.all(accepted.numpy() == 0)
+
+
+def test_verify_temperatures_behind_row_starts_that_fall(llmrs, ctx, be):
+    """Row starts [0, 4, 1]: the second sequence does not fit, the first one's rows have its temperature."""
+    c = make(52, 800, [3, 0])
+    c["heats"] = np.float32([2.0, 0.3])
+    c["u"][:3] = 0.0  # the drafts are accepted, and their probabilities go out
+    want, count, p, margin = S.verify(c["logits"][:4], [0, 4], c["draft"], c["q"], c["u"], c["heats"])
+    assert count[0] == 3 and margin[0, 1] > 1e-4
+    c["row_start"] = np.int32([0, 4, 1])
+    tokens, accepted, out = run(llmrs, ctx, be, c)
+    _reported(llmrs, ctx, 5)
+    assert accepted.tolist() == [3, 0] and np.array_equal(tokens[:4], want)
+    assert np.all(np.abs(out[:4] - p) <= P_OFF * p)
+    assert tokens[4] == 777 and out[4] == 777
