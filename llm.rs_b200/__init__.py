@@ -658,20 +658,21 @@ class CudaBackend:
         [seqs] and token_probs f32 [n]."""
         vocab, n_seqs, dev = logits.shape[1], row_start.shape[0] - 1, self.ctx.device
         lp, lt, n, ld = _rows(logits, vocab, "logits", dev)
+        n_drafts = 0 if draft_tokens is None else draft_tokens.shape[0]
         qp, qld = None, 0
-        if draft_probs is not None and draft_probs.shape[0]:
-            qp, qt, qn, qld = _rows(draft_probs, vocab, "draft_probs", dev)
-            if qt != F32:
-                raise TypeError("draft_probs: dtype %s" % draft_probs.dtype)
-            if qn != draft_tokens.shape[0]:
-                raise ValueError("verify_draft: %d drafted tokens, %d distributions" % (draft_tokens.shape[0], qn))
+        if draft_probs is not None:
+            if draft_probs.shape[0] != n_drafts:
+                raise ValueError("verify_draft: %d drafted tokens, %d distributions" % (n_drafts, draft_probs.shape[0]))
+            if n_drafts:
+                qp, qt, _, qld = _rows(draft_probs, vocab, "draft_probs", dev)
+                if qt != F32:
+                    raise TypeError("draft_probs: dtype %s" % draft_probs.dtype)
         if uniforms.shape != (n,) or tokens.shape != (n,) or accepted.shape != (n_seqs,):
             raise ValueError("verify_draft: uniforms and tokens must be [%d], accepted [%d]" % (n, n_seqs))
         if token_probs is not None and token_probs.shape != (n,):
             raise ValueError("verify_draft: token_probs must be [%d]" % n)
         if temperature is not None and temperature.shape != (n_seqs,):
             raise ValueError("verify_draft: temperature must be [%d]" % n_seqs)
-        n_drafts = 0 if draft_tokens is None else draft_tokens.shape[0]
         self._launch(
             _foreign(logits, row_start, draft_tokens, draft_probs, uniforms, tokens, accepted, token_probs, temperature,
                      workspace),

@@ -132,6 +132,18 @@ def test_caches_and_batches_of_the_host_and_of_other_gpus_are_refused(llmrs):
         be.kv8_attention(here, llmrs.SeqBatch(I(3, device=1), I(2, device=1), I(2, 4, device=1)), rows, rows)
 
 
+def test_draft_probs_have_a_row_for_each_draft(llmrs):
+    """None alone means certain drafts: an empty array beside drafted tokens is a wrong shape."""
+    call, args = _wrappers(llmrs)["verify"]
+    T = lambda n: _tensor(llmrs, (n, 100), np.float32)  # noqa: E731
+    none = _tensor(llmrs, (0,), np.int32)
+    for draft, probs in ((args["draft_tokens"], T(0)), (args["draft_tokens"], T(2)), (none, T(3)), (None, T(3))):
+        with pytest.raises(ValueError, match="distributions"):
+            call(**dict(args, draft_tokens=draft, draft_probs=probs))
+    for draft, probs in ((args["draft_tokens"], None), (none, T(0)), (None, T(0)), (none, None), (None, None)):
+        _all_right(llmrs, call, dict(args, draft_tokens=draft, draft_probs=probs))
+
+
 # ------------------------------------------------------------------ streams
 class _Entries:
     """Stands for the C library: notes the calls."""
