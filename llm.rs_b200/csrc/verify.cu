@@ -152,7 +152,10 @@ __global__ void __launch_bounds__(VT) verify_rows_kernel(VerifyParams p, RowPart
         if (s_seq != INT_MAX)
             T_ = p.temperature[s_seq];
     }
-    const float inv = T_ > 0.0f ? 1.4426950408889634f / T_ : 0.0f;
+    // a subnormal temperature's reciprocal is past f32: it and the differences of the logits
+    // take 2^64 each (a difference that this makes infinite weighs nothing either way)
+    const bool tiny = T_ > 0.0f && T_ < FLT_MIN;
+    const float inv = T_ > 0.0f ? 1.4426950408889634f / (tiny ? T_ * 0x1p64f : T_) : 0.0f;
     float m = -INFINITY;
     int at = INT_MAX;
 #pragma unroll
@@ -176,9 +179,15 @@ __global__ void __launch_bounds__(VT) verify_rows_kernel(VerifyParams p, RowPart
             at = s_at[w];
         }
     float sum = 0.0f;
+    if (tiny) {
 #pragma unroll
-    for (int i = 0; i < VPER; i++)
-        sum += l[i] > -INFINITY ? ex2((l[i] - m) * inv) : 0.0f;
+        for (int i = 0; i < VPER; i++)
+            sum += l[i] > -INFINITY ? ex2((l[i] - m) * 0x1p64f * inv) : 0.0f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPER; i++)
+            sum += l[i] > -INFINITY ? ex2((l[i] - m) * inv) : 0.0f;
+    }
     const double d = warp_sum_d((double)sum);
     if (lane == 0)
         s_s[warp] = d;

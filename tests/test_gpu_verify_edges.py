@@ -1,5 +1,5 @@
 """Verification of drafted tokens where its inputs are at their ends: fewer drafts than the
-row starts ask for, none at all, row starts that fall."""
+row starts ask for, none at all, row starts that fall, the smallest temperatures."""
 import numpy as np
 import pytest
 
@@ -75,3 +75,18 @@ def test_verify_temperatures_behind_row_starts_that_fall(llmrs, ctx, be):
     assert accepted.tolist() == [3, 0] and np.array_equal(tokens[:4], want)
     assert np.all(np.abs(out[:4] - p) <= P_OFF * p)
     assert tokens[4] == 777 and out[4] == 777
+
+
+@pytest.mark.parametrize("heat", [1.1e-38, 4.4e-39, 4e-39, 1e-39, 1e-42, 1e-45])
+@pytest.mark.parametrize("probs", [True, False])
+def test_verify_smallest_temperatures(llmrs, ctx, be, heat, probs):
+    """Below 2^-126 / log2(e) the reciprocal of the temperature is past f32: p is still one at the
+    likeliest token, which several share here."""
+    c = make(53, 3001, [4, 0, 2, 3], heat=heat, probs=probs)
+    c["logits"][:, [17, 2500]] = 60.0
+    c["draft"][:] = 17
+    c["raw"] = c["logits"].copy()
+    if probs:
+        c["q"][:] = np.float32(1 / 3001)
+    assert check(llmrs, ctx, be, c) == 4
+    assert run(llmrs, ctx, be, c)[1].sum() > 0  # u * q < 1/2: some are accepted
