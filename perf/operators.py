@@ -157,12 +157,14 @@ _backend = []
 
 
 def _be():
-    """The framework's backend on torch's stream: made once, as a program does at its start."""
+    """The framework's backend: made once, as a program does at its start, and put on torch's stream."""
     if not _backend:
         pkg = _package()
-        ctx = pkg.Context(0)
-        ctx.set_stream(torch.cuda.current_stream().cuda_stream)
-        _backend.append(pkg.CudaBackend(ctx))
+        _backend.extend((pkg.CudaBackend(pkg.Context(0)), None))
+    stream = torch.cuda.current_stream().cuda_stream
+    if stream != _backend[1]:
+        _backend[0].ctx.set_stream(stream)
+        _backend[1] = stream
     return _backend[0]
 
 
