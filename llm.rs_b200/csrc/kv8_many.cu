@@ -408,9 +408,19 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
     auto wait = [&](int b, int use) { // whole warp
         return __all_sync(0xffffffffu, kv8_wait(&bar[b], (uint32_t)(use & 1), a.err));
     };
-    bool ok = true;
+    // Every role ends on its own, and no value in a register outlives one: behind the ends
+    // roles with 48 and with 160 registers would meet.  After a wait that ran out, products in
+    // flight end before their memory goes.
+    auto leave = [&](bool ok) {
+        for (int i = 0; i < 64 && !ok; i++)
+            __nanosleep(1000);
+        tc_before();
+        asm volatile("bar.sync 1, %0;" ::"n"(MANY_THREADS) : "memory");
+        tc_after();
+    };
 
     if (wg == 0 || wg == 4) {
+        bool ok = true;
         // ================================================= softmax of every other tile: thread = row
         static_assert(2 * 80 + 160 + 2 * 56 + 48 == 6 * 80, "the launch's registers, shared out");
         const int r = threadIdx.x & 127, odd = wg >> 2;
@@ -542,9 +552,11 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
             if (lane == 0)
                 mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
         }
+        leave(ok);
     } else if (wg == 1) {
         // ================================================= output: thread = row
         regs_up<160>();
+        bool ok = true;
         const int r = threadIdx.x - 128;
         const uint32_t lanes = tmem + NS * MB + ((uint32_t)((warp & 3) * 32) << 16);
         float2 acc[D / 2];
@@ -623,9 +635,11 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
             if (lane == 0)
                 mbar_arrive(&bar[B_INFO_EMPTY + i % INFO]);
         }
+        leave(ok);
     } else if (wg == 2 || wg == 5) {
         // ================================================= codes to f16: keys, values
         regs_down<56>();
+        bool ok = true;
         // Eight lanes take eight 16-code units: for D = 128 half the units of two tokens,
         // crosswise, for D = 64 two tokens, so that the eight 16-byte stores of a pass fall
         // into eight bank groups.  Unit n of a thread: token tok + 32 * (n / PER), column
@@ -680,8 +694,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                 load(i + 1);
             }
         }
+        leave(ok);
     } else if (wg == 3) {
         regs_down<48>();
+        bool ok = true;
         if (warp == 12) {
             // ============================================= the products
             constexpr uint32_t QK = idesc_f16(MB, false), PV = idesc_f16(D, true);
@@ -867,13 +883,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                 for (int it = 0; it < 100000 && !mbar_try_wait(&bar[B_Q_FULL + i % Lay::QS], (uint32_t)((i / Lay::QS) & 1)); it++)
                     ;
         }
+        leave(ok);
+        if (warp == 12)
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s_tmem), "r"(512) : "memory");
     }
-    if (!ok) // let products in flight end before their memory goes
-        for (int i = 0; i < 64; i++)
-            __nanosleep(1000);
-    __syncthreads();
-    if (warp == 12)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s_tmem), "r"(512) : "memory");
 }
 
 // Q of the sequences with many rows, once: rotated by its position, brought to
