@@ -39,7 +39,6 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
-#include <mutex>
 
 #include "gemv.cuh"
 #include "kv8_core.cuh"

@@ -60,11 +60,11 @@ struct ManyTile {
     float vs[8];                 // value scales
     float lvs[8];                // log2 of them, rounded up (-inf: zero)
     int first, last, masked;     // of the pair within this range; some row does not see all tokens
-    int tile, s, g, mt;          // which
+    int tile, g, mt;             // which
     int r0, n, len;              // of the sequence
     int from_start, to_end, pieces;
     int item;                    // number of the pair within this range
-    int pad[2];
+    int pad[3];
 };
 static_assert(sizeof(ManyTile) == 192, "16-byte words");
 
@@ -836,7 +836,6 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                             x.last = x.to_end || i == mine - 1;
                             x.masked = hole || own_tile * MB + MB > own.len + own.mt * R + 1;
                             x.tile = own_tile;
-                            x.s = own.s;
                             x.g = own.g;
                             x.mt = own.mt;
                             x.r0 = own.r0;
