@@ -90,3 +90,26 @@ def test_verify_smallest_temperatures(llmrs, ctx, be, heat, probs):
         c["q"][:] = np.float32(1 / 3001)
     assert check(llmrs, ctx, be, c) == 4
     assert run(llmrs, ctx, be, c)[1].sum() > 0  # u * q < 1/2: some are accepted
+
+
+def test_verify_draws_next_to_a_border(llmrs, ctx, be):
+    """Two tokens, exp(-t) and 1, and a draw u that lies beside the border of the first one, p0 =
+    exp(-t) / (1 + exp(-t)), by a share of 1.3e-12 to 1e-11 of it: the 64-bit exponential, off by
+    r^5 / 120 < 1.25e-12 of itself for |r| <= ln(2) / 64 (the likelier token's is exactly 1), still
+    decides each one, and sums with a few roundings of 2^-53 do not matter."""
+    rng = np.random.default_rng(54)
+    t = rng.uniform(0.02, 80.0, 4_000_000).astype(np.float32)
+    w = np.exp(-t.astype(np.float64))
+    p0 = w / (1 + w)
+    u = p0.astype(np.float32)
+    off = (w * (1 - u.astype(np.float64)) - u) / w  # above 0: the first token is drawn
+    some = (np.abs(off) > 1.3e-12) & (np.abs(off) < 1e-11)
+    t, u, off = t[some], u[some], off[some]
+    assert 300 < t.size < 4000 and 0.3 < (off > 0).mean() < 0.7 and t.min() < 2 and t.max() > 60
+    logits = np.stack([-t, np.zeros_like(t)], axis=1)
+    T = llmrs.DeviceTensor.from_numpy
+    n = t.size
+    tokens, accepted = llmrs.DeviceTensor(ctx, (n,), np.int32), llmrs.DeviceTensor(ctx, (n,), np.int32)
+    be.verify_draft(T(ctx, logits), T(ctx, np.arange(n + 1, dtype=np.int32)), None, None, T(ctx, u), tokens, accepted)
+    ctx.sync()
+    assert np.array_equal(tokens.numpy(), np.where(off > 0, 0, 1))
