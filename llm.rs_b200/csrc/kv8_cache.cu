@@ -58,9 +58,9 @@ __device__ __forceinline__ uint32_t code4(float4 x, float inv)
 // stay in registers between the maximum and the codes; longer ones are read again,
 // from the L2.  Full pages are bound by reading the rows: 8192 rows of 8 heads of
 // 128, f32, pages of 32 take 26 us (84 MB: half of the memory's rate, whatever the
-// warps, rows held and CTAs per SM).  A row or two per page are a chain of loads
-// that depend on one another, so a warp to a unit keeps all of a decode step's
-// chains on the GPU at once: 191 rows 5 us, and 14 with a CTA to a unit.
+// warps, rows held and CTAs per SM).  A few rows per page are a chain of loads
+// that depend on one another, so a warp to a unit keeps more of such a batch's
+// chains on the GPU at once, and four warps shorten each (append_one_warp).
 template <class T, int D, int WARPS>
 __global__ void __launch_bounds__(AP_THREADS) kv8_append_kernel(Kv8 c, Kv8Batch b, const T *k, const T *v,
                                                                 long long ld, Kv8Rope rope, uint32_t *err)
@@ -232,6 +232,24 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, const int *pages, 
     }
 }
 
+// Whether a warp takes a unit, in place of four: yes for a row or two per sequence, and up to
+// 32 while the units are many for the rows.  Both forms, us, f32 rows, 8 KV heads of 128, pages
+// of 64, one warp / four:
+//   sequences   1 row      3 rows     6 rows     9 rows     16 rows     32 rows     64 rows
+//     8         3.2/3.2    3.5/3.3    4.2/3.3    5.2/3.5     6.5/3.6    10.8/5.0
+//    32                               4.4/4.4    5.3/4.8     7.3/5.0
+//    64         3.4/4.2    3.9/6.2    4.8/6.6    5.8/7.1     7.7/7.4    13.0/10.6
+//   191         4.3/9.5    5.5/13.4   6.7/14.2   8.0/15.3   11.2/16.6   20.0/24.4   52.4/44.9
+// They cross at rows = units / 64 to units / 85, units = 2 x KV heads x sequences (so also for 2
+// KV heads), and for heads of 64, twice as many to a warp's round, at twice that.  Where the
+// scale grows, one warp takes 7 us longer for a page of 128 held tokens, four take 2.
+bool append_one_warp(const Kv8 &c, const Kv8Batch &b)
+{
+    const long long rows = (b.n_rows + (long long)b.n_seqs - 1) / b.n_seqs; // of a sequence, on average
+    const long long units = 2LL * c.n_kv * b.n_seqs;
+    return rows <= 2 || (rows <= 32 && rows * c.D * 80 <= units * 128);
+}
+
 template <class T, int D>
 cudaError_t append_d(const Kv8 &c, const Kv8Batch &b, const T *k, const T *v, long long ld, const Kv8Rope &r,
                      uint32_t *err, unsigned pages, cudaStream_t stream)
@@ -241,7 +259,7 @@ cudaError_t append_d(const Kv8 &c, const Kv8Batch &b, const T *k, const T *v, lo
         return launch(kernel, dim3(pages, (2 * c.n_kv + per - 1) / per), dim3(AP_THREADS), 0, stream, false, c, b, k, v, ld,
                       r, err);
     };
-    if (b.n_rows <= 2 * b.n_seqs) // a decode step: a row or two per page
+    if (append_one_warp(c, b))
         return run(kv8_append_kernel<T, D, 1>, 1);
     return run(kv8_append_kernel<T, D, FULL_WARPS>, FULL_WARPS);
 }

@@ -1,5 +1,5 @@
-"""The paged 8-bit cache in batches of more sequences than a CTA has threads, and pages whose
-scale grows in a decode step."""
+"""The paged 8-bit cache in batches of more sequences than a CTA has threads, batches that a warp
+or four to a page append, and pages whose scale grows in a decode step."""
 import numpy as np
 import pytest
 
@@ -37,3 +37,17 @@ def test_append_grows_the_scale_of_full_pages(llmrs, ctx, be, page, d, dtype):
     ctx.sync()
     held = [t.table[s, n // page] for s, n in enumerate(lens) if n % page]
     assert all(np.all(t.pool[n][held] > 4 * old[n][held]) for n in old)
+
+
+@pytest.mark.parametrize("seqs,most,kv,d,page,dtype", [
+    (150, 60, 8, 128, 64, "f32"), (150, 60, 8, 64, 16, "bf16"), (60, 12, 8, 128, 128, "f16"), (20, 12, 2, 128, 32, "f32")])
+def test_append_a_few_rows_to_many_sequences(llmrs, ctx, be, seqs, most, kv, d, page, dtype):
+    """Up to `most` rows each, on both sides of where four warps take over from one."""
+    rng = np.random.default_rng(103)
+    lens, rows = rng.integers(0, 90, seqs).tolist(), rng.integers(0, most + 1, seqs).tolist()
+    t = Setup(llmrs, ctx, 103, lens, rows, kv, kv, d, page, dtype)
+    (k, kx), (v, vx) = t.rows("k"), t.rows("v")
+    be.kv8_append(t.cache, t.batch, k, v, t.g_cos, t.g_sin)
+    ctx.sync()
+    S.append(t.pool, t.row_start, t.lens, t.table, kx, vx, t.cos, t.sin)
+    same(t.download(), t.pool)
