@@ -60,11 +60,13 @@ struct ManyTile {
     float vs[8];                 // value scales
     float lvs[8];                // log2 of them, rounded up (-inf: zero)
     int first, last, masked;     // of the pair within this range; some row does not see all tokens
-    int tile, g, mt;             // which
+    int tile;                    // of tokens
+    int pad0;                    // g at 8 of 16 bytes: at 4 the kernel spills 76 bytes, not 16 (two prompts 511 us, 482 so)
+    int g, mt;                   // KV head, tile of rows
     int r0, n, len;              // of the sequence
     int from_start, to_end, pieces;
     int item;                    // number of the pair within this range
-    int pad[3];
+    int pad1[2];
 };
 static_assert(sizeof(ManyTile) == 192, "16-byte words");
 
