@@ -261,8 +261,10 @@ int llmrs_kv8_read(llmrs_ctx *ctx, const llmrs_kv8 *cache, const int *d_pages, i
  * head h / (n_heads/n_kv_heads), any whole ratio.  q is rotated on the way (NULL
  * tables: it is not).  scale multiplies q.k (0: 1/sqrt(head_dim)).  f32 rows are
  * computed to f32 accuracy (against the row's largest values, where the value scales
- * of pages lie further apart than 2^15), 16-bit rows to that of their type.  A row for which
- * no page can be read gets zeros.  d_workspace: llmrs_kv8_attention_workspace
+ * of pages lie further apart than 2^15), f16 rows too, up to the rounding of the result.
+ * bf16 rows: the rotated q and the probabilities are rounded to 11 bits once, and the
+ * result to bf16's 8; its 2-norm error against 64 bits is 3 to 8 % above that of the
+ * result's rounding alone.  A row for which no page can be read gets zeros.  d_workspace: llmrs_kv8_attention_workspace
  * bytes (which depend on the sizes only), 16-byte aligned, contents irrelevant; NULL: the
  * context's scratch (not while capturing, and not by calls that may run at the same
  * time on several streams). */
@@ -287,7 +289,9 @@ int llmrs_kv8_attention(llmrs_ctx *ctx, const llmrs_kv8 *cache, const llmrs_kv8_
  * and the next token is drawn with u[last row] from max(p - q, 0) of the first
  * rejected draft's row (from p where nothing is left over), or from the last
  * row's p when all were accepted: the first token, in index order, whose running
- * sum exceeds u times the total (64-bit sums).  d_temperature [n_seqs] (NULL: 1);
+ * sum exceeds u times the total (the draw: 64-bit exponentials, off by 1.3e-12 of
+ * themselves, and sums; the acceptances: sums of 32 f32 exponentials each, added up in
+ * 64 bits, so p_i(d_i) is off by less than 2^-18 of itself).  d_temperature [n_seqs] (NULL: 1);
  * 0 takes the first most likely token.  -inf (and NaN) logits have no weight; a row
  * without any yields token -1 and accepts nothing.  A draft outside the vocabulary is
  * rejected and reported by llmrs_sync.  Out: d_tokens[rows] the accepted drafts,

@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, const int *pages, 
 //   191         4.3/9.5    5.5/13.4   6.7/14.2   8.0/15.3   11.2/16.6   20.0/24.4   52.4/44.9
 // They cross at rows = units / 64 to units / 85, units = 2 x KV heads x sequences (so also for 2
 // KV heads), and for heads of 64, twice as many to a warp's round, at twice that.  Where the
-// scale grows, one warp takes 7 us longer for a page of 128 held tokens, four take 2.
+// scale grows, one warp takes 7 us longer for a page of 103 held tokens, four take 2.
 bool append_one_warp(const Kv8 &c, const Kv8Batch &b)
 {
     const long long rows = (b.n_rows + (long long)b.n_seqs - 1) / b.n_seqs; // of a sequence, on average

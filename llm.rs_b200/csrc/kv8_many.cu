@@ -6,9 +6,11 @@
 // f16 operands, f32 accumulators in TMEM.  The codes are exact in f16.  f32
 // rows: Q and P are two f16 pieces each (22 bits and more), so the products
 // run twice; f16 rows too (with P in one piece they are 1.4 times as far off as
-// the rounding of the result); bf16 rows: one each.  Every tile's O is a fresh
-// product that registers add up in f32, with the change of the maximum applied
-// there: long sums do not pass through the tensor core's accumulator.
+// the rounding of the result); bf16 rows: one each, of 11 bits, which leaves the
+// result's 2-norm error at 1.72e-3 where its own rounding to 8 bits makes 1.66e-3
+// (two pieces: 1.66e-3, and 615 us for the two prompts below).  Every tile's O is
+// a fresh product that registers add up in f32, with the change of the maximum
+// applied there: long sums do not pass through the tensor core's accumulator.
 //
 // Warpgroups: 0 and 4 softmax of every other tile (thread = row), 1 output
 // (thread = row, D accumulators), 2 and 5 key and value codes to f16 in shared
@@ -26,11 +28,11 @@
 // instructions take 4 to 5 cycles each: so each role that was the longest got a
 // second warpgroup or a kernel of its own, and each keeps its next loads (TMEM
 // columns, codes) in flight while it works.  Two prompts of 3500 to 4096 rows,
-// bf16, 32 heads of 128 over 8: 493 us (496 TFLOP/s; 740 us with one softmax, one
+// bf16, 32 heads of 128 over 8: 475 us (515 TFLOP/s; 740 us with one softmax, one
 // widening and one Q warpgroup), chunks of 3 prompts of 1000 rows behind 0 to 3000
-// tokens, f32: 265 us.  Left: 3400 to 3900 cycles a tile, spread over all roles:
-// without any softmax it would be 394 us, without widening 454, without the
-// output's sums 471.
+// tokens, f32: 267 us.  Left: 3400 to 3900 cycles a tile, spread over all roles:
+// of 493 us (an earlier build) 394 stayed without any softmax, 454 without
+// widening, 471 without the output's sums.
 //
 // Work: the tiles of all (sequence, KV head, tile of rows) in one row, cut into
 // equal consecutive ranges, one per CTA; pieces of a softmax that a range cuts
