@@ -262,9 +262,9 @@ int llmrs_kv8_read(llmrs_ctx *ctx, const llmrs_kv8 *cache, const int *d_pages, i
  * tables: it is not).  scale multiplies q.k (0: 1/sqrt(head_dim)).  f32 rows are
  * computed to f32 accuracy (against the row's largest values, where the value scales
  * of pages lie further apart than 2^15), f16 rows too, up to the rounding of the result.
- * bf16 rows: the rotated q and the probabilities are rounded to 11 bits once, and the
- * result to bf16's 8; its 2-norm error against 64 bits is 3 to 8 % above that of the
- * result's rounding alone.  A row for which no page can be read gets zeros.  d_workspace: llmrs_kv8_attention_workspace
+ * bf16 rows: the probabilities are rounded to 11 bits once, which the rounding of the
+ * result to bf16's 8 hides (2-norm error against 64 bits: that of the result's rounding
+ * alone, to 0.1 %).  A row for which no page can be read gets zeros.  d_workspace: llmrs_kv8_attention_workspace
  * bytes (which depend on the sizes only), 16-byte aligned, contents irrelevant; NULL: the
  * context's scratch (not while capturing, and not by calls that may run at the same
  * time on several streams). */

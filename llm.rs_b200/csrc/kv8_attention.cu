@@ -18,11 +18,13 @@
 // split into two f16 pieces (22 bits and more), the pieces are columns of
 // their own in the same instruction, so one pass over the codes serves both.
 // f16 rows are split too: with one piece each, the roundings of q and P put
-// 3.4e-4 on the result where rounding the result itself costs 2.1e-4.  bf16 rows
-// have one piece of 11 bits each: the result's own rounding to 8 bits is 1.66e-3 in
-// 2-norm, and with q's and P's 1.71e-3 (64 ragged sequences 1.74e-3, one of 131000
-// tokens 1.69e-3 to 1.83e-3); two pieces bring back 1.66e-3 and take 85 us where one
-// takes 65 (one of 131000 tokens, 64 heads over 8).
+// 3.4e-4 on the result where rounding the result itself costs 2.1e-4.  bf16 rows:
+// two pieces of the rotated q, whose errors a sharp head's softmax multiplies, and
+// one of P, 11 bits to the result's 8.  q's small pieces are not columns of their own
+// but multiplied into the same sums.  One sequence of 131000 tokens, 64 heads over 8,
+// 2-norm error and time: 1.68e-3, the rounding of the result alone, and 70 us; with
+// one piece of q 1.69e-3 to 1.83e-3 (scores of some tens: several times the rounding)
+// and 65 us; with both of P in columns too 1.68e-3 and 85 us.
 //
 // Work: the tiles of all (sequence, vector group, KV head) pairs in one row,
 // cut into equal ranges, one per warp, whatever the lengths.  A warp streams
@@ -37,7 +39,7 @@
 //
 // 64 sequences of 37 to 8192 tokens, f32, 32 heads of 128 over 8: 105 us here and 6
 // in the join for 542 MB (83 us at the memory's rate).  131000 tokens, bf16, 64 heads
-// over 8: 53 and 10 us for 268 MB (41).  A launch without work takes 8 us: finding
+// over 8: 58 and 10 us for 268 MB (41).  A launch without work takes 8 us: finding
 // the range, the pages, their scales and q, each a trip to memory.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -75,16 +77,26 @@ struct __align__(16) Tile {
 };
 static_assert(sizeof(Tile) == 48, "three 16-byte words");
 
-template <int D, int NT>
+// whether q's small pieces, where they go into the sums of the large ones, lie in shared
+// memory: 16 columns of 128 dims and both pieces do not fit the registers
+template <int D, bool SPLIT, int NT>
+constexpr bool q_low_shared()
+{
+    return !SPLIT && NT == 2 && D == 128;
+}
+
+template <int D, bool SPLIT, int NT>
 struct FewLay {
     static constexpr int FW = few_warps(NT);
-    static constexpr int STAGES = (NT == 1 ? 2 : 3) * (128 / D);
+    static constexpr bool QLS = q_low_shared<D, SPLIT, NT>();
+    static constexpr int STAGES = (NT == 1 || QLS ? 2 : 3) * (128 / D);
     static constexpr int BOX = FT * D;            // bytes of K or V codes of a tile
     static constexpr int RING = STAGES * 2 * BOX; // per warp
     static constexpr int BATCH = 32;              // tile records made at a time
     static constexpr int TILES = BATCH + 16;      // and held per warp
     static constexpr int tile_off = FW * RING;
-    static constexpr int bar_off = tile_off + FW * TILES * (int)sizeof(Tile);
+    static constexpr int ql_off = tile_off + FW * TILES * (int)sizeof(Tile);
+    static constexpr int bar_off = ql_off + (QLS ? FW * NT * D * 16 : 0);
     static constexpr int bytes = bar_off + FW * STAGES * 16 + 1024; // + alignment slack
     static_assert(bytes <= 232448 - 1024, "shared memory of one CTA, beside the static part");
 };
@@ -139,11 +151,12 @@ __device__ __forceinline__ long long seq_tiles(const FewParams &p, int n, int le
     return (long long)tiles * groups * p.a.c.n_kv;
 }
 
-// T: type of the rows; SPLIT: two f16 pieces per value (f32 rows); NT: columns / 8
+// T: type of the rows; SPLIT: both pieces of q and P are columns of their own, in place of q's
+// small pieces being multiplied into the sums of the large ones (bf16 rows); NT: columns / 8
 template <class T, int D, bool SPLIT, int NT>
 __global__ void __launch_bounds__(few_warps(NT) * 32, 1) kv8_few_kernel(const __grid_constant__ FewParams p)
 {
-    using Lay = FewLay<D, NT>;
+    using Lay = FewLay<D, SPLIT, NT>;
     constexpr int FW = Lay::FW;
     constexpr int GV = group_vectors<SPLIT, NT>();
     constexpr int KS = D / 16;    // k steps of q.k
@@ -345,6 +358,8 @@ __global__ void __launch_bounds__(few_warps(NT) * 32, 1) kv8_few_kernel(const __
 
     // ---- the pair in progress
     uint32_t qf[NT][KS][2];     // q as B fragments
+    uint2 ql[NT][SPLIT || Lay::QLS ? 1 : KS]; // its small pieces, here or
+    uint2 *qls = reinterpret_cast<uint2 *>(smem + Lay::ql_off) + warp * NT * KS * 32 + lane; // [column tile][k step][lane]
     float acc[MT][NT][4];       // O^T: (dim row gl / gl+8, column 2t4 / 2t4+1)
     float m[NT][2], l[NT][2], fac[NT][2];
     int lim[NT][2];             // last position the column's row attends to
@@ -396,18 +411,21 @@ __global__ void __launch_bounds__(few_warps(NT) * 32, 1) kv8_few_kernel(const __
             e = max(-126, min(126, e));
             const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
-            for (int k = 0; k < KS; k++)
+            for (int k = 0; k < KS; k++) {
+                uint32_t low[2];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const float x0 = q[4 * k + 2 * h] * down, x1 = q[4 * k + 2 * h + 1] * down;
                     const uint32_t w = pack16(x0, x1);
-                    if constexpr (SPLIT) {
-                        const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-                        qf[j][k][h] = gl < 4 ? w : pack16(x0 - r.x, x1 - r.y);
-                    } else {
-                        qf[j][k][h] = w;
-                    }
+                    const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+                    low[h] = pack16(x0 - r.x, x1 - r.y);
+                    qf[j][k][h] = SPLIT && gl >= 4 ? low[h] : w;
                 }
+                if constexpr (Lay::QLS) // read back by this lane alone
+                    qls[(j * KS + k) * 32] = make_uint2(low[0], low[1]);
+                else if constexpr (!SPLIT)
+                    ql[j][k] = make_uint2(low[0], low[1]);
+            }
             const float f = up * a.scale * 1.4426950408889634f; // scores in powers of two
             const int pos = live ? x.len + row : -1;
 #pragma unroll
@@ -470,7 +488,15 @@ __global__ void __launch_bounds__(few_warps(NT) * 32, 1) kv8_few_kernel(const __
                     const uint32_t a1 = codes_f16(x1, 0x4140), a3 = codes_f16(x1, 0x4342);
 #pragma unroll
                     for (int j = 0; j < NT; j++) {
-                        if (u == 0 && k == 0)
+                        const bool first = u == 0 && k == 0;
+                        if constexpr (!SPLIT) {
+                            const uint2 b = Lay::QLS ? qls[(j * KS + 4 * u + k) * 32] : ql[j][Lay::QLS ? 0 : 4 * u + k];
+                            if (first)
+                                mma16816_first(s[mt][j], a0, a1, a2, a3, b.x, b.y);
+                            else
+                                mma16816(s[mt][j], a0, a1, a2, a3, b.x, b.y);
+                        }
+                        if (SPLIT && first)
                             mma16816_first(s[mt][j], a0, a1, a2, a3, qf[j][0][0], qf[j][0][1]);
                         else
                             mma16816(s[mt][j], a0, a1, a2, a3, qf[j][4 * u + k][0], qf[j][4 * u + k][1]);
@@ -747,7 +773,7 @@ int run_few(const FewParams &p, int ctas, cudaStream_t stream)
 {
     constexpr int GV = group_vectors<SPLIT, NT>();
     constexpr int FW = few_warps(NT);
-    LLMRS_CUDA_TRY(launch(kv8_few_kernel<T, D, SPLIT, NT>, dim3(ctas), dim3(FW * 32), FewLay<D, NT>::bytes, stream,
+    LLMRS_CUDA_TRY(launch(kv8_few_kernel<T, D, SPLIT, NT>, dim3(ctas), dim3(FW * 32), FewLay<D, SPLIT, NT>::bytes, stream,
                           p.many != INT32_MAX, p));
     LLMRS_CUDA_TRY(launch(kv8_join_kernel<T, D, GV>, dim3(4 * ctas), dim3(JT), 0, stream, true, p.a,
                           (const float *)p.part, (const JoinHead *)p.head, ctas * FW));
@@ -772,7 +798,7 @@ template <class T, bool SPLIT, int D, int NT>
 cudaError_t prepare_few()
 {
     return cudaFuncSetAttribute(kv8_few_kernel<T, D, SPLIT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                FewLay<D, NT>::bytes);
+                                FewLay<D, SPLIT, NT>::bytes);
 }
 
 template <class T, bool SPLIT>
@@ -805,8 +831,9 @@ long long mean_vectors(int rep, int n_rows, int n_seqs)
 // A sequence with more vectors per KV head than this goes to the kernel for many
 // rows: three groups here cost what its tile of 128 rows costs whatever it holds.
 // 16 sequences of 300 to 4000 tokens, heads of 128, f32 rows: 16 vectors 68 us
-// here, 88 there, 32 vectors 109 and 90; bf16 rows: 32 vectors 72 and 79, 48
-// vectors 93 and 82; heads of 64 cross at the same places.
+// here, 88 there, 32 vectors 109 and 90; bf16 rows, both kernels launched: 16 vectors 57
+// and 64, 32 vectors 75 and 66, 48 vectors 95 and 68, but sequences of 4 to 36 vectors
+// side by side 68, and 78 with a border at 32; heads of 64 cross at the same places.
 constexpr int many_from(int dtype) { return 3 * (dtype == LLMRS_BF16 ? 16 : 8); }
 
 // whether a sequence may have that many: with no more rows than sequences (a

@@ -6,11 +6,13 @@
 // f16 operands, f32 accumulators in TMEM.  The codes are exact in f16.  f32
 // rows: Q and P are two f16 pieces each (22 bits and more), so the products
 // run twice; f16 rows too (with P in one piece they are 1.4 times as far off as
-// the rounding of the result); bf16 rows: one each, of 11 bits, which leaves the
-// result's 2-norm error at 1.72e-3 where its own rounding to 8 bits makes 1.66e-3
-// (two pieces: 1.66e-3, and 615 us for the two prompts below).  Every tile's O is
-// a fresh product that registers add up in f32, with the change of the maximum
-// applied there: long sums do not pass through the tensor core's accumulator.
+// the rounding of the result); bf16 rows: two of Q, whose errors a sharp head's
+// softmax multiplies, and one of P, 11 bits to the result's 8 (2-norm error 1.68e-3,
+// the rounding of the result alone; with one of Q 1.72e-3, and several times the
+// rounding where scores reach some tens, in 475 us for the two prompts below; with two
+// of P 615 us).  Every tile's O is a fresh product that registers add up in f32,
+// with the change of the maximum applied there: long sums do not pass through the
+// tensor core's accumulator.
 //
 // Warpgroups: 0 and 4 softmax of every other tile (thread = row), 1 output
 // (thread = row, D accumulators), 2 and 5 key and value codes to f16 in shared
@@ -24,15 +26,15 @@
 // tile i - 1 runs and the scores of tile i + 2 are made.  K and V are double
 // buffered, Q too but for two pieces of 128 dims.
 //
-// What a tile costs is not its products' 1000 cycles but the roles' chains, whose
+// What a tile costs is not its products' 1000 to 2000 cycles but the roles' chains, whose
 // instructions take 4 to 5 cycles each: so each role that was the longest got a
 // second warpgroup or a kernel of its own, and each keeps its next loads (TMEM
 // columns, codes) in flight while it works.  Two prompts of 3500 to 4096 rows,
-// bf16, 32 heads of 128 over 8: 475 us (515 TFLOP/s; 740 us with one softmax, one
-// widening and one Q warpgroup), chunks of 3 prompts of 1000 rows behind 0 to 3000
-// tokens, f32: 267 us.  Left: 3400 to 3900 cycles a tile, spread over all roles:
-// of 493 us (an earlier build) 394 stayed without any softmax, 454 without
-// widening, 471 without the output's sums.
+// bf16, 32 heads of 128 over 8: 523 us (468 TFLOP/s; with one piece of Q 475, and
+// 740 with one softmax, one widening and one Q warpgroup), chunks of 3 prompts of
+// 1000 rows behind 0 to 3000 tokens, f32: 267 us.  Left: 3400 to 3900 cycles a tile,
+// spread over all roles: of 493 us (an earlier build, one piece of Q) 394 stayed
+// without any softmax, 454 without widening, 471 without the output's sums.
 //
 // Work: the tiles of all (sequence, KV head, tile of rows) in one row, cut into
 // equal consecutive ranges, one per CTA; pieces of a softmax that a range cuts
@@ -63,7 +65,7 @@ struct ManyTile {
     float lvs[8];                // log2 of them, rounded up (-inf: zero)
     int first, last, masked;     // of the pair within this range; some row does not see all tokens
     int tile;                    // of tokens
-    int pad0;                    // g at 8 of 16 bytes: at 4 the kernel spills 76 bytes, not 16 (two prompts 511 us, 482 so)
+    int pad0;                    // g at 8 of 16 bytes: at 4 the kernel spills 76 bytes, not 16 (7 %)
     int g, mt;                   // KV head, tile of rows
     int r0, n, len;              // of the sequence
     int from_start, to_end, pieces;
@@ -1034,9 +1036,9 @@ int kv8_many_prepare(void)
     if (e == cudaSuccess)
         e = prepare<__half, 64, 2, 2>();
     if (e == cudaSuccess)
-        e = prepare<__nv_bfloat16, 128, 1, 1>();
+        e = prepare<__nv_bfloat16, 128, 2, 1>();
     if (e == cudaSuccess)
-        e = prepare<__nv_bfloat16, 64, 1, 1>();
+        e = prepare<__nv_bfloat16, 64, 2, 1>();
     if (e != cudaSuccess)
         return fail(LLMRS_ECUDA, "kv8 kernel attributes: %s", cudaGetErrorString(e));
     return LLMRS_OK;
@@ -1056,8 +1058,8 @@ int kv8_many(const Kv8Attn &a, int many, void *ws, int sms, cudaStream_t stream)
         return a.c.D == 128 ? run<float, 128, 2, 2>(p, ctas, stream) : run<float, 64, 2, 2>(p, ctas, stream);
     if (a.dtype == LLMRS_F16)
         return a.c.D == 128 ? run<__half, 128, 2, 2>(p, ctas, stream) : run<__half, 64, 2, 2>(p, ctas, stream);
-    return a.c.D == 128 ? run<__nv_bfloat16, 128, 1, 1>(p, ctas, stream)
-                        : run<__nv_bfloat16, 64, 1, 1>(p, ctas, stream);
+    return a.c.D == 128 ? run<__nv_bfloat16, 128, 2, 1>(p, ctas, stream)
+                        : run<__nv_bfloat16, 64, 2, 1>(p, ctas, stream);
 }
 
 } // namespace llmrs
