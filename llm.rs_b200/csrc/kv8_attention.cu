@@ -22,9 +22,9 @@
 // two pieces of the rotated q, whose errors a sharp head's softmax multiplies, and
 // one of P, 11 bits to the result's 8.  q's small pieces are not columns of their own
 // but multiplied into the same sums.  One sequence of 131000 tokens, 64 heads over 8,
-// 2-norm error and time: 1.68e-3, the rounding of the result alone, and 70 us; with
-// one piece of q 1.69e-3 to 1.83e-3 (scores of some tens: several times the rounding)
-// and 65 us; with both of P in columns too 1.68e-3 and 85 us.
+// 2-norm error and time: 1.64e-3 to 1.69e-3 by the input, the rounding of the result
+// alone, and 70 us; with one piece of q 1.69e-3 to 1.83e-3 (scores of some tens: several
+// times the rounding) and 65 us; with both of P in columns too as now and 85 us.
 //
 // Work: the tiles of all (sequence, vector group, KV head) pairs in one row,
 // cut into equal ranges, one per warp, whatever the lengths.  A warp streams

@@ -7,12 +7,13 @@
 // rows: Q and P are two f16 pieces each (22 bits and more), so the products
 // run twice; f16 rows too (with P in one piece they are 1.4 times as far off as
 // the rounding of the result); bf16 rows: two of Q, whose errors a sharp head's
-// softmax multiplies, and one of P, 11 bits to the result's 8 (2-norm error 1.68e-3,
-// the rounding of the result alone; with one of Q 1.72e-3, and several times the
-// rounding where scores reach some tens, in 475 us for the two prompts below; with two
-// of P 615 us).  Every tile's O is a fresh product that registers add up in f32,
-// with the change of the maximum applied there: long sums do not pass through the
-// tensor core's accumulator.
+// softmax multiplies, and one of P, 11 bits to the result's 8.  The two prompts below,
+// 2-norm error and time: 1.66e-3, the rounding of the result alone, and 530 us; with
+// value scales' mantissas in P 1.67e-3 and 523 us, with one piece of Q too 1.72e-3 (and
+// several times the rounding where scores reach some tens) and 475; with two of P 1.66e-3
+// and 615.  Every tile's O is a fresh product that registers add up in f32, with the
+// change of the maximum applied there: long sums do not pass through the tensor core's
+// accumulator.
 //
 // Warpgroups: 0 and 4 softmax of every other tile (thread = row), 1 output
 // (thread = row, D accumulators), 2 and 5 key and value codes to f16 in shared
@@ -30,7 +31,7 @@
 // instructions take 4 to 5 cycles each: so each role that was the longest got a
 // second warpgroup or a kernel of its own, and each keeps its next loads (TMEM
 // columns, codes) in flight while it works.  Two prompts of 3500 to 4096 rows,
-// bf16, 32 heads of 128 over 8: 523 us (468 TFLOP/s; with one piece of Q 475, and
+// bf16, 32 heads of 128 over 8: 530 us (462 TFLOP/s; with one piece of Q 475, and
 // 740 with one softmax, one widening and one Q warpgroup), chunks of 3 prompts of
 // 1000 rows behind 0 to 3000 tokens, f32: 267 us.  Left: 3400 to 3900 cycles a tile,
 // spread over all roles: of 493 us (an earlier build, one piece of Q) 394 stayed
@@ -449,7 +450,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                 fac = live ? p.facs[(size_t)(x.r0 + row) * a.n_heads + x.g * rep + r % rep] : 0.0f;
             }
             float top = -INFINITY, sum = 0.0f;
-            int shift = 0; // P is p * vs * 2^shift
+            int shift = 0; // P is p * vs * 2^shift / unit
+            float unit = 1.0f;
             if (busy) {
                 const bool masked = x.masked;
                 if (masked) { // S becomes the scores themselves, the unseen ones at -inf
@@ -483,6 +485,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                     }
                     t0 = fmaxf(t0, t1) * (masked ? 1.0f : f * x.ks[g]); // the factor is not negative
                     top = fmaxf(top, t0);
+                    if constexpr (PP == 1)
+                        unit = t0 + x.lvs[g] > ref2 ? x.vs[g] : unit;
                     ref2 = fmaxf(ref2, t0 + x.lvs[g]);
                 };
                 { // the next columns are on their way meanwhile
@@ -503,6 +507,13 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                 // whatever the scales of pages that the row hardly sees.  p and vs are f32
                 // factors, not one power of two, so P and the sum share p's rounding.
                 const float ref = top == -INFINITY ? 0.0f : top;
+                // P in one piece: the mantissa of the largest's scale goes back in with the output, so
+                // that tokens of its pages have P = p * 2^n and a probability of one is exact
+                float inv = 1.0f;
+                if constexpr (PP == 1) {
+                    unit = __uint_as_float((__float_as_uint(unit) & 0x7fffffu) | 0x3f800000u);
+                    inv = __frcp_rn(unit);
+                }
                 if (ref2 > -INFINITY) // some seen page has a scale above 0
                     shift = (int)fminf(fmaxf(P_SCALE_LOG2 - ceilf(ref2 - ref), -126.0f), 126.0f);
                 auto probabilities = [&](int g, const uint32_t *s) { // 16 of them, over the scores of group g
@@ -510,7 +521,11 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
                     // largest), 2^up goes to p
                     const float up = fmaxf(x.lvs[g] + (float)(shift - 60), 0.0f);
                     const float kf = masked ? 1.0f : f * x.ks[g], add = up - ref;
-                    const float by = x.vs[g] * exp2i(shift - (int)up);
+                    float by = x.vs[g] * exp2i(shift - (int)up);
+                    if constexpr (PP == 1) { // by / unit, rounded once
+                        const float q = by * inv;
+                        by = fmaf(fmaf(-q, unit, by), inv, q);
+                    }
                     float2 g01 = make_float2(0.0f, 0.0f);
                     uint32_t ph[8], pl[8];
 #pragma unroll
@@ -550,7 +565,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv8_many_kernel(const __grid_
             }
             float *hand = ring + (i % RING) * 3 * MB;
             hand[r] = top;
-            hand[MB + r] = exp2i(-shift);
+            hand[MB + r] = exp2i(-shift) * unit;
             hand[2 * MB + r] = sum;
             tc_before();
             mbar_arrive(&bar[B_P_FULL + i % NS]);
